@@ -27,6 +27,7 @@ extern "C" {
 /* element type of the 16-bit tensors */
 #define NA1D_BF16 0 /* replaces the bf16_ana1d module, na1d_tensorcore/nattn.py:12-20 */
 #define NA1D_FP16 1 /* replaces the fp16_ana1d module, na1d_tensorcore/nattn.py:21-29 */
+#define NA1D_FP32 2 /* rows and weight of a head (na1d_head) only */
 
 /* status codes */
 #define NA1D_OK 0
@@ -42,6 +43,8 @@ extern "C" {
 #define NA1D_ERR_UNSUPPORTED (-10)   /* the requested kernel family / tiling cannot run this shape */
 #define NA1D_ERR_BAD_DROPOUT (-12)   /* dropout probability outside [0,1) */
 #define NA1D_ERR_BAD_STRIDE (-11)    /* a stride is not a positive multiple of 8 elements, or the token stride is below C */
+
+#define NA1D_ERR_BAD_SCALE (-13)     /* a scale or temperature is not positive and finite, or a margin where there is none */
 
 #define NA1D_MAX_WINDOW 128 /* the reference asserts win <= 80, models/PCF_NATransformer.py:53 */
 
@@ -296,6 +299,56 @@ int na1d_stats_pool_forward(float* out, float* stats, const void* logits, const 
 int na1d_stats_pool_backward(void* d_logits, void* dx, const float* d_out, const float* out, const float* stats,
                              const void* logits, const void* x, int64_t N, int64_t T, int64_t C,
                              float floor, int dtype, void* stream);
+
+/* ------------------------------------------------------------------------------------------
+ * Losses of a classification head whose (rows, classes) logits are never stored: softmax cross entropy of z = scale x w^T, the same on
+ * scaled cosines with an additive angular margin on the label's (what models/PCF_NATransformer.py feeds AAM-softmax with), and the
+ * Kullback-Leibler divergence from a teacher of whose logits the top ones are known.
+ *
+ *   top == 0:  loss_i = log sum_v exp z_iv - z_iy, y = labels[i]; rows with labels[i] == ignore_index do not count. normalize: z is scale
+ *              times the cosine, and the label's scale cos(angle + margin), cos a cos m - sqrt(max(1 - cos^2 a, 2e-7)) sin m.
+ *   top == k:  q = softmax over the entries j of row i with teacher_index >= 0 of teacher_logits / temperature, p = softmax over all classes of
+ *              z / temperature; loss_i = temperature^2 sum_j q_j (log q_j - log p_(index j)). Rows without an entry (or with nothing but
+ *              logits of -infinity) do not count. A class may come twice.
+ * A label or entry that is no class makes its row's loss, and what depends on it, NaN; nothing is read outside the tensors. A row or class
+ * of zeros has no direction: its cosines are 0 and its gradient is. The mean is over rows that count, and 0 where none does.
+ *
+ * Products are of 16-bit values (dtype) with sums in fp32; fp32 rows or weights are rounded to dtype first, and their gradients are fp32. The
+ * gradient of the logits is rounded to dtype once, before its products with weight and rows; everything else is held in fp32. No atomics
+ * on results: the same bits from run to run. Nothing of a row that does not count is read by a product.
+ * ---------------------------------------------------------------------------------------- */
+#define NA1D_HEAD_MEAN 0
+#define NA1D_HEAD_SUM 1
+#define NA1D_HEAD_NONE 2
+#define NA1D_HEAD_MAX_ROWS (1 << 22)
+#define NA1D_HEAD_MAX_DIM (1 << 14)
+#define NA1D_HEAD_MAX_CLASSES (1 << 24)
+#define NA1D_HEAD_MAX_TOP 1024
+typedef struct {
+    int64_t rows, dim, classes, top;   /* top: entries of the teacher a row, 0 for labels */
+    const void* x;                     /* (rows, dim), x_stride elements from row to row */
+    int64_t x_stride;
+    const void* weight;                /* (classes, dim), weight_stride elements from row to row */
+    int64_t weight_stride;
+    const int64_t* labels;             /* (rows); top == 0 */
+    const float* teacher_logits;       /* (rows, top) dense; top > 0 */
+    const int64_t* teacher_index;      /* (rows, top) dense, negative: no entry */
+    int64_t ignore_index;
+    float scale, margin, temperature;
+    int normalize, reduction;
+    int dtype;                         /* NA1D_BF16 or NA1D_FP16: type of the products */
+    int x_type, weight_type;           /* dtype or NA1D_FP32 */
+} na1d_head;
+/* Bytes of the buffers below (negative: status code); host-only. */
+int64_t na1d_head_saved_bytes(const na1d_head* head);
+int64_t na1d_head_forward_scratch(const na1d_head* head);
+int64_t na1d_head_backward_scratch(const na1d_head* head, int want_x, int want_weight);
+/* loss: (rows) with NA1D_HEAD_NONE, else one number. saved (256-byte aligned): kept for the backward pass; scratch (256-byte aligned): free
+ * when the call's work is done. */
+int na1d_head_forward(const na1d_head* head, float* loss, void* saved, void* scratch, void* stream);
+/* d_x (rows, dim) and d_weight (classes, dim), dense, of x_type and weight_type, 16-byte aligned; either may be NULL. d_loss as loss. The
+ * weight (and nothing else of the forward's inputs) is read again; saved is only read, so passes over it may overlap. */
+int na1d_head_backward(const na1d_head* head, void* d_x, void* d_weight, const float* d_loss, void* saved, void* scratch, void* stream);
 
 /* ------------------------------------------------------------------------------------------
  * Window index arithmetic as the kernels compute it, for bit-exact checking:

@@ -14,6 +14,7 @@ HEADER = os.path.join(ROOT, "include", "na1d_b200.h")
 
 NA1D_BF16 = 0
 NA1D_FP16 = 1
+NA1D_FP32 = 2
 
 
 class Na1dError(RuntimeError):
@@ -119,6 +120,26 @@ for _name, _args in (
     _f = getattr(_lib, _name)
     _f.restype = _i32
     _f.argtypes = _args + [_i32, _ptr]
+
+
+class Head(ctypes.Structure):
+    """na1d_head of the header."""
+    _fields_ = [("rows", _i64), ("dim", _i64), ("classes", _i64), ("top", _i64), ("x", _ptr), ("x_stride", _i64), ("weight", _ptr),
+                ("weight_stride", _i64), ("labels", _ptr), ("teacher_logits", _ptr), ("teacher_index", _ptr), ("ignore_index", _i64),
+                ("scale", _f32), ("margin", _f32), ("temperature", _f32), ("normalize", _i32), ("reduction", _i32), ("dtype", _i32),
+                ("x_type", _i32), ("weight_type", _i32)]
+
+
+_lib.na1d_head_saved_bytes.restype = _i64
+_lib.na1d_head_saved_bytes.argtypes = [_ptr]
+_lib.na1d_head_forward_scratch.restype = _i64
+_lib.na1d_head_forward_scratch.argtypes = [_ptr]
+_lib.na1d_head_backward_scratch.restype = _i64
+_lib.na1d_head_backward_scratch.argtypes = [_ptr, _i32, _i32]
+_lib.na1d_head_forward.restype = _i32
+_lib.na1d_head_forward.argtypes = [_ptr] * 5
+_lib.na1d_head_backward.restype = _i32
+_lib.na1d_head_backward.argtypes = [_ptr] * 7
 _lib.na1d_tensor_map_cache_stats.restype = _i32
 _lib.na1d_tensor_map_cache_stats.argtypes = [_ptr, _ptr]
 _lib.na1d_set_kernel_family.restype = _i32

@@ -1,6 +1,7 @@
 // C ABI of the library: argument validation, kernel-family choice, launches. No torch types.
 #include "../../include/na1d_b200.h"
 #include "na1d_internal.h"
+#include "na1d_head.cuh"
 
 #include <atomic>
 #include <climits>
@@ -17,6 +18,10 @@ int cuda_status(cudaError_t e) {
     g_last_cuda_error = (int)e;
     return NA1D_ERR_CUDA;
 }
+
+}  // namespace
+int na1d::api_cuda_status(cudaError_t e) { return cuda_status(e); }
+namespace {
 
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
@@ -227,6 +232,7 @@ const char* na1d_status_string(int status) {
         case NA1D_ERR_UNSUPPORTED: return "the requested kernel family or tiling does not support this shape";
         case NA1D_ERR_BAD_DROPOUT: return "bad dropout probability: need 0 <= p < 1";
         case NA1D_ERR_BAD_STRIDE: return "bad stride: element strides must be positive multiples of 8, the token stride >= C";
+        case NA1D_ERR_BAD_SCALE: return "bad scale: scale and temperature have to be positive and finite, a margin needs normalised rows and labels";
         default: return "unknown status";
     }
 }
@@ -366,7 +372,7 @@ int na1d_tensor_map_cache_stats(int64_t* hits, int64_t* misses) {
 
 int na1d_device_status(void) {
     // every word is read (and cleared) before anything is reported; an expired wait in any kernel wins over a failed read
-    const int words[11] = {na1d::mlp_read_status(), na1d::mlp_bwd_read_status(), na1d::wgrad_read_status(), na1d::tc_read_status(), na1d::tc_bwd_read_status(), na1d::tc_seg_read_status(),
+    const int words[13] = {na1d::head::logits_read_status(), na1d::head::grad_read_status(), na1d::mlp_read_status(), na1d::mlp_bwd_read_status(), na1d::wgrad_read_status(), na1d::tc_read_status(), na1d::tc_bwd_read_status(), na1d::tc_seg_read_status(),
                           na1d::tc_bwd_seg_read_status(), na1d::tc_unfused_read_status(), na1d::tc_unfused_t_read_status(),
                           na1d::tc_drop_read_status(), na1d::tc_bwd_drop_read_status()};
     int v = 0, w = 0;

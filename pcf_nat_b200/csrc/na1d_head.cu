@@ -1,0 +1,227 @@
+// C ABI of the losses of a classification head: checks of the arguments, where the pieces lie in the caller's buffers, order of the passes.
+#include "na1d_head.cuh"
+
+#include <climits>
+#include <cmath>
+
+namespace na1d {
+namespace head {
+
+Shape shape_of(const na1d_head& h) {
+    Shape s = {};
+    s.N = h.rows; s.D = h.dim; s.V = h.classes; s.k = h.top;
+    s.Np = round_up(s.N, kTile);
+    s.Dp = round_up(s.D, 8);
+    s.parts = (s.V + kTile - 1) / kTile * (kTile / kPart);
+    s.x_stride = h.x_stride; s.w_stride = h.weight_stride;
+    s.norm = h.normalize != 0;
+    // the weight is read where it is if TMA can: 16-bit rows on 16-byte boundaries
+    s.copy_w = h.weight_type != h.dtype || h.weight_stride % 8 != 0 || h.weight_stride < s.D || (reinterpret_cast<uintptr_t>(h.weight) & 15) != 0;
+    s.cs = kLog2e * h.scale / (s.k ? h.temperature : 1.f);
+    return s;
+}
+
+Saved saved_at(const na1d_head& h, const Shape& s, void* base) {
+    Saved v = {};
+    int64_t at = 0;
+    auto take = [&](int64_t bytes) {
+        uint8_t* p = static_cast<uint8_t*>(base) + at;   // (with base null: sizes alone)
+        at += round_up(bytes, 256);
+        return static_cast<void*>(p);
+    };
+    v.words = static_cast<Words*>(take(sizeof(Words)));
+    v.place = static_cast<int*>(take(s.N * 4));
+    v.row = static_cast<int*>(take(s.Np * 4));
+    v.lse2 = static_cast<float*>(take(s.Np * 4));
+    if (s.norm) {
+        v.ix = static_cast<float*>(take(s.Np * 4));
+        v.iw = static_cast<float*>(take(round_up(s.V, kTile) * 4));
+    }
+    if (s.k) {
+        v.q = static_cast<float*>(take(s.N * s.k * 4));
+        v.q_all = static_cast<float*>(take(s.N * s.k * 4));
+        v.index = static_cast<int*>(take(s.N * s.k * 4));
+        v.entry = static_cast<float*>(take(s.N * s.k * 4));
+    } else {
+        v.target = static_cast<int*>(take(s.Np * 4));
+        v.slope = static_cast<float*>(take(s.Np * 4));
+    }
+    v.x = take(s.Np * s.Dp * 2);
+    if (s.copy_w) v.w = take(s.V * s.Dp * 2);
+    v.bytes = at;
+    return v;
+}
+
+// A piece of the classes has gradients of at most kPieceBytes, so that they are still in L2 (or nearly) when the products read them, and
+// at least four tiles, below which the sums over pieces would cost more than the products.
+constexpr int64_t kPieceBytes = 96ll << 20;
+Pieces pieces_of(const Shape& s, bool want_x, bool want_w) {
+    Pieces p = {};
+    const int64_t pairs = device_sm_count() / 2;
+    p.tiles = (s.V + kTile - 1) / kTile;
+    int64_t most = kPieceBytes / (s.Np * kTile * 2);
+    most = most < 4 ? 4 : most;
+    p.count = (p.tiles + most - 1) / most;
+    p.piece_tiles = (p.tiles + p.count - 1) / p.count;
+    p.count = (p.tiles + p.piece_tiles - 1) / p.piece_tiles;
+    p.pitch = p.piece_tiles * kTile;
+    p.d_tiles = (int)((s.D + kTile - 1) / kTile);
+    p.d_width = (int)round_up((s.D + p.d_tiles - 1) / p.d_tiles, 32);
+    // splits of the contractions: about as many steps to an item as a pair has in all
+    const int64_t steps_x = p.pitch / 64, steps_w = s.Np / 64;
+    const int64_t items_x = want_x ? s.Np / kTile * p.d_tiles : 0, items_w = want_w ? p.piece_tiles * p.d_tiles : 0;
+    int64_t share = (items_x * steps_x + items_w * steps_w + pairs - 1) / pairs;
+    share = share < 8 ? 8 : share;
+    auto splits = [&](int64_t steps, int64_t most_splits) {
+        int64_t n = (steps + share - 1) / share;
+        n = n > most_splits ? most_splits : n;
+        return (int)(n < 1 ? 1 : n);
+    };
+    p.splits_x = splits(steps_x, 32);
+    p.splits_w = splits(steps_w, 16);
+    return p;
+}
+
+namespace {
+
+bool type_ok(int t) { return t == NA1D_BF16 || t == NA1D_FP16 || t == NA1D_FP32; }
+bool bad_align(const void* p, int64_t n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) != 0; }
+
+int check(const na1d_head* h) {
+    if (!h) return NA1D_ERR_NULL_POINTER;
+    if (h->dtype != NA1D_BF16 && h->dtype != NA1D_FP16) return NA1D_ERR_BAD_DTYPE;
+    if (!type_ok(h->x_type) || !type_ok(h->weight_type)) return NA1D_ERR_BAD_DTYPE;
+    if ((h->x_type != NA1D_FP32 && h->x_type != h->dtype) || (h->weight_type != NA1D_FP32 && h->weight_type != h->dtype)) return NA1D_ERR_BAD_DTYPE;
+    if (h->rows <= 0 || h->dim <= 0 || h->classes <= 0 || h->top < 0) return NA1D_ERR_BAD_SHAPE;
+    if (h->rows > NA1D_HEAD_MAX_ROWS || h->dim > NA1D_HEAD_MAX_DIM || h->classes > NA1D_HEAD_MAX_CLASSES || h->top > NA1D_HEAD_MAX_TOP) return NA1D_ERR_TOO_LARGE;
+    if (h->x_stride < 0 || h->weight_stride < 0) return NA1D_ERR_BAD_STRIDE;
+    if (h->reduction != NA1D_HEAD_MEAN && h->reduction != NA1D_HEAD_SUM && h->reduction != NA1D_HEAD_NONE) return NA1D_ERR_BAD_SHAPE;
+    if (!(h->scale > 0.f) || !std::isfinite(h->scale) || !std::isfinite(h->margin)) return NA1D_ERR_BAD_SCALE;
+    if (h->top > 0 && (!(h->temperature > 0.f) || !std::isfinite(h->temperature))) return NA1D_ERR_BAD_SCALE;
+    if ((h->top > 0 || !h->normalize) && h->margin != 0.f) return NA1D_ERR_BAD_SCALE;
+    if (!h->x || !h->weight || (h->top ? !h->teacher_logits || !h->teacher_index : !h->labels)) return NA1D_ERR_NULL_POINTER;
+    if (bad_align(h->x, h->x_type == NA1D_FP32 ? 4 : 2) || bad_align(h->weight, h->weight_type == NA1D_FP32 ? 4 : 2) || bad_align(h->labels, 8) ||
+        bad_align(h->teacher_index, 8) || bad_align(h->teacher_logits, 4))
+        return NA1D_ERR_MISALIGNED;
+    return NA1D_OK;
+}
+
+// the forward pass's scratch: partial maxima and sums, the blocks' losses, which rows have a teacher
+struct Forward {
+    float2* part;
+    float* block_sums;
+    int* flags;
+    int64_t bytes;
+};
+Forward forward_at(const Shape& s, void* base) {
+    Forward f = {};
+    int64_t at = 0;
+    auto take = [&](int64_t bytes) {
+        uint8_t* p = static_cast<uint8_t*>(base) + at;
+        at += round_up(bytes, 256);
+        return static_cast<void*>(p);
+    };
+    f.part = static_cast<float2*>(take(s.parts * s.Np * 8));
+    f.block_sums = static_cast<float*>(take((s.N + 31) / 32 * 4));
+    if (s.k) f.flags = static_cast<int*>(take(s.N * 4));
+    f.bytes = at;
+    return f;
+}
+// the backward pass's: gradients of a piece's logits, partial sums of both products, the rows' factors
+struct Backward {
+    void* grad;
+    float *part_x, *part_w, *coef;
+    int64_t bytes;
+};
+Backward backward_at(const na1d_head& h, const Shape& s, const Pieces& p, bool want_x, bool want_w, void* base) {
+    Backward b = {};
+    int64_t at = 0;
+    auto take = [&](int64_t bytes) {
+        uint8_t* q = static_cast<uint8_t*>(base) + at;
+        at += round_up(bytes, 256);
+        return static_cast<void*>(q);
+    };
+    b.grad = take(s.Np * p.pitch * 2);
+    if (want_x) b.part_x = static_cast<float*>(take(p.splits_x * s.Np * s.Dp * 4));
+    if (want_w) b.part_w = static_cast<float*>(take(p.splits_w * p.pitch * s.Dp * 4));
+    if (h.reduction == NA1D_HEAD_NONE) b.coef = static_cast<float*>(take((s.Np + 1) * 4));
+    b.bytes = at;
+    return b;
+}
+#define NA1D_HEAD_TRY(call) \
+    if (cudaError_t e = (call)) return api_cuda_status(e)
+
+int forward(const na1d_head& h, float* loss, void* saved, void* scratch, cudaStream_t st) {
+    bind_primary_context();
+    const Shape s = shape_of(h);
+    const Saved sv = saved_at(h, s, saved);
+    const Forward f = forward_at(s, scratch);
+    const void* w = s.copy_w ? sv.w : h.weight;
+    const int64_t ldw = s.copy_w ? s.Dp : h.weight_stride;
+    NA1D_HEAD_TRY(cudaMemsetAsync(sv.words, 0, sizeof(Words), st));
+    if (s.k) NA1D_HEAD_TRY(teacher(h, s, sv, f.flags, st));
+    NA1D_HEAD_TRY(rows(h, s, sv, f.flags, loss, st));
+    NA1D_HEAD_TRY(weight(h, s, sv, st));
+    if (s.k) NA1D_HEAD_TRY(entries(h, s, sv, w, ldw, st));
+    NA1D_HEAD_TRY(stats(h, s, sv, f.part, w, ldw, st));
+    NA1D_HEAD_TRY(combine(h, s, sv, f.part, f.block_sums, loss, w, ldw, st));
+    return NA1D_OK;
+}
+
+int backward(const na1d_head& h, void* dx, void* dw, const float* d_loss, void* saved, void* scratch, cudaStream_t st) {
+    bind_primary_context();
+    const Shape s = shape_of(h);
+    const Saved sv = saved_at(h, s, saved);
+    const Pieces p = pieces_of(s, dx != nullptr, dw != nullptr);
+    const Backward b = backward_at(h, s, p, dx != nullptr, dw != nullptr, scratch);
+    const void* w = s.copy_w ? sv.w : h.weight;
+    const int64_t ldw = s.copy_w ? s.Dp : h.weight_stride;
+    if (b.coef) NA1D_HEAD_TRY(coefficients(h, s, sv, d_loss, b.coef, st));
+    for (int64_t i = 0; i < p.count; ++i) {
+        const int64_t v0 = i * p.pitch, cols = s.V - v0 < p.pitch ? s.V - v0 : p.pitch;
+        NA1D_HEAD_TRY(gradients(h, s, sv, b.coef, b.grad, p.pitch, v0, (cols + kTile - 1) / kTile, w, ldw, st));
+        if (s.k) NA1D_HEAD_TRY(put_entries(h, s, sv, b.coef, b.grad, p.pitch, v0, cols, st));
+        NA1D_HEAD_TRY(products(h, s, sv, b.grad, p, v0, cols, i > 0, b.part_x, b.part_w, w, ldw, st));
+        const bool last = i + 1 == p.count;
+        if (dw || last)
+            NA1D_HEAD_TRY(finish(h, s, sv, last ? dx : nullptr, dw, b.part_x, b.part_w, d_loss, b.coef, p.splits_x, p.splits_w, v0, cols, p.pitch, w, ldw, st));
+    }
+    return NA1D_OK;
+}
+
+}  // namespace
+}  // namespace head
+}  // namespace na1d
+
+extern "C" {
+
+int64_t na1d_head_saved_bytes(const na1d_head* head) {
+    if (int s = na1d::head::check(head)) return s;
+    const na1d::head::Shape s = na1d::head::shape_of(*head);
+    return na1d::head::saved_at(*head, s, nullptr).bytes;
+}
+int64_t na1d_head_forward_scratch(const na1d_head* head) {
+    if (int s = na1d::head::check(head)) return s;
+    return na1d::head::forward_at(na1d::head::shape_of(*head), nullptr).bytes;
+}
+int64_t na1d_head_backward_scratch(const na1d_head* head, int want_x, int want_weight) {
+    if (int s = na1d::head::check(head)) return s;
+    const na1d::head::Shape s = na1d::head::shape_of(*head);
+    return na1d::head::backward_at(*head, s, na1d::head::pieces_of(s, want_x != 0, want_weight != 0), want_x != 0, want_weight != 0, nullptr).bytes;
+}
+int na1d_head_forward(const na1d_head* head, float* loss, void* saved, void* scratch, void* stream) {
+    if (int s = na1d::head::check(head)) return s;
+    if (!loss || !saved || !scratch) return NA1D_ERR_NULL_POINTER;
+    if (na1d::head::bad_align(saved, 256) || na1d::head::bad_align(scratch, 256) || na1d::head::bad_align(loss, 4)) return NA1D_ERR_MISALIGNED;
+    return na1d::head::forward(*head, loss, saved, scratch, (cudaStream_t)stream);
+}
+int na1d_head_backward(const na1d_head* head, void* d_x, void* d_weight, const float* d_loss, void* saved, void* scratch, void* stream) {
+    if (int s = na1d::head::check(head)) return s;
+    if (!d_loss || !saved || !scratch || (!d_x && !d_weight)) return NA1D_ERR_NULL_POINTER;
+    if (na1d::head::bad_align(saved, 256) || na1d::head::bad_align(scratch, 256) || na1d::head::bad_align(d_x, 16) || na1d::head::bad_align(d_weight, 16) ||
+        na1d::head::bad_align(d_loss, 4))
+        return NA1D_ERR_MISALIGNED;
+    return na1d::head::backward(*head, d_x, d_weight, d_loss, saved, scratch, (cudaStream_t)stream);
+}
+
+}  // extern "C"

@@ -1,0 +1,284 @@
+// Products of a head's rows and weight, s = x w^T, tile by tile on CTA pairs (cta_group::2), that never leave the chip as they are:
+//   stats      a running maximum and sum of 2^z per row, over 128 classes at a time
+//   gradient   the gradient of the logits in 16 bits, p minus the target's, for a piece of the classes
+// A pair takes 256 rows and 256 classes: each CTA stages its 128 rows of x and half of the tile's rows of w by TMA (six stages of 64
+// channels), the leader issues the products, and eight warps of each CTA read the accumulators back, a row per lane and half of the columns,
+// while the next tile's products fill the other half of tensor memory.
+#include "na1d_head.cuh"
+#include "na1d_mlp.cuh"
+
+namespace na1d {
+namespace head {
+namespace {
+
+__device__ int g_head_status = 0;
+
+constexpr int kThreads = 384;                       // warp 0: loads, 1: MMA issue, 2: tensor memory, 4-11: epilogue
+constexpr int kStep = 64, kHalf = 128;
+constexpr int kOperand = kHalf * kStep * 2;         // 16 KB: 128 rows of 64 channels
+constexpr int kStageBytes = 2 * kOperand;
+constexpr int kStages = 6;
+constexpr int kSmem = kStages * kStageBytes + 1024;
+constexpr uint32_t kCols = 512;
+constexpr int kBand = 16;                           // row tiles that are walked together through the classes
+
+struct Barriers {
+    uint64_t full[kStages], empty[kStages], acc_full[2], acc_empty[2];
+    uint32_t tmem;
+    int abort;
+};
+struct Maps { CUtensorMap x, w; };
+struct Args {
+    const Words* words;
+    const int* target;
+    const float *ix, *iw, *lse2, *slope, *coef;
+    float2* part;               // stats: (classes / 128, Np)
+    void* grad;                 // gradient: (Np, pitch)
+    long long Np, pitch;
+    int V, v0, tiles, steps, tail;   // first class and tiles of classes of this launch; stages of a tile, products of 16 channels in the last one
+    float cs;
+    bool fp16;
+};
+
+__device__ __forceinline__ float exp2_fast(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+// tile t: bands of kBand row tiles, in a band the classes outside and its row tiles inside, so that the pairs at work share both operands in L2
+struct Tile { int m, n; };
+__device__ __forceinline__ Tile tile_at(int t, int row_tiles, int tiles) {
+    const int band = t / (kBand * tiles), first = band * kBand, height = min(kBand, row_tiles - first);
+    t -= band * kBand * tiles;
+    return Tile{first + t % height, t / height};
+}
+
+template <typename E, bool GRAD, bool NORM>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) logits_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Args g) {
+    extern __shared__ uint8_t raw[];
+    uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~(uintptr_t)1023);
+    __shared__ Barriers bar;
+    const int warp = ptx::warp_index(), lane = threadIdx.x & 31;
+    const uint32_t rank = pair::cta_rank();
+    const int first = blockIdx.x >> 1, step = gridDim.x >> 1;
+    volatile int* abort_flag = &bar.abort;
+
+    if (warp == 0) {
+        if (lane < kStages) { ptx::mbar_init(&bar.full[lane], 1); ptx::mbar_init(&bar.empty[lane], 1); }
+        else if (lane < kStages + 2) { ptx::mbar_init(&bar.acc_full[lane - kStages], 1); ptx::mbar_init(&bar.acc_empty[lane - kStages], 16); }
+        else if (lane == kStages + 2) bar.abort = 0;
+        ptx::fence_mbar_init();
+    } else if (warp == 1 && lane < 2) {
+        ptx::prefetch_tensormap(lane ? &maps.w : &maps.x);
+    }
+    if (warp == 2) { pair::tmem_alloc(&bar.tmem, kCols); pair::tmem_relinquish(); }
+    ptx::tc_fence_before_sync();
+    __syncthreads();
+    pair::cluster_sync();
+    ptx::tc_fence_after_sync();
+    const uint32_t tmem = bar.tmem;
+    const int counted = g.words->counted, row_tiles = (counted + kTile - 1) / kTile, items = row_tiles * g.tiles;
+
+    if (warp == 0) {
+        if (ptx::elect_one()) {
+            int slot = 0, n = 0;
+            uint32_t phase = 1;   // the first round finds the slots empty
+            bool ok = true;
+            for (int i = first; ok && i < items; i += step) {
+                const Tile t = tile_at(i, row_tiles, g.tiles);
+                const int m = t.m * kTile + rank * kHalf, v = g.v0 + t.n * kTile + rank * kHalf;
+                for (int k = 0; k < g.steps; ++k) {
+                    if (!ptx::mbar_wait_relaxed(&bar.empty[slot], phase) || *abort_flag) { atomicExch(&g_head_status, 1); *abort_flag = 1; ok = false; break; }
+                    const uint32_t full = pair::in_leader(&bar.full[slot]);
+                    uint8_t* s = smem + slot * kStageBytes;
+                    if (rank == 0) ptx::mbar_expect_tx(&bar.full[slot], 2 * kStageBytes);
+                    pair::load_2d(s, &maps.x, full, k * kStep, m);
+                    pair::load_2d(s + kOperand, &maps.w, full, k * kStep, v);
+                    ++n;
+                    if (++slot == kStages) { slot = 0; phase ^= 1; }
+                }
+            }
+            if (!ok && rank == 0)   // loads that are on their way arrive before the CTAs leave
+                for (int j = n - 1; j >= 0 && j >= n - kStages; --j) ptx::mbar_wait(&bar.full[j % kStages], (j / kStages) & 1, 1u << 14);
+        }
+    } else if (warp == 1) {
+        if (rank == 0 && ptx::elect_one()) {
+            constexpr uint32_t idesc = ptx::instr_desc(tc::Fmt<E>::v, 0, 0, 256, kTile);
+            int slot = 0, it = 0;
+            uint32_t phase = 0;
+            bool ok = true;
+            for (int i = first; ok && i < items; i += step, ++it) {
+                const uint32_t d = tmem + (it & 1) * kTile;
+                if (!ptx::mbar_wait(&bar.acc_empty[it & 1], ((it >> 1) & 1) ^ 1) || *abort_flag) { atomicExch(&g_head_status, 2); *abort_flag = 1; break; }
+                ptx::tc_fence_after_sync();
+                for (int k = 0; k < g.steps; ++k) {
+                    if (!ptx::mbar_wait(&bar.full[slot], phase) || *abort_flag) { atomicExch(&g_head_status, 3); *abort_flag = 1; ok = false; break; }
+                    ptx::tc_fence_after_sync();
+                    const uint32_t s = ptx::smem_u32(smem + slot * kStageBytes);
+                    const uint64_t a = pair::k_major(s), b = pair::k_major(s + kOperand);
+                    const int products = k + 1 < g.steps ? kStep / 16 : g.tail;
+#pragma unroll
+                    for (int j = 0; j < kStep / 16; ++j)
+                        if (j < products) pair::mma_ss(d, tc::desc_advance(a, j * 32), tc::desc_advance(b, j * 32), idesc, k > 0 || j > 0);
+                    pair::commit(&bar.empty[slot]);
+                    if (++slot == kStages) { slot = 0; phase ^= 1; }
+                }
+                if (ok) pair::commit(&bar.acc_full[it & 1]);
+            }
+        }
+    } else if (warp >= 4) {
+        const int q = warp & 3, h = (warp - 4) >> 2;   // tensor-memory lanes 32 q .. + 31 (those a warp reaches), half h of the columns
+        const uint32_t lanes = (uint32_t)(q * 32) << 16;
+        const float up = GRAD ? gradient_scale(g.words, g.fp16, NORM) : 1.f;
+        int it = 0;
+        for (int i = first; i < items; i += step, ++it) {
+            const Tile t = tile_at(i, row_tiles, g.tiles);
+            const int c = t.m * kTile + rank * kHalf + q * 32 + lane, v = g.v0 + t.n * kTile + h * kHalf;
+            const bool live = c < counted;
+            const int target = live && g.target ? g.target[c] : kIgnored;
+            // (a row of zeros has no direction: its products are 0 whatever they are multiplied with, and it gets no gradient)
+            const float ix = NORM ? (live ? g.ix[c] : 0.f) : 1.f, cs = ix > 0.f ? g.cs * ix : g.cs;
+            float lse2 = 0.f, out = 0.f, at_target = 0.f;
+            if (GRAD && live) {
+                lse2 = g.lse2[c];
+                out = up * ix * (g.coef ? g.coef[c] : 1.f);
+                if (g.target) at_target = g.slope[c] * out;
+            }
+            if (!ptx::mbar_wait_relaxed(&bar.acc_full[it & 1], (it >> 1) & 1) || *abort_flag) { atomicExch(&g_head_status, 4); *abort_flag = 1; break; }
+            ptx::tc_fence_after_sync();
+            const uint32_t acc = tmem + lanes + (it & 1) * kTile + h * kHalf;
+            float most = -INFINITY, sum = 0.f;
+#pragma unroll 1
+            for (int n = 0; n < kHalf; n += 32) {
+                float d[32];
+                pair::tmem_ld32(acc + n, d);
+                ptx::tmem_ld_wait();
+                const int col = v + n;
+                const bool hit = (unsigned)(target - col) < 32u;
+                if constexpr (NORM) {
+                    const float4* iw = reinterpret_cast<const float4*>(g.iw + col);
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) {
+                        const float4 f = __ldg(iw + j);
+                        d[4 * j] *= f.x; d[4 * j + 1] *= f.y; d[4 * j + 2] *= f.z; d[4 * j + 3] *= f.w;
+                    }
+                }
+                if constexpr (!GRAD) {
+                    if (col + 32 > g.V) {
+#pragma unroll
+                        for (int j = 0; j < 32; ++j)
+                            if (col + j >= g.V) d[j] = -INFINITY;
+                    }
+                    if (hit) {   // the target's logit is added in its own form
+#pragma unroll
+                        for (int j = 0; j < 32; ++j)
+                            if (j == target - col) d[j] = -INFINITY;
+                    }
+                    float m[8];
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) m[j] = fmaxf(fmaxf(d[j], d[j + 8]), fmaxf(d[j + 16], d[j + 24]));
+                    const float top = fmaxf(fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3])), fmaxf(fmaxf(m[4], m[5]), fmaxf(m[6], m[7])));
+                    const float to = fmaxf(most, top * cs), by = to > -INFINITY ? to : 0.f;
+                    float s[4] = {};
+#pragma unroll
+                    for (int j = 0; j < 32; ++j) s[j & 3] += exp2_fast(fmaf(d[j], cs, -by));
+                    sum = sum * exp2_fast(most - by) + ((s[0] + s[1]) + (s[2] + s[3]));
+                    most = to;
+                } else {
+                    uint32_t packed[16];
+                    if constexpr (NORM) {
+                        const float4* iw = reinterpret_cast<const float4*>(g.iw + col);
+#pragma unroll
+                        for (int j = 0; j < 8; ++j) {
+                            const float4 f = __ldg(iw + j);
+                            d[4 * j] = exp2_fast(fmaf(d[4 * j], cs, -lse2)) * (out * f.x);
+                            d[4 * j + 1] = exp2_fast(fmaf(d[4 * j + 1], cs, -lse2)) * (out * f.y);
+                            d[4 * j + 2] = exp2_fast(fmaf(d[4 * j + 2], cs, -lse2)) * (out * f.z);
+                            d[4 * j + 3] = exp2_fast(fmaf(d[4 * j + 3], cs, -lse2)) * (out * f.w);
+                        }
+                        if (hit) {
+                            const float f = at_target * g.iw[target];
+#pragma unroll
+                            for (int j = 0; j < 32; ++j)
+                                if (j == target - col) d[j] = f;
+                        }
+                    } else {
+#pragma unroll
+                        for (int j = 0; j < 32; ++j) d[j] = exp2_fast(fmaf(d[j], cs, -lse2)) * out;
+                        if (hit) {
+#pragma unroll
+                            for (int j = 0; j < 32; ++j)
+                                if (j == target - col) d[j] = at_target;
+                        }
+                    }
+                    if (!live || col + 32 > g.V) {   // rows and classes that are not there: zeros, whatever was staged
+#pragma unroll
+                        for (int j = 0; j < 32; ++j)
+                            if (!live || col + j >= g.V) d[j] = 0.f;
+                    }
+#pragma unroll
+                    for (int j = 0; j < 16; ++j) packed[j] = Cvt<E>::pack2(d[2 * j], d[2 * j + 1]);
+                    E* dst = reinterpret_cast<E*>(g.grad) + (size_t)c * g.pitch + (col - g.v0);
+                    store_sector(dst, packed);
+                    store_sector(dst + 16, packed + 8);
+                }
+            }
+            ptx::tc_fence_before_sync();
+            __syncwarp();
+            if (lane == 0) pair::arrive_cluster(pair::in_leader(&bar.acc_empty[it & 1]));
+            if (!GRAD && live) g.part[(size_t)(v / kPart) * g.Np + c] = make_float2(most, sum);
+        }
+    }
+    __syncwarp();
+    ptx::tc_fence_before_sync();
+    __syncthreads();
+    pair::cluster_sync();   // neither CTA leaves while the other may still signal it or read its operands
+    if (warp == 2) pair::tmem_dealloc(tmem, kCols);
+}
+
+template <typename E, bool GRAD, bool NORM>
+cudaError_t run(const Shape& s, const Saved& sv, const Args& a, const void* w, int64_t ldw, int dtype, cudaStream_t st) {
+    Maps maps;
+    const int64_t dx[2] = {s.D, s.Np}, sx[1] = {s.Dp}, dw[2] = {s.D, s.V}, sw[1] = {ldw};
+    const int box[2] = {kStep, kHalf};
+    if (!make_matrix_map(&maps.x, sv.x, dtype, 2, dx, sx, box) || !make_matrix_map(&maps.w, w, dtype, 2, dw, sw, box)) return cudaErrorInvalidValue;
+    auto* kern = logits_kernel<E, GRAD, NORM>;
+    if (cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem)) return e;
+    const int64_t items = s.Np / kTile * a.tiles, pairs = device_sm_count() / 2;
+    kern<<<2 * (int)(items < pairs ? items : pairs), kThreads, kSmem, st>>>(maps, a);
+    return cudaGetLastError();
+}
+template <bool GRAD>
+cudaError_t launch(const na1d_head& h, const Shape& s, const Saved& sv, Args a, const void* w, int64_t ldw, cudaStream_t st) {
+    a.words = sv.words; a.target = s.k ? nullptr : sv.target; a.ix = sv.ix; a.iw = sv.iw; a.lse2 = sv.lse2; a.slope = sv.slope;
+    a.Np = s.Np; a.V = (int)s.V; a.cs = s.cs; a.fp16 = h.dtype == NA1D_FP16;
+    a.steps = (int)((s.D + kStep - 1) / kStep);
+    a.tail = (int)((s.D - (int64_t)(a.steps - 1) * kStep + 15) / 16);
+    using B = __nv_bfloat16;
+    if (h.dtype == NA1D_BF16) return s.norm ? run<B, GRAD, true>(s, sv, a, w, ldw, 0, st) : run<B, GRAD, false>(s, sv, a, w, ldw, 0, st);
+    return s.norm ? run<__half, GRAD, true>(s, sv, a, w, ldw, 1, st) : run<__half, GRAD, false>(s, sv, a, w, ldw, 1, st);
+}
+
+}  // namespace
+
+cudaError_t stats(const na1d_head& h, const Shape& s, const Saved& sv, float2* part, const void* w, int64_t ldw, cudaStream_t st) {
+    Args a = {};
+    a.part = part;
+    a.tiles = (int)((s.V + kTile - 1) / kTile);
+    return launch<false>(h, s, sv, a, w, ldw, st);
+}
+cudaError_t gradients(const na1d_head& h, const Shape& s, const Saved& sv, const float* coef, void* grad, int64_t pitch, int64_t v0, int64_t tiles, const void* w,
+                      int64_t ldw, cudaStream_t st) {
+    Args a = {};
+    a.coef = coef; a.grad = grad; a.pitch = pitch; a.v0 = (int)v0; a.tiles = (int)tiles;
+    return launch<true>(h, s, sv, a, w, ldw, st);
+}
+int logits_read_status() {
+    int v = 0, zero = 0;
+    if (cudaMemcpyFromSymbol(&v, g_head_status, sizeof(int)) != cudaSuccess) return -1;
+    if (v != 0) cudaMemcpyToSymbol(g_head_status, &zero, sizeof(int));
+    return v;
+}
+
+}  // namespace head
+}  // namespace na1d

@@ -1,0 +1,603 @@
+// The passes around the products of a head's losses: each reads its inputs once, a warp to a row or a class.
+#include "na1d_head.cuh"
+
+namespace na1d {
+namespace head {
+namespace {
+
+constexpr int kWarps = 8, kThreads = 32 * kWarps;
+
+// element i of a tensor of one of the three types
+__device__ __forceinline__ float load_any(const void* p, int type, long long i) {
+    if (type == NA1D_FP32) return static_cast<const float*>(p)[i];
+    const unsigned short raw = static_cast<const unsigned short*>(p)[i];
+    return type == NA1D_BF16 ? Cvt<__nv_bfloat16>::from_bits(raw) : Cvt<__half>::from_bits(raw);
+}
+__device__ __forceinline__ void store_any(void* p, int type, long long i, float v) {
+    if (type == NA1D_FP32) static_cast<float*>(p)[i] = v;
+    else if (type == NA1D_BF16) static_cast<__nv_bfloat16*>(p)[i] = __float2bfloat16_rn(v);
+    else static_cast<__half*>(p)[i] = __float2half_rn(v);
+}
+__device__ __forceinline__ float warp_sum(float v) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    return v;
+}
+__device__ __forceinline__ float warp_max(float v) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
+    return v;
+}
+__device__ __forceinline__ float exp2_fast(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+// One row of D elements to 16 bits at dst (Dp of them, zeros behind D; null: not stored), returns 1 / its length (0 where that is 0).
+// wide: rows start on 16 bytes, D is a multiple of 8.
+template <typename E>
+__device__ __forceinline__ float copy_row(E* dst, const void* src, int type, long long at, int D, int Dp, bool wide, bool norm, int lane) {
+    float ss = 0.f;
+    // eight elements to a lane at a time in every form, so that a row's length has the same bits in all of them
+    for (int j = lane; j < Dp / 8; j += 32) {
+        uint4 v;
+        if (wide && type != NA1D_FP32) {
+            v = __ldg(reinterpret_cast<const uint4*>(static_cast<const E*>(src) + at) + j);
+        } else {
+            float f[8];
+            if (wide) {
+                const float4* p = reinterpret_cast<const float4*>(static_cast<const float*>(src) + at) + 2 * j;
+                const float4 a = __ldg(p), b = __ldg(p + 1);
+                f[0] = a.x; f[1] = a.y; f[2] = a.z; f[3] = a.w; f[4] = b.x; f[5] = b.y; f[6] = b.z; f[7] = b.w;
+            } else {
+#pragma unroll
+                for (int k = 0; k < 8; ++k) f[k] = 8 * j + k < D ? load_any(src, type, at + 8 * j + k) : 0.f;
+            }
+            v = Cvt<E>::pack(f);
+        }
+        if (dst) reinterpret_cast<uint4*>(dst)[j] = v;
+        if (norm) {
+            float f[8];
+            Cvt<E>::unpack(v, f);
+#pragma unroll
+            for (int k = 0; k < 8; ++k) ss = fmaf(f[k], f[k], ss);
+        }
+    }
+    if (!norm) return 1.f;
+    ss = warp_sum(ss);
+    return ss > 0.f ? rsqrtf(ss) : ss == 0.f ? 0.f : ss;   // (NaN stays)
+}
+
+// ---------------------------------------------------------------- a teacher's probabilities
+// softmax over a row's entries; a warp to a row. An entry counts with a class in [0, V); one beyond is an error that shows as NaN.
+__global__ void __launch_bounds__(kThreads) teacher_kernel(const float* __restrict__ logits, const int64_t* __restrict__ index, int N, int k, long long V, float rt,
+                                                           float* __restrict__ q, float* __restrict__ q_all, int* __restrict__ out, int* __restrict__ flags) {
+    const int i = blockIdx.x * kWarps + (threadIdx.x >> 5), lane = threadIdx.x & 31;
+    if (i >= N) return;
+    const size_t at = (size_t)i * k;
+    float most = -INFINITY;
+    bool bad = false, nan = false;
+    for (int j = lane; j < k; j += 32) {
+        const int64_t v = index[at + j];
+        if (v < 0) continue;
+        const float t = logits[at + j] * rt;
+        bad |= v >= V;
+        nan |= t != t;
+        most = fmaxf(most, t);
+    }
+    most = warp_max(most);
+    bad = __any_sync(0xffffffffu, bad);
+    nan = __any_sync(0xffffffffu, nan) || most == INFINITY;
+    const bool any = most > -INFINITY || bad || nan;
+    float sum = 0.f;
+    for (int j = lane; j < k; j += 32) {
+        const int64_t v = index[at + j];
+        const bool there = v >= 0;
+        const float e = there && most > -INFINITY ? expf(logits[at + j] * rt - most) : 0.f;
+        sum += e;
+        q[at + j] = e;
+        out[at + j] = !there ? kIgnored : v < V ? (int)v : kBad;
+    }
+    sum = warp_sum(sum);
+    const float r = bad || nan ? NAN : 1.f / sum;
+    __syncwarp();
+    // a class that comes twice: its first entry gets all of its probability in q_all, the others none and, in `out`, are taken out for the
+    // gradient (their bits are inverted: the forward pass still reads them)
+    for (int j0 = 0; j0 < k; j0 += 32) {
+        const int j = j0 + lane;
+        float p = 0.f, all = 0.f;
+        int v = kIgnored;
+        bool first = true;
+        if (j < k) {
+            p = q[at + j];
+            p = any && (p > 0.f || r != r) ? p * r : 0.f;
+            all = p;
+            v = out[at + j];
+            if (v >= 0)
+                for (int o = 0; o < k; ++o)
+                    if (o != j && index[at + o] == v) {
+                        first &= o > j;
+                        const float e = expf(logits[at + o] * rt - most);
+                        all += e * r;
+                    }
+        }
+        __syncwarp();
+        if (j < k) {
+            q_all[at + j] = first ? all : 0.f;
+            if (r != r && out[at + j] >= 0) q_all[at + j] = r;
+        }
+        // (q is read by other lanes no more: each reads its own)
+        if (j < k) {
+            q[at + j] = out[at + j] == kBad || (r != r && v >= 0) ? r : p;
+            if (v >= 0 && !first) out[at + j] = ~v - 2;   // <= -3: class -3 - out
+        }
+        __syncwarp();
+    }
+    if (lane == 0) flags[i] = any;
+}
+// class of an entry as the forward pass reads it
+__device__ __forceinline__ int entry_class(int v) { return v <= -3 ? -3 - v : v; }
+
+// ---------------------------------------------------------------- rows that count, side by side
+struct RowArgs {
+    const void* x;
+    const int64_t* labels;
+    const int* flags;
+    float* loss;               // (N) zeros for rows that do not count; null where the loss is one number
+    Words* words;
+    int *place, *row, *target;
+    float* ix;
+    void* out;
+    long long x_stride, ignore, V;
+    int N, Np, D, Dp, type, per_block;
+    bool wide, norm;
+};
+// A block takes `per_block` rows. It counts the rows before its own itself: labels are few bytes, and no block waits for another.
+template <typename E>
+__global__ void __launch_bounds__(kThreads) rows_kernel(const __grid_constant__ RowArgs a) {
+    __shared__ int sums[kWarps], places[kThreads], base_s;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, r0 = blockIdx.x * a.per_block, r1 = min(a.N, r0 + a.per_block);
+    auto counts = [&](int i) { return a.flags ? a.flags[i] != 0 : a.labels[i] != a.ignore; };
+    int before = 0;
+    for (int i = threadIdx.x; i < r0; i += kThreads) before += counts(i);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) before += __shfl_xor_sync(0xffffffffu, before, o);
+    if (lane == 0) sums[warp] = before;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        int s = 0;
+        for (int w = 0; w < kWarps; ++w) s += sums[w];
+        base_s = s;
+    }
+    __syncthreads();
+    int base = base_s;
+    E* out = static_cast<E*>(a.out);
+    float most = 0.f;
+    for (int c0 = r0; c0 < r1; c0 += kThreads) {
+        const int i = c0 + threadIdx.x;
+        const bool in = i < r1, on = in && counts(i);
+        const unsigned mask = __ballot_sync(0xffffffffu, on);
+        __syncthreads();
+        if (lane == 0) sums[warp] = __popc(mask);
+        __syncthreads();
+        int c = base + __popc(mask & ((1u << lane) - 1));
+        for (int w = 0; w < warp; ++w) c += sums[w];
+        int total = 0;
+        for (int w = 0; w < kWarps; ++w) total += sums[w];
+        if (in) {
+            // a row that does not count: the free places from the end are filled with zeros in the order of such rows
+            places[threadIdx.x] = on ? c : -1 - (a.N - 1 - (i - c));
+            a.place[i] = on ? c : kIgnored;
+            if (on) {
+                a.row[c] = i;
+                if (a.labels) {
+                    const int64_t v = a.labels[i];
+                    a.target[c] = v >= 0 && v < a.V ? (int)v : kBad;
+                }
+            } else if (a.loss) a.loss[i] = 0.f;
+        }
+        __syncthreads();
+        const int n = min(kThreads, r1 - c0);
+        for (int j = warp; j < n; j += kWarps) {
+            const int p = places[j];
+            if (p >= 0) {
+                const float ix = copy_row<E>(out + (size_t)p * a.Dp, a.x, a.type, (c0 + j) * a.x_stride, a.D, a.Dp, a.wide, a.norm, lane);
+                if (a.norm && lane == 0) a.ix[p] = ix;
+                most = fmaxf(most, ix);
+            } else {
+                for (int e = lane; e < a.Dp / 8; e += 32) reinterpret_cast<uint4*>(out + (size_t)(-1 - p) * a.Dp)[e] = make_uint4(0, 0, 0, 0);
+            }
+        }
+        base += total;
+        __syncthreads();
+    }
+    for (int p = a.N + blockIdx.x; p < a.Np; p += gridDim.x)
+        for (int e = threadIdx.x; e < a.Dp / 8; e += kThreads) reinterpret_cast<uint4*>(out + (size_t)p * a.Dp)[e] = make_uint4(0, 0, 0, 0);
+    if (a.norm && lane == 0 && most > 0.f) atomicMax(&a.words->most_ix, __float_as_int(most));   // (the largest, in whatever order)
+    if (r1 == a.N && threadIdx.x == 0) a.words->counted = base;
+}
+
+// ---------------------------------------------------------------- the weight
+struct WeightArgs {
+    const void* w;
+    void* out;
+    float* iw;
+    Words* words;
+    long long stride;
+    int V, D, Dp, type;
+    bool wide, norm;
+};
+template <typename E>
+__global__ void __launch_bounds__(kThreads) weight_kernel(const __grid_constant__ WeightArgs a) {
+    const int lane = threadIdx.x & 31;
+    float most = 0.f;
+    for (int v = blockIdx.x * kWarps + (threadIdx.x >> 5); v < a.V; v += gridDim.x * kWarps) {
+        const float iw = copy_row<E>(a.out ? static_cast<E*>(a.out) + (size_t)v * a.Dp : nullptr, a.w, a.type, v * a.stride, a.D, a.Dp, a.wide, a.norm, lane);
+        if (a.norm && lane == 0) a.iw[v] = iw;
+        most = fmaxf(most, iw);
+    }
+    if (a.norm && lane == 0 && most > 0.f) atomicMax(&a.words->most_iw, __float_as_int(most));
+}
+
+// ---------------------------------------------------------------- single logits
+// x (a 16-bit row of Dp, zeros behind D) times a row of the weight: one warp, every lane gets the sum
+template <typename E>
+__device__ __forceinline__ float dot_row(const E* x, const E* w, int D8, int lane) {
+    float s = 0.f;
+    for (int j = lane; j < D8; j += 32) {
+        float a[8], b[8];
+        Cvt<E>::unpack(__ldg(reinterpret_cast<const uint4*>(x) + j), a);
+        Cvt<E>::unpack(__ldg(reinterpret_cast<const uint4*>(w) + j), b);
+#pragma unroll
+        for (int k = 0; k < 8; ++k) s = fmaf(a[k], b[k], s);
+    }
+    return warp_sum(s);
+}
+struct Products {
+    const void *x, *w;
+    const float *ix, *iw;
+    long long ldw;
+    int Dp;
+    float cs;
+    bool norm;
+};
+// the logit of row c and class v as a product or a cosine
+template <typename E>
+__device__ __forceinline__ float logit_of(const Products& p, int c, int v, int lane) {
+    const float s = dot_row(static_cast<const E*>(p.x) + (size_t)c * p.Dp, static_cast<const E*>(p.w) + (size_t)v * p.ldw, p.Dp / 8, lane);
+    return p.norm ? s * p.ix[c] * p.iw[v] : s;
+}
+// the teacher's entries: a warp to four of a row's
+constexpr int kEntries = 4;
+template <typename E>
+__global__ void __launch_bounds__(kThreads) entries_kernel(const __grid_constant__ Products p, const Words* __restrict__ words, const int* __restrict__ row,
+                                                           const int* __restrict__ index, int k, float* __restrict__ entry) {
+    const int lane = threadIdx.x & 31, groups = (k + kEntries - 1) / kEntries;
+    const long long n = (long long)words->counted * groups;
+    for (long long i = (long long)blockIdx.x * kWarps + (threadIdx.x >> 5); i < n; i += (long long)gridDim.x * kWarps) {
+        const int c = (int)(i / groups), j0 = (int)(i % groups) * kEntries;
+        const size_t at = (size_t)row[c] * k;
+#pragma unroll
+        for (int e = 0; e < kEntries; ++e) {
+            const int j = j0 + e;
+            if (j >= k) break;
+            const int v = entry_class(index[at + j]);
+            const float z = v >= 0 ? logit_of<E>(p, c, v, lane) * p.cs : 0.f;
+            if (lane == 0) entry[at + j] = z;
+        }
+    }
+}
+
+// ---------------------------------------------------------------- log-sum-exp and loss
+struct CombineArgs {
+    const float2* part;
+    Words* words;
+    const int *row, *target, *index;
+    const float *q, *q_all;
+    float *entry, *lse2, *slope, *block_sums, *loss;
+    long long Np;
+    int parts, k, reduction;
+    float cos_m, sin_m, tau2;
+    bool margin;
+    Products p;
+};
+// A block takes 32 rows: its warps share out the partial sums (a lane to a row), then take four rows each for what belongs to the target
+// or the teacher's entries. The last block to finish adds up the blocks' sums in their order.
+template <typename E>
+__global__ void __launch_bounds__(kThreads) combine_kernel(const __grid_constant__ CombineArgs a) {
+    __shared__ float top_s[kWarps][32], sum_s[kWarps][32], loss_s[32];
+    __shared__ int last;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, counted = a.words->counted, c0 = blockIdx.x * 32;
+    if (c0 < counted) {
+        float most = -INFINITY, sum = 0.f;
+        if (c0 + lane < counted)
+            for (int p = warp; p < a.parts; p += kWarps) {
+                const float2 v = a.part[(size_t)p * a.Np + c0 + lane];
+                const float to = fmaxf(most, v.x), by = to > -INFINITY ? to : 0.f;
+                sum = sum * exp2_fast(most - by) + v.y * exp2_fast(v.x - by);
+                most = to;
+            }
+        top_s[warp][lane] = most;
+        sum_s[warp][lane] = sum;
+        __syncthreads();
+        for (int j = warp; j < 32; j += kWarps) {
+            const int c = c0 + j;
+            float loss = 0.f;
+            if (c < counted) {
+                float m = -INFINITY, s = 0.f;
+#pragma unroll
+                for (int w = 0; w < kWarps; ++w) m = fmaxf(m, top_s[w][j]);
+                const float by = m > -INFINITY ? m : 0.f;
+#pragma unroll
+                for (int w = 0; w < kWarps; ++w) s += sum_s[w][j] * exp2_fast(top_s[w][j] - by);
+                if (a.k == 0) {
+                    const int target = a.target[c];
+                    if (target < 0) {
+                        loss = NAN;
+                        if (lane == 0) a.lse2[c] = NAN;
+                    } else {
+                        float z = logit_of<E>(a.p, c, target, lane), slope = 1.f;
+                        if (a.margin) {   // cos(angle + m) and its derivative
+                            const float sine2 = fmaf(-z, z, 1.f), sine = sqrtf(fmaxf(sine2, kSineFloor));
+                            slope = a.cos_m + (sine2 > kSineFloor ? z / sine : 0.f) * a.sin_m;
+                            z = z * a.cos_m - sine * a.sin_m;
+                        }
+                        z *= a.p.cs;
+                        // the other classes' sum against the target: others = sum 2^(z_v - top), top the largest of all
+                        const float top = fmaxf(m, z), others = s * exp2_fast((m > -INFINITY ? m : top) - top), own = exp2_fast(z - top);
+                        const float all = others + own;
+                        loss = z == top ? log1pf(others) : fmaf(top - z, kLn2, logf(all));
+                        if (lane == 0) {
+                            a.lse2[c] = top + log2f(all);
+                            a.slope[c] = -(others / all) * slope;
+                        }
+                    }
+                } else {
+                    const float lse2 = m + log2f(s);
+                    const size_t at = (size_t)a.row[c] * a.k;
+                    for (int e = lane; e < a.k; e += 32) {
+                        const float q = a.q[at + e], z2 = a.entry[at + e] - lse2;
+                        if (q > 0.f) loss += q * (logf(q) - z2 * kLn2);
+                        else if (q != q) loss = q;
+                        a.entry[at + e] = exp2_fast(z2) - a.q_all[at + e];
+                    }
+                    loss = warp_sum(loss) * a.tau2;
+                    if (lane == 0) a.lse2[c] = loss == loss ? lse2 : NAN;   // (an entry that is no class: nothing of the row counts)
+                }
+                if (a.reduction == NA1D_HEAD_NONE && lane == 0) a.loss[a.row[c]] = loss;
+            }
+            if (lane == 0) loss_s[j] = loss;
+        }
+        __syncthreads();
+    }
+    if (a.reduction == NA1D_HEAD_NONE) return;
+    if (warp == 0) {
+        const float s = c0 < counted ? warp_sum(loss_s[lane]) : 0.f;
+        if (lane == 0) {
+            a.block_sums[blockIdx.x] = s;
+            __threadfence();
+            last = atomicAdd(&a.words->ticket, 1) == (int)gridDim.x - 1;
+        }
+    }
+    __syncthreads();
+    if (!last) return;
+    __threadfence();
+    float s = 0.f;
+    for (int b = threadIdx.x; b < (int)gridDim.x; b += kThreads) s += __ldcg(a.block_sums + b);
+    s = warp_sum(s);
+    if (lane == 0) top_s[warp][0] = s;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        s = 0.f;
+        for (int w = 0; w < kWarps; ++w) s += top_s[w][0];
+        *a.loss = a.reduction == NA1D_HEAD_MEAN ? s / (float)max(counted, 1) : s;
+    }
+}
+
+// ---------------------------------------------------------------- backward
+// factors of single rows' losses, side by side as the rows; fp16: relative to the largest, which follows them
+__global__ void __launch_bounds__(1024) coefficients_kernel(const float* __restrict__ d_loss, const Words* __restrict__ words, const int* __restrict__ row, long long Np,
+                                                            bool relative, float* __restrict__ coef) {
+    __shared__ float most_s[32];
+    const int counted = words->counted;
+    float most = 0.f;
+    if (relative) {
+        for (int c = threadIdx.x; c < counted; c += 1024) most = fmaxf(most, fabsf(d_loss[row[c]]));
+        most = warp_max(most);
+        if ((threadIdx.x & 31) == 0) most_s[threadIdx.x >> 5] = most;
+        __syncthreads();
+        most = warp_max(most_s[threadIdx.x & 31]);
+    }
+    if (!(most > 0.f) || most == INFINITY) most = 1.f;
+    const float r = 1.f / most;
+    for (int c = threadIdx.x; c < counted; c += 1024) coef[c] = relative ? d_loss[row[c]] * r : d_loss[row[c]];
+    if (threadIdx.x == 0) coef[Np] = most;
+}
+// the gradients at the teacher's entries, in their places in a piece's gradients
+template <typename E>
+__global__ void __launch_bounds__(kThreads) put_kernel(E* __restrict__ grad, long long pitch, int v0, int cols, const Words* __restrict__ words, const int* __restrict__ row,
+                                                       const int* __restrict__ index, const float* __restrict__ entry, const float* __restrict__ coef,
+                                                       const float* __restrict__ ix, const float* __restrict__ iw, int k, bool fp16, bool norm) {
+    const long long n = (long long)words->counted * k;
+    const float up = gradient_scale(words, fp16, norm);
+    for (long long i = (long long)blockIdx.x * kThreads + threadIdx.x; i < n; i += (long long)gridDim.x * kThreads) {
+        const int c = (int)(i / k), j = (int)(i - (long long)c * k);
+        const size_t at = (size_t)row[c] * k + j;
+        const int v = index[at];
+        if ((unsigned)(v - v0) >= (unsigned)cols || v < 0) continue;
+        const float f = up * (coef ? coef[c] : 1.f) * (norm ? ix[c] : 1.f);
+        grad[(size_t)c * pitch + (v - v0)] = E(entry[at] * (norm ? f * iw[v] : f));
+    }
+}
+
+struct FinishArgs {
+    void *dx, *dw;
+    const float *part_x, *part_w, *d_loss, *coef;
+    const void *x, *w;
+    const float *ix, *iw;
+    const int* place;
+    Words* words;
+    long long Np, piece_rows, ldw;
+    int N, D, Dp, cols, v0, splits_x, splits_w, x_type, w_type, reduction;
+    float factor;
+    bool fp16, norm;
+};
+// One row of a gradient: the splits' sum, without its part along the row it belongs to where that is normalised, times the common factor.
+template <typename E>
+__device__ __forceinline__ void finish_row(void* out, int type, long long at, const float* part, long long split, int splits, const E* own, float inverse, float f,
+                                           bool norm, int D, int Dp, int lane) {
+    float along = 0.f;
+    if (norm) {
+        for (int j = lane; j < Dp / 8; j += 32) {
+            float x[8], s[8] = {};
+            Cvt<E>::unpack(__ldg(reinterpret_cast<const uint4*>(own) + j), x);
+            for (int k = 0; k < splits; ++k) {
+                const float4* p = reinterpret_cast<const float4*>(part + k * split) + 2 * j;
+                const float4 u = p[0], v = p[1];
+                s[0] += u.x; s[1] += u.y; s[2] += u.z; s[3] += u.w; s[4] += v.x; s[5] += v.y; s[6] += v.z; s[7] += v.w;
+            }
+#pragma unroll
+            for (int e = 0; e < 8; ++e) along = fmaf(x[e], 8 * j + e < D ? s[e] : 0.f, along);
+        }
+        along = warp_sum(along) * inverse * inverse;
+    }
+    const bool wide = D % 8 == 0 && type != NA1D_FP32;
+    for (int j = lane; j < Dp / 8; j += 32) {
+        float s[8] = {};
+        for (int k = 0; k < splits; ++k) {
+            const float4* p = reinterpret_cast<const float4*>(part + k * split) + 2 * j;
+            const float4 u = p[0], v = p[1];
+            s[0] += u.x; s[1] += u.y; s[2] += u.z; s[3] += u.w; s[4] += v.x; s[5] += v.y; s[6] += v.z; s[7] += v.w;
+        }
+        if (norm) {
+            float x[8];
+            Cvt<E>::unpack(__ldg(reinterpret_cast<const uint4*>(own) + j), x);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) s[e] = fmaf(-along, x[e], s[e]);
+        }
+#pragma unroll
+        for (int e = 0; e < 8; ++e) s[e] *= f;
+        if (wide) reinterpret_cast<uint4*>(static_cast<E*>(out) + at)[j] = Cvt<E>::pack(s);
+        else
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+                if (8 * j + e < D) store_any(out, type, at + 8 * j + e, s[e]);
+    }
+}
+template <typename E>
+__global__ void __launch_bounds__(kThreads) finish_kernel(const __grid_constant__ FinishArgs a) {
+    const int lane = threadIdx.x & 31, counted = a.words->counted, n = (a.dx ? a.N : 0) + a.cols;
+    float f = a.factor / gradient_scale(a.words, a.fp16, a.norm);
+    if (a.reduction == NA1D_HEAD_NONE) f *= a.coef[a.Np];
+    else f *= a.d_loss[0] / (a.reduction == NA1D_HEAD_MEAN ? (float)max(counted, 1) : 1.f);
+    for (int i = blockIdx.x * kWarps + (threadIdx.x >> 5); i < n; i += gridDim.x * kWarps) {
+        if (i < a.cols) {
+            const int v = a.v0 + i;
+            finish_row<E>(a.dw, a.w_type, (long long)v * a.D, a.part_w + (size_t)i * a.Dp, a.piece_rows * a.Dp, a.splits_w, static_cast<const E*>(a.w) + (size_t)v * a.ldw,
+                          a.norm ? a.iw[v] : 1.f, f, a.norm, a.D, a.Dp, lane);
+        } else {
+            const int r = i - a.cols, c = a.place[r];
+            if (c < 0) {
+                for (int j = lane; j < a.D; j += 32) store_any(a.dx, a.x_type, (long long)r * a.D + j, 0.f);
+                continue;
+            }
+            finish_row<E>(a.dx, a.x_type, (long long)r * a.D, a.part_x + (size_t)c * a.Dp, a.Np * a.Dp, a.splits_x, static_cast<const E*>(a.x) + (size_t)c * a.Dp,
+                          a.norm ? a.ix[c] : 1.f, f, a.norm, a.D, a.Dp, lane);
+        }
+    }
+}
+
+int blocks_for(int64_t warps, int64_t most = 148 * 8) {
+    const int64_t b = (warps + kWarps - 1) / kWarps;
+    return (int)(b < 1 ? 1 : b < most ? b : most);
+}
+Products products_of(const Shape& s, const Saved& sv, const void* w, int64_t ldw) {
+    return Products{sv.x, w, sv.ix, sv.iw, ldw, (int)s.Dp, s.cs, s.norm};
+}
+
+}  // namespace
+
+cudaError_t teacher(const na1d_head& h, const Shape& s, const Saved& sv, int* flags, cudaStream_t st) {
+    teacher_kernel<<<(unsigned)((s.N + kWarps - 1) / kWarps), kThreads, 0, st>>>(h.teacher_logits, h.teacher_index, (int)s.N, (int)s.k, s.V, 1.f / h.temperature, sv.q, sv.q_all,
+                                                                                 sv.index, flags);
+    return cudaGetLastError();
+}
+cudaError_t rows(const na1d_head& h, const Shape& s, const Saved& sv, const int* flags, float* loss, cudaStream_t st) {
+    RowArgs a = {};
+    a.x = h.x; a.labels = s.k ? nullptr : h.labels; a.flags = flags;
+    a.loss = h.reduction == NA1D_HEAD_NONE ? loss : nullptr;
+    a.words = sv.words; a.place = sv.place; a.row = sv.row; a.target = sv.target; a.ix = sv.ix; a.out = sv.x;
+    a.x_stride = h.x_stride; a.ignore = h.ignore_index; a.V = s.V;
+    a.N = (int)s.N; a.Np = (int)s.Np; a.D = (int)s.D; a.Dp = (int)s.Dp; a.type = h.x_type; a.norm = s.norm;
+    a.wide = s.D % 8 == 0 && h.x_stride % 8 == 0 && (reinterpret_cast<uintptr_t>(h.x) & 15) == 0;
+    const int64_t per = round_up((s.N + 295) / 296, kWarps);
+    a.per_block = (int)per;
+    const unsigned blocks = (unsigned)((s.N + per - 1) / per);
+    if (h.dtype == NA1D_BF16) rows_kernel<__nv_bfloat16><<<blocks, kThreads, 0, st>>>(a);
+    else rows_kernel<__half><<<blocks, kThreads, 0, st>>>(a);
+    return cudaGetLastError();
+}
+cudaError_t weight(const na1d_head& h, const Shape& s, const Saved& sv, cudaStream_t st) {
+    if (!s.copy_w && !s.norm) return cudaSuccess;
+    WeightArgs a = {};
+    a.w = h.weight; a.out = s.copy_w ? sv.w : nullptr; a.iw = sv.iw; a.words = sv.words; a.stride = h.weight_stride;
+    a.V = (int)s.V; a.D = (int)s.D; a.Dp = (int)s.Dp; a.type = h.weight_type; a.norm = s.norm;
+    a.wide = s.D % 8 == 0 && h.weight_stride % 8 == 0 && (reinterpret_cast<uintptr_t>(h.weight) & 15) == 0;
+    if (h.dtype == NA1D_BF16) weight_kernel<__nv_bfloat16><<<blocks_for(s.V), kThreads, 0, st>>>(a);
+    else weight_kernel<__half><<<blocks_for(s.V), kThreads, 0, st>>>(a);
+    return cudaGetLastError();
+}
+cudaError_t entries(const na1d_head& h, const Shape& s, const Saved& sv, const void* w, int64_t ldw, cudaStream_t st) {
+    const int blocks = blocks_for(s.N * ((s.k + kEntries - 1) / kEntries));
+    const Products p = products_of(s, sv, w, ldw);
+    if (h.dtype == NA1D_BF16) entries_kernel<__nv_bfloat16><<<blocks, kThreads, 0, st>>>(p, sv.words, sv.row, sv.index, (int)s.k, sv.entry);
+    else entries_kernel<__half><<<blocks, kThreads, 0, st>>>(p, sv.words, sv.row, sv.index, (int)s.k, sv.entry);
+    return cudaGetLastError();
+}
+cudaError_t combine(const na1d_head& h, const Shape& s, const Saved& sv, const float2* part, float* block_sums, float* loss, const void* w, int64_t ldw,
+                    cudaStream_t st) {
+    CombineArgs a = {};
+    a.part = part; a.words = sv.words; a.row = sv.row; a.target = sv.target; a.index = sv.index; a.q = sv.q; a.q_all = sv.q_all;
+    a.entry = sv.entry; a.lse2 = sv.lse2; a.slope = sv.slope; a.block_sums = block_sums; a.loss = loss;
+    a.Np = s.Np; a.parts = (int)s.parts; a.k = (int)s.k; a.reduction = h.reduction;
+    a.margin = s.norm && h.margin != 0.f;
+    a.cos_m = (float)cos((double)h.margin); a.sin_m = (float)sin((double)h.margin);
+    a.tau2 = h.temperature * h.temperature;
+    a.p = products_of(s, sv, w, ldw);
+    const unsigned blocks = (unsigned)((s.N + 31) / 32);
+    if (h.dtype == NA1D_BF16) combine_kernel<__nv_bfloat16><<<blocks, kThreads, 0, st>>>(a);
+    else combine_kernel<__half><<<blocks, kThreads, 0, st>>>(a);
+    return cudaGetLastError();
+}
+cudaError_t coefficients(const na1d_head& h, const Shape& s, const Saved& sv, const float* d_loss, float* coef, cudaStream_t st) {
+    coefficients_kernel<<<1, 1024, 0, st>>>(d_loss, sv.words, sv.row, s.Np, h.dtype == NA1D_FP16, coef);
+    return cudaGetLastError();
+}
+cudaError_t put_entries(const na1d_head& h, const Shape& s, const Saved& sv, const float* coef, void* grad, int64_t pitch, int64_t v0, int64_t cols, cudaStream_t st) {
+    const int blocks = blocks_for((s.N * s.k + 31) / 32);
+    if (h.dtype == NA1D_BF16)
+        put_kernel<<<blocks, kThreads, 0, st>>>(static_cast<__nv_bfloat16*>(grad), pitch, (int)v0, (int)cols, sv.words, sv.row, sv.index, sv.entry, coef, sv.ix, sv.iw,
+                                                (int)s.k, false, s.norm);
+    else
+        put_kernel<<<blocks, kThreads, 0, st>>>(static_cast<__half*>(grad), pitch, (int)v0, (int)cols, sv.words, sv.row, sv.index, sv.entry, coef, sv.ix, sv.iw, (int)s.k,
+                                                true, s.norm);
+    return cudaGetLastError();
+}
+cudaError_t finish(const na1d_head& h, const Shape& s, const Saved& sv, void* dx, void* dw, const float* part_x, const float* part_w, const float* d_loss,
+                   const float* coef, int splits_x, int splits_w, int64_t v0, int64_t cols, int64_t piece_rows, const void* w, int64_t ldw, cudaStream_t st) {
+    FinishArgs a = {};
+    a.dx = dx; a.dw = dw; a.part_x = part_x; a.part_w = part_w; a.d_loss = d_loss; a.coef = coef;
+    a.x = sv.x; a.w = w; a.ix = sv.ix; a.iw = sv.iw; a.place = sv.place; a.words = sv.words;
+    a.Np = s.Np; a.piece_rows = piece_rows; a.ldw = ldw;
+    a.N = (int)s.N; a.D = (int)s.D; a.Dp = (int)s.Dp; a.cols = dw ? (int)cols : 0; a.v0 = (int)v0; a.splits_x = splits_x; a.splits_w = splits_w;
+    a.x_type = h.x_type; a.w_type = h.weight_type; a.reduction = h.reduction; a.norm = s.norm; a.fp16 = h.dtype == NA1D_FP16;
+    a.factor = s.k ? h.scale * h.temperature : h.scale;
+    const int blocks = blocks_for((dx ? s.N : 0) + a.cols, 148 * 8);
+    if (h.dtype == NA1D_BF16) finish_kernel<__nv_bfloat16><<<blocks, kThreads, 0, st>>>(a);
+    else finish_kernel<__half><<<blocks, kThreads, 0, st>>>(a);
+    return cudaGetLastError();
+}
+
+}  // namespace head
+}  // namespace na1d
