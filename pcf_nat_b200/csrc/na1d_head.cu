@@ -30,21 +30,22 @@ Saved saved_at(const na1d_head& h, const Shape& s, void* base) {
         return static_cast<void*>(p);
     };
     v.words = static_cast<Words*>(take(sizeof(Words)));
+    v.own_count = static_cast<int*>(take(round_up(s.V, kTile) * 4));   // (behind the words: both start as zeros)
+    v.zeros = at;
     v.place = static_cast<int*>(take(s.N * 4));
     v.row = static_cast<int*>(take(s.Np * 4));
     v.lse2 = static_cast<float*>(take(s.Np * 4));
+    v.target = static_cast<int*>(take(s.Np * 4));
+    v.slope = static_cast<float*>(take(s.Np * 4));
+    v.own = static_cast<int*>(take(s.V * kOwn * 4));
     if (s.norm) {
         v.ix = static_cast<float*>(take(s.Np * 4));
         v.iw = static_cast<float*>(take(round_up(s.V, kTile) * 4));
     }
     if (s.k) {
         v.q = static_cast<float*>(take(s.N * s.k * 4));
-        v.q_all = static_cast<float*>(take(s.N * s.k * 4));
         v.index = static_cast<int*>(take(s.N * s.k * 4));
         v.entry = static_cast<float*>(take(s.N * s.k * 4));
-    } else {
-        v.target = static_cast<int*>(take(s.Np * 4));
-        v.slope = static_cast<float*>(take(s.Np * 4));
     }
     v.x = take(s.Np * s.Dp * 2);
     if (s.copy_w) v.w = take(s.V * s.Dp * 2);
@@ -158,11 +159,10 @@ int forward(const na1d_head& h, float* loss, void* saved, void* scratch, cudaStr
     const Forward f = forward_at(s, scratch);
     const void* w = s.copy_w ? sv.w : h.weight;
     const int64_t ldw = s.copy_w ? s.Dp : h.weight_stride;
-    NA1D_HEAD_TRY(cudaMemsetAsync(sv.words, 0, sizeof(Words), st));
+    NA1D_HEAD_TRY(cudaMemsetAsync(saved, 0, sv.zeros, st));
     if (s.k) NA1D_HEAD_TRY(teacher(h, s, sv, f.flags, st));
     NA1D_HEAD_TRY(rows(h, s, sv, f.flags, loss, st));
     NA1D_HEAD_TRY(weight(h, s, sv, st));
-    if (s.k) NA1D_HEAD_TRY(entries(h, s, sv, w, ldw, st));
     NA1D_HEAD_TRY(stats(h, s, sv, f.part, w, ldw, st));
     NA1D_HEAD_TRY(combine(h, s, sv, f.part, f.block_sums, loss, w, ldw, st));
     return NA1D_OK;
@@ -180,7 +180,6 @@ int backward(const na1d_head& h, void* dx, void* dw, const float* d_loss, void* 
     for (int64_t i = 0; i < p.count; ++i) {
         const int64_t v0 = i * p.pitch, cols = s.V - v0 < p.pitch ? s.V - v0 : p.pitch;
         NA1D_HEAD_TRY(gradients(h, s, sv, b.coef, b.grad, p.pitch, v0, (cols + kTile - 1) / kTile, w, ldw, st));
-        if (s.k) NA1D_HEAD_TRY(put_entries(h, s, sv, b.coef, b.grad, p.pitch, v0, cols, st));
         NA1D_HEAD_TRY(products(h, s, sv, b.grad, p, v0, cols, i > 0, b.part_x, b.part_w, w, ldw, st));
         const bool last = i + 1 == p.count;
         if (dw || last)

@@ -20,6 +20,8 @@ constexpr int kTile = 256;            // rows and classes of a product tile (a p
 constexpr int kPart = 128;            // classes that one partial maximum and sum stand for
 constexpr float kSineFloor = 2e-7f;   // of the squared sine in the margin's formula
 constexpr int kIgnored = -1, kBad = -2;
+constexpr int kNoClass = 0x7fffffff;  // behind a row's entries, which are sorted by class
+constexpr int kOwn = 8;               // rows of a class whose own gradients' roundings are made good
 
 inline int64_t round_up(int64_t x, int64_t m) { return (x + m - 1) / m * m; }
 
@@ -35,18 +37,19 @@ struct Saved {
     Words* words;
     int* place;        // (N)  c of a row, or kIgnored
     int* row;          // (Np) row of c
-    int* target;       // (Np) class of c, or kBad (classes only)
     float* lse2;       // (Np) log2 of the softmax's sum
-    float* slope;      // (Np) gradient of the target's logit: (p - 1) psi' (classes only)
+    int* target;       // (Np) the row's own class: its label (or kBad), or the entry with the largest gradient
+    float* slope;      // (Np) gradient of that class's logit: (p - 1) psi', or p - q
+    int* own_count;    // (V rounded up) rows whose own class it is
+    int* own;          // (V, kOwn) and the first of them to come
     float* ix;         // (Np) 1 / |x| (normalised)
     float* iw;         // (V rounded up) 1 / |w|
-    float* q;          // (N, k) teacher's probabilities, 0 where there is none
-    float* q_all;      // (N, k) the same with a class's later entries added to its first
-    int* index;        // (N, k) class, kIgnored (none, or not its first entry) or kBad
-    float* entry;      // (N, k) the entry's logit in powers of two, then its gradient p - q_all
+    float* q;          // (N, k) teacher's probabilities, sorted by class
+    int* index;        // (N, k) classes in their order, kNoClass behind them
+    float* entry;      // (N, k) the entry's logit as a power of two, then its gradient p - q
     void* x;           // (Np, Dp) 16 bits, zeros behind the rows that count
     void* w;           // (V, Dp) 16 bits, where the weight is not used in its place
-    int64_t bytes;
+    int64_t zeros, bytes;   // the first of them start as zeros
 };
 
 struct Shape {
@@ -71,11 +74,9 @@ Pieces pieces_of(const Shape& s, bool want_x, bool want_w);
 cudaError_t teacher(const na1d_head& h, const Shape& s, const Saved& sv, int* flags, cudaStream_t st);
 cudaError_t rows(const na1d_head& h, const Shape& s, const Saved& sv, const int* flags, float* loss, cudaStream_t st);
 cudaError_t weight(const na1d_head& h, const Shape& s, const Saved& sv, cudaStream_t st);
-cudaError_t entries(const na1d_head& h, const Shape& s, const Saved& sv, const void* w, int64_t ldw, cudaStream_t st);
 cudaError_t combine(const na1d_head& h, const Shape& s, const Saved& sv, const float2* part, float* block_sums, float* loss, const void* w, int64_t ldw,
                     cudaStream_t st);
 cudaError_t coefficients(const na1d_head& h, const Shape& s, const Saved& sv, const float* d_loss, float* coef, cudaStream_t st);
-cudaError_t put_entries(const na1d_head& h, const Shape& s, const Saved& sv, const float* coef, void* grad, int64_t pitch, int64_t v0, int64_t cols, cudaStream_t st);
 // gradients of rows v0 .. v0 + cols of the weight (cols may be 0) and, where dx is given, of the rows
 cudaError_t finish(const na1d_head& h, const Shape& s, const Saved& sv, void* dx, void* dw, const float* part_x, const float* part_w, const float* d_loss,
                    const float* coef, int splits_x, int splits_w, int64_t v0, int64_t cols, int64_t piece_rows, const void* w, int64_t ldw, cudaStream_t st);
@@ -101,6 +102,10 @@ __device__ __forceinline__ float gradient_scale(const Words* w, bool fp16, bool 
     e = 6 - e;
     return ldexpf(1.f, e < -100 ? -100 : e > 100 ? 100 : e);
 }
+
+// The gradient of a row's own class as it is rounded to 16 bits, in one order of operations: `out` = row_factor(..)
+__device__ __forceinline__ float row_factor(float up, float ix, float coef, bool norm) { return norm ? up * ix * coef : up * coef; }
+__device__ __forceinline__ float own_gradient(float slope, float out, float iw, bool norm) { return norm ? (slope * out) * iw : slope * out; }
 
 }  // namespace head
 }  // namespace na1d

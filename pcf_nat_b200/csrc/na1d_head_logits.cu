@@ -30,12 +30,13 @@ struct Barriers {
 struct Maps { CUtensorMap x, w; };
 struct Args {
     const Words* words;
-    const int* target;
+    const int *row, *target, *index;
     const float *ix, *iw, *lse2, *slope, *coef;
+    float* entry;
     float2* part;               // stats: (classes / 128, Np)
     void* grad;                 // gradient: (Np, pitch)
     long long Np, pitch;
-    int V, v0, tiles, steps, tail;   // first class and tiles of classes of this launch; stages of a tile, products of 16 channels in the last one
+    int V, v0, tiles, k, steps, tail;   // first class and tiles of classes of this launch; stages of a tile, products of 16 channels in the last one
     float cs;
     bool fp16;
 };
@@ -53,7 +54,9 @@ __device__ __forceinline__ Tile tile_at(int t, int row_tiles, int tiles) {
     return Tile{first + t % height, t / height};
 }
 
-template <typename E, bool GRAD, bool NORM>
+// TOP: the rows have a teacher's entries, sorted by class, instead of a label. A lane has the place of its row's next entry at hand, and the
+// class of the one after it.
+template <typename E, bool GRAD, bool NORM, bool TOP>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) logits_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Args g) {
     extern __shared__ uint8_t raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~(uintptr_t)1023);
@@ -135,15 +138,35 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) logits_
             const Tile t = tile_at(i, row_tiles, g.tiles);
             const int c = t.m * kTile + rank * kHalf + q * 32 + lane, v = g.v0 + t.n * kTile + h * kHalf;
             const bool live = c < counted;
-            const int target = live && g.target ? g.target[c] : kIgnored;
+            const int target = !TOP && live ? g.target[c] : kIgnored;
             // (a row of zeros has no direction: its products are 0 whatever they are multiplied with, and it gets no gradient)
             const float ix = NORM ? (live ? g.ix[c] : 0.f) : 1.f, cs = ix > 0.f ? g.cs * ix : g.cs;
             float lse2 = 0.f, out = 0.f, at_target = 0.f;
             if (GRAD && live) {
                 lse2 = g.lse2[c];
-                out = up * ix * (g.coef ? g.coef[c] : 1.f);
-                if (g.target) at_target = g.slope[c] * out;
+                out = row_factor(up, ix, g.coef ? g.coef[c] : 1.f, NORM);
+                if (!TOP && target >= 0) at_target = own_gradient(g.slope[c], out, NORM ? g.iw[target] : 1.f, NORM);
             }
+            const int* classes = nullptr;
+            float* entry = nullptr;
+            int next = kNoClass, after = kNoClass, pos = 0;
+            if (TOP && live) {
+                classes = g.index + (size_t)g.row[c] * g.k;
+                entry = g.entry + (size_t)g.row[c] * g.k;
+                int end = g.k;
+                while (pos < end) {   // the first entry whose class is v or more
+                    const int mid = (pos + end) >> 1;
+                    if (__ldg(classes + mid) < v) pos = mid + 1;
+                    else end = mid;
+                }
+                if (pos < g.k) next = __ldg(classes + pos);
+                if (pos + 1 < g.k) after = __ldg(classes + pos + 1);
+            }
+            auto advance = [&]() {
+                ++pos;
+                next = after;
+                after = pos + 1 < g.k ? __ldg(classes + pos + 1) : kNoClass;
+            };
             if (!ptx::mbar_wait_relaxed(&bar.acc_full[it & 1], (it >> 1) & 1) || *abort_flag) { atomicExch(&g_head_status, 4); *abort_flag = 1; break; }
             ptx::tc_fence_after_sync();
             const uint32_t acc = tmem + lanes + (it & 1) * kTile + h * kHalf;
@@ -154,7 +177,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) logits_
                 pair::tmem_ld32(acc + n, d);
                 ptx::tmem_ld_wait();
                 const int col = v + n;
-                const bool hit = (unsigned)(target - col) < 32u;
+                const bool hit = !TOP && (unsigned)(target - col) < 32u;
                 if constexpr (NORM) {
                     const float4* iw = reinterpret_cast<const float4*>(g.iw + col);
 #pragma unroll
@@ -173,6 +196,18 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) logits_
 #pragma unroll
                         for (int j = 0; j < 32; ++j)
                             if (j == target - col) d[j] = -INFINITY;
+                    }
+                    if constexpr (TOP) {
+                        while (__any_sync(0xffffffffu, next < col + 32)) {
+                            if (next < col + 32) {
+                                float z = 0.f;
+#pragma unroll
+                                for (int j = 0; j < 32; ++j)
+                                    if (j == next - col) z = d[j];
+                                entry[pos] = z * cs;
+                                advance();
+                            }
+                        }
                     }
                     float m[8];
 #pragma unroll
@@ -197,10 +232,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) logits_
                             d[4 * j + 3] = exp2_fast(fmaf(d[4 * j + 3], cs, -lse2)) * (out * f.w);
                         }
                         if (hit) {
-                            const float f = at_target * g.iw[target];
 #pragma unroll
                             for (int j = 0; j < 32; ++j)
-                                if (j == target - col) d[j] = f;
+                                if (j == target - col) d[j] = at_target;
                         }
                     } else {
 #pragma unroll
@@ -209,6 +243,17 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) logits_
 #pragma unroll
                             for (int j = 0; j < 32; ++j)
                                 if (j == target - col) d[j] = at_target;
+                        }
+                    }
+                    if constexpr (TOP) {
+                        while (__any_sync(0xffffffffu, next < col + 32)) {
+                            if (next < col + 32) {
+                                const float f = own_gradient(entry[pos], out, NORM ? __ldg(g.iw + next) : 1.f, NORM);
+#pragma unroll
+                                for (int j = 0; j < 32; ++j)
+                                    if (j == next - col) d[j] = f;
+                                advance();
+                            }
                         }
                     }
                     if (!live || col + 32 > g.V) {   // rows and classes that are not there: zeros, whatever was staged
@@ -236,13 +281,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) logits_
     if (warp == 2) pair::tmem_dealloc(tmem, kCols);
 }
 
-template <typename E, bool GRAD, bool NORM>
+template <typename E, bool GRAD, bool NORM, bool TOP>
 cudaError_t run(const Shape& s, const Saved& sv, const Args& a, const void* w, int64_t ldw, int dtype, cudaStream_t st) {
     Maps maps;
     const int64_t dx[2] = {s.D, s.Np}, sx[1] = {s.Dp}, dw[2] = {s.D, s.V}, sw[1] = {ldw};
     const int box[2] = {kStep, kHalf};
     if (!make_matrix_map(&maps.x, sv.x, dtype, 2, dx, sx, box) || !make_matrix_map(&maps.w, w, dtype, 2, dw, sw, box)) return cudaErrorInvalidValue;
-    auto* kern = logits_kernel<E, GRAD, NORM>;
+    auto* kern = logits_kernel<E, GRAD, NORM, TOP>;
     if (cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem)) return e;
     const int64_t items = s.Np / kTile * a.tiles, pairs = device_sm_count() / 2;
     kern<<<2 * (int)(items < pairs ? items : pairs), kThreads, kSmem, st>>>(maps, a);
@@ -250,13 +295,18 @@ cudaError_t run(const Shape& s, const Saved& sv, const Args& a, const void* w, i
 }
 template <bool GRAD>
 cudaError_t launch(const na1d_head& h, const Shape& s, const Saved& sv, Args a, const void* w, int64_t ldw, cudaStream_t st) {
-    a.words = sv.words; a.target = s.k ? nullptr : sv.target; a.ix = sv.ix; a.iw = sv.iw; a.lse2 = sv.lse2; a.slope = sv.slope;
-    a.Np = s.Np; a.V = (int)s.V; a.cs = s.cs; a.fp16 = h.dtype == NA1D_FP16;
+    a.words = sv.words; a.row = sv.row; a.target = sv.target; a.index = sv.index; a.entry = sv.entry;
+    a.ix = sv.ix; a.iw = sv.iw; a.lse2 = sv.lse2; a.slope = sv.slope;
+    a.Np = s.Np; a.V = (int)s.V; a.k = (int)s.k; a.cs = s.cs; a.fp16 = h.dtype == NA1D_FP16;
     a.steps = (int)((s.D + kStep - 1) / kStep);
     a.tail = (int)((s.D - (int64_t)(a.steps - 1) * kStep + 15) / 16);
     using B = __nv_bfloat16;
-    if (h.dtype == NA1D_BF16) return s.norm ? run<B, GRAD, true>(s, sv, a, w, ldw, 0, st) : run<B, GRAD, false>(s, sv, a, w, ldw, 0, st);
-    return s.norm ? run<__half, GRAD, true>(s, sv, a, w, ldw, 1, st) : run<__half, GRAD, false>(s, sv, a, w, ldw, 1, st);
+    if (s.k) {
+        if (h.dtype == NA1D_BF16) return s.norm ? run<B, GRAD, true, true>(s, sv, a, w, ldw, 0, st) : run<B, GRAD, false, true>(s, sv, a, w, ldw, 0, st);
+        return s.norm ? run<__half, GRAD, true, true>(s, sv, a, w, ldw, 1, st) : run<__half, GRAD, false, true>(s, sv, a, w, ldw, 1, st);
+    }
+    if (h.dtype == NA1D_BF16) return s.norm ? run<B, GRAD, true, false>(s, sv, a, w, ldw, 0, st) : run<B, GRAD, false, false>(s, sv, a, w, ldw, 0, st);
+    return s.norm ? run<__half, GRAD, true, false>(s, sv, a, w, ldw, 1, st) : run<__half, GRAD, false, false>(s, sv, a, w, ldw, 1, st);
 }
 
 }  // namespace

@@ -70,74 +70,41 @@ __device__ __forceinline__ float copy_row(E* dst, const void* src, int type, lon
 }
 
 // ---------------------------------------------------------------- a teacher's probabilities
-// softmax over a row's entries; a warp to a row. An entry counts with a class in [0, V); one beyond is an error that shows as NaN.
+// Softmax over a row's entries, and the entries in the order of their classes, so that a tile of classes finds its own; a warp to a row. An
+// entry counts with a class in [0, V); one beyond (or a logit that is no number) makes the row's probabilities NaN.
 __global__ void __launch_bounds__(kThreads) teacher_kernel(const float* __restrict__ logits, const int64_t* __restrict__ index, int N, int k, long long V, float rt,
-                                                           float* __restrict__ q, float* __restrict__ q_all, int* __restrict__ out, int* __restrict__ flags) {
+                                                           float* __restrict__ q, int* __restrict__ out, int* __restrict__ flags) {
     const int i = blockIdx.x * kWarps + (threadIdx.x >> 5), lane = threadIdx.x & 31;
     if (i >= N) return;
     const size_t at = (size_t)i * k;
     float most = -INFINITY;
-    bool bad = false, nan = false;
+    bool bad = false;
     for (int j = lane; j < k; j += 32) {
         const int64_t v = index[at + j];
         if (v < 0) continue;
         const float t = logits[at + j] * rt;
-        bad |= v >= V;
-        nan |= t != t;
+        bad |= v >= V || t != t || t == INFINITY;
         most = fmaxf(most, t);
     }
     most = warp_max(most);
     bad = __any_sync(0xffffffffu, bad);
-    nan = __any_sync(0xffffffffu, nan) || most == INFINITY;
-    const bool any = most > -INFINITY || bad || nan;
+    auto weight = [&](int j) { return index[at + j] >= 0 && most > -INFINITY ? expf(logits[at + j] * rt - most) : 0.f; };
     float sum = 0.f;
+    for (int j = lane; j < k; j += 32) sum += weight(j);
+    sum = warp_sum(sum);
+    const float r = 1.f / sum;
     for (int j = lane; j < k; j += 32) {
         const int64_t v = index[at + j];
-        const bool there = v >= 0;
-        const float e = there && most > -INFINITY ? expf(logits[at + j] * rt - most) : 0.f;
-        sum += e;
-        q[at + j] = e;
-        out[at + j] = !there ? kIgnored : v < V ? (int)v : kBad;
+        int rank = 0;   // entries without a class come last
+        for (int o = 0; o < k; ++o) {
+            const int64_t u = index[at + o];
+            rank += (v >= 0 ? u >= 0 && (u < v || (u == v && o < j)) : u >= 0 || o < j);
+        }
+        q[at + rank] = v < 0 ? 0.f : bad ? NAN : most > -INFINITY ? weight(j) * r : 0.f;
+        out[at + rank] = v >= 0 && v < V ? (int)v : kNoClass;
     }
-    sum = warp_sum(sum);
-    const float r = bad || nan ? NAN : 1.f / sum;
-    __syncwarp();
-    // a class that comes twice: its first entry gets all of its probability in q_all, the others none and, in `out`, are taken out for the
-    // gradient (their bits are inverted: the forward pass still reads them)
-    for (int j0 = 0; j0 < k; j0 += 32) {
-        const int j = j0 + lane;
-        float p = 0.f, all = 0.f;
-        int v = kIgnored;
-        bool first = true;
-        if (j < k) {
-            p = q[at + j];
-            p = any && (p > 0.f || r != r) ? p * r : 0.f;
-            all = p;
-            v = out[at + j];
-            if (v >= 0)
-                for (int o = 0; o < k; ++o)
-                    if (o != j && index[at + o] == v) {
-                        first &= o > j;
-                        const float e = expf(logits[at + o] * rt - most);
-                        all += e * r;
-                    }
-        }
-        __syncwarp();
-        if (j < k) {
-            q_all[at + j] = first ? all : 0.f;
-            if (r != r && out[at + j] >= 0) q_all[at + j] = r;
-        }
-        // (q is read by other lanes no more: each reads its own)
-        if (j < k) {
-            q[at + j] = out[at + j] == kBad || (r != r && v >= 0) ? r : p;
-            if (v >= 0 && !first) out[at + j] = ~v - 2;   // <= -3: class -3 - out
-        }
-        __syncwarp();
-    }
-    if (lane == 0) flags[i] = any;
+    if (lane == 0) flags[i] = bad || most > -INFINITY;
 }
-// class of an entry as the forward pass reads it
-__device__ __forceinline__ int entry_class(int v) { return v <= -3 ? -3 - v : v; }
 
 // ---------------------------------------------------------------- rows that count, side by side
 struct RowArgs {
@@ -268,34 +235,14 @@ __device__ __forceinline__ float logit_of(const Products& p, int c, int v, int l
     const float s = dot_row(static_cast<const E*>(p.x) + (size_t)c * p.Dp, static_cast<const E*>(p.w) + (size_t)v * p.ldw, p.Dp / 8, lane);
     return p.norm ? s * p.ix[c] * p.iw[v] : s;
 }
-// the teacher's entries: a warp to four of a row's
-constexpr int kEntries = 4;
-template <typename E>
-__global__ void __launch_bounds__(kThreads) entries_kernel(const __grid_constant__ Products p, const Words* __restrict__ words, const int* __restrict__ row,
-                                                           const int* __restrict__ index, int k, float* __restrict__ entry) {
-    const int lane = threadIdx.x & 31, groups = (k + kEntries - 1) / kEntries;
-    const long long n = (long long)words->counted * groups;
-    for (long long i = (long long)blockIdx.x * kWarps + (threadIdx.x >> 5); i < n; i += (long long)gridDim.x * kWarps) {
-        const int c = (int)(i / groups), j0 = (int)(i % groups) * kEntries;
-        const size_t at = (size_t)row[c] * k;
-#pragma unroll
-        for (int e = 0; e < kEntries; ++e) {
-            const int j = j0 + e;
-            if (j >= k) break;
-            const int v = entry_class(index[at + j]);
-            const float z = v >= 0 ? logit_of<E>(p, c, v, lane) * p.cs : 0.f;
-            if (lane == 0) entry[at + j] = z;
-        }
-    }
-}
-
 // ---------------------------------------------------------------- log-sum-exp and loss
 struct CombineArgs {
     const float2* part;
     Words* words;
-    const int *row, *target, *index;
-    const float *q, *q_all;
-    float *entry, *lse2, *slope, *block_sums, *loss;
+    const int *row, *index;
+    int *target, *own_count, *own;
+    const float *q, *entry;
+    float *gradient, *lse2, *slope, *block_sums, *loss;
     long long Np;
     int parts, k, reduction;
     float cos_m, sin_m, tau2;
@@ -309,6 +256,10 @@ __global__ void __launch_bounds__(kThreads) combine_kernel(const __grid_constant
     __shared__ float top_s[kWarps][32], sum_s[kWarps][32], loss_s[32];
     __shared__ int last;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, counted = a.words->counted, c0 = blockIdx.x * 32;
+    auto own_row = [&](int v, int c) {   // (in whatever order: they are sorted before they are added up)
+        const int n = atomicAdd(a.own_count + v, 1);
+        if (n < kOwn) a.own[(size_t)v * kOwn + n] = c;
+    };
     if (c0 < counted) {
         float most = -INFINITY, sum = 0.f;
         if (c0 + lane < counted)
@@ -351,16 +302,38 @@ __global__ void __launch_bounds__(kThreads) combine_kernel(const __grid_constant
                         if (lane == 0) {
                             a.lse2[c] = top + log2f(all);
                             a.slope[c] = -(others / all) * slope;
+                            own_row(target, c);
                         }
                     }
                 } else {
                     const float lse2 = m + log2f(s);
                     const size_t at = (size_t)a.row[c] * a.k;
+                    // (a class that comes twice has its entries side by side: all of them take the gradient of the class)
+                    float best = -1.f, own = 0.f;
+                    int own_class = kBad;
                     for (int e = lane; e < a.k; e += 32) {
-                        const float q = a.q[at + e], z2 = a.entry[at + e] - lse2;
+                        const int v = a.index[at + e];
+                        const float q = a.q[at + e];
+                        if (q != q) loss = q;
+                        if (v == kNoClass) continue;
+                        const float z2 = a.entry[at + e] - lse2;
                         if (q > 0.f) loss += q * (logf(q) - z2 * kLn2);
-                        else if (q != q) loss = q;
-                        a.entry[at + e] = exp2_fast(z2) - a.q_all[at + e];
+                        float all = q;
+                        for (int o = e - 1; o >= 0 && a.index[at + o] == v; --o) all += a.q[at + o];
+                        for (int o = e + 1; o < a.k && a.index[at + o] == v; ++o) all += a.q[at + o];
+                        const float g = exp2_fast(z2) - all;
+                        if (fabsf(g) > best) { best = fabsf(g); own = g; own_class = v; }
+                        a.gradient[at + e] = g;
+                    }
+                    for (int o = 16; o > 0; o >>= 1) {   // the largest of all, the lowest class of equals
+                        const float b = __shfl_xor_sync(0xffffffffu, best, o), g = __shfl_xor_sync(0xffffffffu, own, o);
+                        const int v = __shfl_xor_sync(0xffffffffu, own_class, o);
+                        if (b > best || (b == best && v < own_class)) { best = b; own = g; own_class = v; }
+                    }
+                    if (lane == 0) {
+                        a.target[c] = own_class;
+                        a.slope[c] = own;
+                        if (own_class >= 0) own_row(own_class, c);
                     }
                     loss = warp_sum(loss) * a.tau2;
                     if (lane == 0) a.lse2[c] = loss == loss ? lse2 : NAN;   // (an entry that is no class: nothing of the row counts)
@@ -414,49 +387,57 @@ __global__ void __launch_bounds__(1024) coefficients_kernel(const float* __restr
     for (int c = threadIdx.x; c < counted; c += 1024) coef[c] = relative ? d_loss[row[c]] * r : d_loss[row[c]];
     if (threadIdx.x == 0) coef[Np] = most;
 }
-// the gradients at the teacher's entries, in their places in a piece's gradients
-template <typename E>
-__global__ void __launch_bounds__(kThreads) put_kernel(E* __restrict__ grad, long long pitch, int v0, int cols, const Words* __restrict__ words, const int* __restrict__ row,
-                                                       const int* __restrict__ index, const float* __restrict__ entry, const float* __restrict__ coef,
-                                                       const float* __restrict__ ix, const float* __restrict__ iw, int k, bool fp16, bool norm) {
-    const long long n = (long long)words->counted * k;
-    const float up = gradient_scale(words, fp16, norm);
-    for (long long i = (long long)blockIdx.x * kThreads + threadIdx.x; i < n; i += (long long)gridDim.x * kThreads) {
-        const int c = (int)(i / k), j = (int)(i - (long long)c * k);
-        const size_t at = (size_t)row[c] * k + j;
-        const int v = index[at];
-        if ((unsigned)(v - v0) >= (unsigned)cols || v < 0) continue;
-        const float f = up * (coef ? coef[c] : 1.f) * (norm ? ix[c] : 1.f);
-        grad[(size_t)c * pitch + (v - v0)] = E(entry[at] * (norm ? f * iw[v] : f));
-    }
-}
-
 struct FinishArgs {
     void *dx, *dw;
     const float *part_x, *part_w, *d_loss, *coef;
     const void *x, *w;
     const float *ix, *iw;
-    const int* place;
+    const float* slope;
+    const int *place, *target, *own_count, *own;
     Words* words;
     long long Np, piece_rows, ldw;
     int N, D, Dp, cols, v0, splits_x, splits_w, x_type, w_type, reduction;
     float factor;
     bool fp16, norm;
 };
-// One row of a gradient: the splits' sum, without its part along the row it belongs to where that is normalised, times the common factor.
+// What rounding took from the gradient of row c's own class (the largest of the row, mostly): it is made good in fp32
 template <typename E>
+__device__ __forceinline__ float own_rest(const FinishArgs& a, int c, float up) {
+    const int v = a.target[c];
+    const float f = own_gradient(a.slope[c], row_factor(up, a.norm ? a.ix[c] : 1.f, a.coef ? a.coef[c] : 1.f, a.norm), a.norm ? a.iw[v] : 1.f, a.norm);
+    const float rest = f - (float)E(f);
+    return fabsf(rest) < INFINITY ? rest : 0.f;
+}
+template <typename E>
+__device__ __forceinline__ void unpack_row(const E* row, int j, float* f) { Cvt<E>::unpack(__ldg(reinterpret_cast<const uint4*>(row) + j), f); }
+// One row of a gradient: the splits' sum and what rounding took (`n` rows of the other operand times `rest`: `other(i)`), without its part along the row it
+// belongs to where that is normalised, times the common factor.
+template <typename E, typename Other>
 __device__ __forceinline__ void finish_row(void* out, int type, long long at, const float* part, long long split, int splits, const E* own, float inverse, float f,
-                                           bool norm, int D, int Dp, int lane) {
+                                           int n, const float* rest, Other other, bool norm, int D, int Dp, int lane) {
+    auto sum = [&](int j, float* s) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) s[e] = 0.f;
+        for (int k = 0; k < splits; ++k) {
+            const float4* p = reinterpret_cast<const float4*>(part + k * split) + 2 * j;
+            const float4 u = p[0], v = p[1];
+            s[0] += u.x; s[1] += u.y; s[2] += u.z; s[3] += u.w; s[4] += v.x; s[5] += v.y; s[6] += v.z; s[7] += v.w;
+        }
+#pragma unroll
+        for (int i = 0; i < kOwn; ++i) {
+            if (i >= n) break;
+            float x[8];
+            unpack_row(other(i), j, x);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) s[e] = fmaf(rest[i], x[e], s[e]);
+        }
+    };
     float along = 0.f;
     if (norm) {
         for (int j = lane; j < Dp / 8; j += 32) {
-            float x[8], s[8] = {};
-            Cvt<E>::unpack(__ldg(reinterpret_cast<const uint4*>(own) + j), x);
-            for (int k = 0; k < splits; ++k) {
-                const float4* p = reinterpret_cast<const float4*>(part + k * split) + 2 * j;
-                const float4 u = p[0], v = p[1];
-                s[0] += u.x; s[1] += u.y; s[2] += u.z; s[3] += u.w; s[4] += v.x; s[5] += v.y; s[6] += v.z; s[7] += v.w;
-            }
+            float x[8], s[8];
+            unpack_row(own, j, x);
+            sum(j, s);
 #pragma unroll
             for (int e = 0; e < 8; ++e) along = fmaf(x[e], 8 * j + e < D ? s[e] : 0.f, along);
         }
@@ -464,15 +445,11 @@ __device__ __forceinline__ void finish_row(void* out, int type, long long at, co
     }
     const bool wide = D % 8 == 0 && type != NA1D_FP32;
     for (int j = lane; j < Dp / 8; j += 32) {
-        float s[8] = {};
-        for (int k = 0; k < splits; ++k) {
-            const float4* p = reinterpret_cast<const float4*>(part + k * split) + 2 * j;
-            const float4 u = p[0], v = p[1];
-            s[0] += u.x; s[1] += u.y; s[2] += u.z; s[3] += u.w; s[4] += v.x; s[5] += v.y; s[6] += v.z; s[7] += v.w;
-        }
+        float s[8];
+        sum(j, s);
         if (norm) {
             float x[8];
-            Cvt<E>::unpack(__ldg(reinterpret_cast<const uint4*>(own) + j), x);
+            unpack_row(own, j, x);
 #pragma unroll
             for (int e = 0; e < 8; ++e) s[e] = fmaf(-along, x[e], s[e]);
         }
@@ -488,22 +465,40 @@ __device__ __forceinline__ void finish_row(void* out, int type, long long at, co
 template <typename E>
 __global__ void __launch_bounds__(kThreads) finish_kernel(const __grid_constant__ FinishArgs a) {
     const int lane = threadIdx.x & 31, counted = a.words->counted, n = (a.dx ? a.N : 0) + a.cols;
-    float f = a.factor / gradient_scale(a.words, a.fp16, a.norm);
+    const float up = gradient_scale(a.words, a.fp16, a.norm);
+    float f = a.factor / up;
     if (a.reduction == NA1D_HEAD_NONE) f *= a.coef[a.Np];
     else f *= a.d_loss[0] / (a.reduction == NA1D_HEAD_MEAN ? (float)max(counted, 1) : 1.f);
+    const E *x = static_cast<const E*>(a.x), *w = static_cast<const E*>(a.w);
     for (int i = blockIdx.x * kWarps + (threadIdx.x >> 5); i < n; i += gridDim.x * kWarps) {
+        float rest[kOwn];
         if (i < a.cols) {
-            const int v = a.v0 + i;
-            finish_row<E>(a.dw, a.w_type, (long long)v * a.D, a.part_w + (size_t)i * a.Dp, a.piece_rows * a.Dp, a.splits_w, static_cast<const E*>(a.w) + (size_t)v * a.ldw,
-                          a.norm ? a.iw[v] : 1.f, f, a.norm, a.D, a.Dp, lane);
+            const int v = a.v0 + i, count = a.own_count[v], rows = count <= kOwn ? count : 0;   // (of many rows the roundings average out)
+            int rows_in_order[kOwn];
+            if (rows) {
+                const int mine = lane < rows ? a.own[(size_t)v * kOwn + lane] : kNoClass;
+                int rank = 0;
+#pragma unroll
+                for (int o = 0; o < kOwn; ++o) rank += __shfl_sync(0xffffffffu, mine, o) < mine;
+#pragma unroll
+                for (int o = 0; o < kOwn; ++o) {
+                    const unsigned who = __ballot_sync(0xffffffffu, lane < rows && rank == o);
+                    rows_in_order[o] = __shfl_sync(0xffffffffu, mine, who ? __ffs(who) - 1 : 0);
+                    rest[o] = o < rows ? own_rest<E>(a, rows_in_order[o], up) : 0.f;
+                }
+            }
+            finish_row<E>(a.dw, a.w_type, (long long)v * a.D, a.part_w + (size_t)i * a.Dp, a.piece_rows * a.Dp, a.splits_w, w + (size_t)v * a.ldw,
+                          a.norm ? a.iw[v] : 1.f, f, rows, rest, [&](int o) { return x + (size_t)rows_in_order[o] * a.Dp; }, a.norm, a.D, a.Dp, lane);
         } else {
             const int r = i - a.cols, c = a.place[r];
             if (c < 0) {
                 for (int j = lane; j < a.D; j += 32) store_any(a.dx, a.x_type, (long long)r * a.D + j, 0.f);
                 continue;
             }
-            finish_row<E>(a.dx, a.x_type, (long long)r * a.D, a.part_x + (size_t)c * a.Dp, a.Np * a.Dp, a.splits_x, static_cast<const E*>(a.x) + (size_t)c * a.Dp,
-                          a.norm ? a.ix[c] : 1.f, f, a.norm, a.D, a.Dp, lane);
+            const int v = a.target[c];
+            rest[0] = v >= 0 ? own_rest<E>(a, c, up) : 0.f;
+            finish_row<E>(a.dx, a.x_type, (long long)r * a.D, a.part_x + (size_t)c * a.Dp, a.Np * a.Dp, a.splits_x, x + (size_t)c * a.Dp, a.norm ? a.ix[c] : 1.f, f,
+                          v >= 0 ? 1 : 0, rest, [&](int) { return w + (size_t)v * a.ldw; }, a.norm, a.D, a.Dp, lane);
         }
     }
 }
@@ -519,8 +514,8 @@ Products products_of(const Shape& s, const Saved& sv, const void* w, int64_t ldw
 }  // namespace
 
 cudaError_t teacher(const na1d_head& h, const Shape& s, const Saved& sv, int* flags, cudaStream_t st) {
-    teacher_kernel<<<(unsigned)((s.N + kWarps - 1) / kWarps), kThreads, 0, st>>>(h.teacher_logits, h.teacher_index, (int)s.N, (int)s.k, s.V, 1.f / h.temperature, sv.q, sv.q_all,
-                                                                                 sv.index, flags);
+    teacher_kernel<<<(unsigned)((s.N + kWarps - 1) / kWarps), kThreads, 0, st>>>(h.teacher_logits, h.teacher_index, (int)s.N, (int)s.k, s.V, 1.f / h.temperature, sv.q, sv.index,
+                                                                                 flags);
     return cudaGetLastError();
 }
 cudaError_t rows(const na1d_head& h, const Shape& s, const Saved& sv, const int* flags, float* loss, cudaStream_t st) {
@@ -548,18 +543,11 @@ cudaError_t weight(const na1d_head& h, const Shape& s, const Saved& sv, cudaStre
     else weight_kernel<__half><<<blocks_for(s.V), kThreads, 0, st>>>(a);
     return cudaGetLastError();
 }
-cudaError_t entries(const na1d_head& h, const Shape& s, const Saved& sv, const void* w, int64_t ldw, cudaStream_t st) {
-    const int blocks = blocks_for(s.N * ((s.k + kEntries - 1) / kEntries));
-    const Products p = products_of(s, sv, w, ldw);
-    if (h.dtype == NA1D_BF16) entries_kernel<__nv_bfloat16><<<blocks, kThreads, 0, st>>>(p, sv.words, sv.row, sv.index, (int)s.k, sv.entry);
-    else entries_kernel<__half><<<blocks, kThreads, 0, st>>>(p, sv.words, sv.row, sv.index, (int)s.k, sv.entry);
-    return cudaGetLastError();
-}
 cudaError_t combine(const na1d_head& h, const Shape& s, const Saved& sv, const float2* part, float* block_sums, float* loss, const void* w, int64_t ldw,
                     cudaStream_t st) {
     CombineArgs a = {};
-    a.part = part; a.words = sv.words; a.row = sv.row; a.target = sv.target; a.index = sv.index; a.q = sv.q; a.q_all = sv.q_all;
-    a.entry = sv.entry; a.lse2 = sv.lse2; a.slope = sv.slope; a.block_sums = block_sums; a.loss = loss;
+    a.part = part; a.words = sv.words; a.row = sv.row; a.target = sv.target; a.own_count = sv.own_count; a.own = sv.own; a.index = sv.index; a.q = sv.q;
+    a.entry = a.gradient = sv.entry; a.lse2 = sv.lse2; a.slope = sv.slope; a.block_sums = block_sums; a.loss = loss;
     a.Np = s.Np; a.parts = (int)s.parts; a.k = (int)s.k; a.reduction = h.reduction;
     a.margin = s.norm && h.margin != 0.f;
     a.cos_m = (float)cos((double)h.margin); a.sin_m = (float)sin((double)h.margin);
@@ -574,21 +562,12 @@ cudaError_t coefficients(const na1d_head& h, const Shape& s, const Saved& sv, co
     coefficients_kernel<<<1, 1024, 0, st>>>(d_loss, sv.words, sv.row, s.Np, h.dtype == NA1D_FP16, coef);
     return cudaGetLastError();
 }
-cudaError_t put_entries(const na1d_head& h, const Shape& s, const Saved& sv, const float* coef, void* grad, int64_t pitch, int64_t v0, int64_t cols, cudaStream_t st) {
-    const int blocks = blocks_for((s.N * s.k + 31) / 32);
-    if (h.dtype == NA1D_BF16)
-        put_kernel<<<blocks, kThreads, 0, st>>>(static_cast<__nv_bfloat16*>(grad), pitch, (int)v0, (int)cols, sv.words, sv.row, sv.index, sv.entry, coef, sv.ix, sv.iw,
-                                                (int)s.k, false, s.norm);
-    else
-        put_kernel<<<blocks, kThreads, 0, st>>>(static_cast<__half*>(grad), pitch, (int)v0, (int)cols, sv.words, sv.row, sv.index, sv.entry, coef, sv.ix, sv.iw, (int)s.k,
-                                                true, s.norm);
-    return cudaGetLastError();
-}
 cudaError_t finish(const na1d_head& h, const Shape& s, const Saved& sv, void* dx, void* dw, const float* part_x, const float* part_w, const float* d_loss,
                    const float* coef, int splits_x, int splits_w, int64_t v0, int64_t cols, int64_t piece_rows, const void* w, int64_t ldw, cudaStream_t st) {
     FinishArgs a = {};
     a.dx = dx; a.dw = dw; a.part_x = part_x; a.part_w = part_w; a.d_loss = d_loss; a.coef = coef;
     a.x = sv.x; a.w = w; a.ix = sv.ix; a.iw = sv.iw; a.place = sv.place; a.words = sv.words;
+    a.slope = sv.slope; a.target = sv.target; a.own_count = sv.own_count; a.own = sv.own;
     a.Np = s.Np; a.piece_rows = piece_rows; a.ldw = ldw;
     a.N = (int)s.N; a.D = (int)s.D; a.Dp = (int)s.Dp; a.cols = dw ? (int)cols : 0; a.v0 = (int)v0; a.splits_x = splits_x; a.splits_w = splits_w;
     a.x_type = h.x_type; a.w_type = h.weight_type; a.reduction = h.reduction; a.norm = s.norm; a.fp16 = h.dtype == NA1D_FP16;
