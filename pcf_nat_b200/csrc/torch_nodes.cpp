@@ -20,6 +20,7 @@
 #include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/jit/frontend/tracer.h>
 
@@ -1073,6 +1074,133 @@ OptTensor valid_tokens(const Tensor& padding, int64_t T, int64_t N) {
     return out;
 }
 
+// ---------------------------------------------------------------- losses of a classification head
+struct HeadCall {
+    int64_t ignore, normalize, reduction, dtype;
+    double scale, margin, temperature;
+};
+int head_code(const Tensor& t) { return t.scalar_type() == at::kFloat ? NA1D_FP32 : code(t); }
+na1d_head head_of(const HeadCall& c, int64_t rows, int64_t x_stride, int x_type, const void* x, const Tensor& w) {
+    na1d_head h = {};
+    h.rows = rows; h.dim = w.size(1); h.classes = w.size(0);
+    h.x = x; h.x_stride = x_stride; h.weight = ptr(w); h.weight_stride = w.stride(0);
+    h.ignore_index = c.ignore; h.scale = (float)c.scale; h.margin = (float)c.margin; h.temperature = (float)c.temperature;
+    h.normalize = (int)c.normalize; h.reduction = (int)c.reduction; h.dtype = (int)c.dtype; h.x_type = x_type; h.weight_type = head_code(w);
+    return h;
+}
+int64_t head_bytes(int64_t bytes, const char* where) {
+    if (bytes < 0) check((int)bytes, where);
+    return bytes;
+}
+Tensor head_buffer(int64_t bytes, const Tensor& like) { return at::empty({bytes}, like.options().dtype(at::kByte)); }
+
+// x with its rows one after the other, `x_stride` elements apart
+struct HeadForward {
+    na1d_head h;
+    Tensor loss, saved;
+    HeadForward(const Tensor& x, int64_t x_stride, const Tensor& w, const OptTensor& labels, const OptTensor& logits, const OptTensor& index, const HeadCall& c) {
+        h = head_of(c, x.numel() / w.size(1), x_stride, head_code(x), ptr(x), w);
+        if (labels) h.labels = static_cast<const int64_t*>(ptr(*labels));
+        if (index) {
+            h.top = index->size(-1);
+            h.teacher_logits = fptr(*logits);
+            h.teacher_index = static_cast<const int64_t*>(ptr(*index));
+        }
+        saved = head_buffer(head_bytes(na1d_head_saved_bytes(&h), "na1d_head_saved_bytes"), x);
+        const Tensor scratch = head_buffer(head_bytes(na1d_head_forward_scratch(&h), "na1d_head_forward_scratch"), x);
+        loss = c.reduction == NA1D_HEAD_NONE ? empty_f32(x.sizes().slice(0, x.dim() - 1), x) : empty_f32({}, x);
+        check(na1d_head_forward(&h, fptr(loss), ptr(saved), ptr(scratch), stream()), "na1d_head_forward");
+    }
+};
+// whether the forward pass reads the weight where it is: then the backward pass does so too, else it has a copy of its own
+bool head_in_place(const na1d_head& h) {
+    return h.weight_type == h.dtype && h.weight_stride % 8 == 0 && h.weight_stride >= h.dim && (reinterpret_cast<uintptr_t>(h.weight) & 15) == 0;
+}
+
+struct NA1dHead : public torch::autograd::Function<NA1dHead> {
+    static Tensor forward(AutogradContext* ctx, const Tensor& x, const Tensor& w, const OptTensor& labels, const OptTensor& logits, const OptTensor& index, int64_t x_stride,
+                          int64_t ignore, int64_t normalize, int64_t reduction, int64_t dtype, double scale, double margin, double temperature) {
+        const HeadCall c{ignore, normalize, reduction, dtype, scale, margin, temperature};
+        HeadForward f(x, x_stride, w, labels, logits, index, c);
+        const bool in_place = head_in_place(f.h);
+        ctx->save_for_backward({f.saved, in_place ? w : Tensor()});
+        f.h.x = f.h.labels = static_cast<const int64_t*>(ptr(f.saved));   // (the backward pass reads neither)
+        f.h.teacher_logits = fptr(f.saved);
+        f.h.teacher_index = f.h.labels;
+        auto& d = ctx->saved_data;
+        d["head"] = std::string(reinterpret_cast<const char*>(&f.h), sizeof f.h);
+        d["x"] = x.sizes().vec();
+        d["x_type"] = (int64_t)x.scalar_type();
+        d["w_type"] = (int64_t)w.scalar_type();
+        d["in_place"] = in_place;
+        ctx->set_materialize_grads(false);
+        return f.loss;
+    }
+    static variable_list backward(AutogradContext* ctx, variable_list grads) {
+        variable_list out(13);
+        if (!grads[0].defined()) return out;
+        const bool again = at::GradMode::is_enabled();
+        {
+            const at::NoGradGuard off;
+            auto& d = ctx->saved_data;
+            na1d_head h;
+            const std::string kept = d["head"].toStringRef();
+            std::memcpy(&h, kept.data(), sizeof h);
+            const variable_list s = ctx->get_saved_variables();
+            const Tensor saved = aligned(s[0], 256);
+            const c10::cuda::CUDAGuard guard(saved.device());
+            Tensor w = s[1];
+            if (d["in_place"].toBool()) {   // wherever a hook has put it
+                if (w.stride(1) != 1 || w.stride(0) % 8 != 0 || w.stride(0) < w.size(1)) w = w.contiguous();
+                w = w.storage_offset() % 8 == 0 && (reinterpret_cast<uintptr_t>(w.data_ptr()) & 15) == 0 ? w : w.clone(at::MemoryFormat::Contiguous);
+                h.weight = ptr(w);
+                h.weight_stride = w.stride(0);
+            }
+            const bool want_x = ctx->needs_input_grad(0), want_w = ctx->needs_input_grad(1);
+            const Tensor d_loss = grads[0].to(at::kFloat).contiguous();
+            if (want_x) out[0] = at::empty(d["x"].toIntVector(), saved.options().dtype((at::ScalarType)d["x_type"].toInt()));
+            if (want_w) out[1] = at::empty({h.classes, h.dim}, saved.options().dtype((at::ScalarType)d["w_type"].toInt()));
+            const Tensor scratch = head_buffer(head_bytes(na1d_head_backward_scratch(&h, want_x, want_w), "na1d_head_backward_scratch"), saved);
+            check(na1d_head_backward(&h, ptr(out[0]), ptr(out[1]), fptr(d_loss), ptr(saved), ptr(scratch), stream()), "na1d_head_backward");
+        }
+        if (again) {   // the gradients are constants to no second pass: it is refused
+            const auto refuse = std::make_shared<torch::autograd::DelayedError>("the losses of a head are differentiated once", (int64_t)2);
+            variable_list in(2);
+            for (int i = 0; i < 2; ++i)
+                if (out[i].defined()) in[i] = out[i].detach().set_requires_grad(true);
+            const variable_list marked = (*refuse)(std::move(in));
+            out[0] = marked[0];
+            out[1] = marked[1];
+        }
+        return out;
+    }
+};
+
+OptTensor head(const Tensor& x, const Tensor& w, const OptTensor& labels, const OptTensor& logits, const OptTensor& index, double scale, double margin,
+               double temperature, bool normalize, int64_t ignore, int64_t reduction) {
+    auto usable = [&](const Tensor& t, at::ScalarType type) { return plain(t) && t.device() == x.device() && t.scalar_type() == type && t.is_contiguous() && !t.requires_grad(); };
+    if (!eager_mode() || !plain(x) || !plain(w) || x.device() != w.device() || x.dim() < 1 || w.dim() != 2 || x.numel() == 0 || w.numel() == 0 || x.size(-1) != w.size(1) ||
+        (labels.has_value() == index.has_value()) || logits.has_value() != index.has_value() || reduction < 0 || reduction > 2)
+        return std::nullopt;
+    auto type = x.scalar_type();
+    if (type == at::kFloat && at::autocast::is_autocast_enabled(at::kCUDA)) type = at::autocast::get_autocast_dtype(at::kCUDA);
+    if ((type != at::kBFloat16 && type != at::kHalf) || (x.scalar_type() != type && x.scalar_type() != at::kFloat) ||
+        (w.scalar_type() != type && w.scalar_type() != at::kFloat) || w.stride(1) != 1)
+        return std::nullopt;
+    const int64_t D = w.size(1), rows = x.numel() / D;
+    if (x.dim() == 2 ? x.stride(1) != 1 : !x.is_contiguous()) return std::nullopt;
+    const int64_t x_stride = x.dim() == 2 ? x.stride(0) : D;
+    if (labels && (!usable(*labels, at::kLong) || labels->sizes() != x.sizes().slice(0, x.dim() - 1))) return std::nullopt;
+    if (index && (!usable(*index, at::kLong) || !usable(*logits, at::kFloat) || index->sizes() != logits->sizes() || index->dim() != x.dim() || index->numel() == 0 ||
+                  index->numel() != rows * index->size(-1) || index->sizes().slice(0, x.dim() - 1) != x.sizes().slice(0, x.dim() - 1)))
+        return std::nullopt;
+    const c10::cuda::OptionalCUDAGuard guard(x.device());
+    const HeadCall c{ignore, normalize, reduction, type == at::kBFloat16 ? NA1D_BF16 : NA1D_FP16, scale, margin, temperature};
+    if (at::GradMode::is_enabled() && (x.requires_grad() || w.requires_grad()))
+        return NA1dHead::apply(x, w, labels, logits, index, x_stride, c.ignore, c.normalize, c.reduction, c.dtype, c.scale, c.margin, c.temperature);
+    return HeadForward(x, x_stride, w, labels, logits, index, c).loss;
+}
+
 }  // namespace
 
 PYBIND11_MODULE(_na1d_torch, m) {
@@ -1086,6 +1214,7 @@ PYBIND11_MODULE(_na1d_torch, m) {
     NA1D_DEF(fuse);
     NA1D_DEF(layer);
     NA1D_DEF(valid_tokens);
+    NA1D_DEF(head);
 #undef NA1D_DEF
     m.def("eager_mode", &eager_mode);
 }

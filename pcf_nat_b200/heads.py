@@ -57,11 +57,15 @@ def _forward(cfg, x, weight, labels, teacher_logits, teacher_index):
 
 
 class _HeadFunction(torch.autograd.Function):
+    """The route of calls that the C++ node (csrc/torch_nodes.cpp) leaves to Python."""
+
     @staticmethod
     def forward(ctx, x, weight, labels, teacher_logits, teacher_index, cfg):
         loss, saved, head = _forward(cfg, x, weight, labels, teacher_logits, teacher_index)
-        ctx.save_for_backward(weight, saved)
-        ctx.head, ctx.x_dtype = head, x.dtype
+        # the weight is read again where it is, unless the forward pass made a copy of its own (then the copy is in `saved`)
+        ctx.in_place = weight.dtype != torch.float32 and weight.stride(0) % 8 == 0 and weight.stride(0) >= weight.shape[1] and weight.data_ptr() % 16 == 0
+        ctx.save_for_backward(saved, weight if ctx.in_place else None)
+        ctx.head, ctx.x_dtype, ctx.w_dtype = head, x.dtype, weight.dtype
         ctx.set_materialize_grads(False)
         return loss
 
@@ -70,19 +74,24 @@ class _HeadFunction(torch.autograd.Function):
     def backward(ctx, d_loss):
         if d_loss is None:
             return (None,) * 6
-        weight, saved = ctx.saved_tensors
-        head, want_x, want_w = ctx.head, ctx.needs_input_grad[0], ctx.needs_input_grad[1]
-        # what the backward pass reads is in `saved`, the weight apart
-        head.x = head.labels = head.teacher_logits = head.teacher_index = saved.data_ptr()
-        head.weight = weight.data_ptr()
-        ref = ctypes.byref(head)
-        with ops._on_device(weight.device):
+        saved, weight = ctx.saved_tensors
+        head, want_x, want_w = _lib.Head.from_buffer_copy(ctx.head), ctx.needs_input_grad[0], ctx.needs_input_grad[1]
+        dev = saved.device
+        with ops._on_device(dev):
+            if saved.data_ptr() % 256:                  # (saved tensors come back from wherever a hook has put them)
+                saved = saved.clone()
+            head.x = head.labels = head.teacher_logits = head.teacher_index = saved.data_ptr()   # not read any more
+            if ctx.in_place:
+                if weight.stride(1) != 1 or weight.stride(0) % 8 or weight.stride(0) < weight.shape[1] or weight.data_ptr() % 16:
+                    weight = weight.clone(memory_format=torch.contiguous_format)
+                head.weight, head.weight_stride = weight.data_ptr(), weight.stride(0)
+            ref = ctypes.byref(head)
             d_loss = d_loss.to(torch.float32).contiguous()
-            dx = torch.empty((head.rows, head.dim), dtype=ctx.x_dtype, device=weight.device) if want_x else None
-            dw = torch.empty((head.classes, head.dim), dtype=weight.dtype, device=weight.device) if want_w else None
-            scratch = _buffer(_bytes(_L.na1d_head_backward_scratch(ref, want_x, want_w), "na1d_head_backward_scratch"), weight.device)
+            dx = torch.empty((head.rows, head.dim), dtype=ctx.x_dtype, device=dev) if want_x else None
+            dw = torch.empty((head.classes, head.dim), dtype=ctx.w_dtype, device=dev) if want_w else None
+            scratch = _buffer(_bytes(_L.na1d_head_backward_scratch(ref, want_x, want_w), "na1d_head_backward_scratch"), dev)
             check(_L.na1d_head_backward(ref, dx.data_ptr() if want_x else None, dw.data_ptr() if want_w else None, d_loss.data_ptr(), saved.data_ptr(),
-                                        scratch.data_ptr(), ops._stream(weight)), "na1d_head_backward")
+                                        scratch.data_ptr(), ops._stream(saved)), "na1d_head_backward")
         return dx, dw, None, None, None, None
 
 
@@ -143,6 +152,28 @@ def _run(dt, x, weight, labels, teacher_logits, teacher_index, cfg, reduction):
     return loss.view(shape) if reduction == "none" else loss
 
 
+def _native(x, weight, labels, teacher_logits, teacher_index, cfg, reduction):
+    """The call as one C++ node, or None where it is not of the forms that this takes."""
+    if (type(x) not in _PLAIN or type(weight) not in _PLAIN or torch.compiler.is_compiling() or reduction not in _REDUCTION or
+            type(labels) not in _PLAIN_OR_NONE or type(teacher_logits) not in _PLAIN_OR_NONE or type(teacher_index) not in _PLAIN_OR_NONE):
+        return None
+    ignore, scale, margin, temperature, normalize = cfg
+    return ops.native.head(x, weight, labels, teacher_logits, teacher_index, scale, margin, temperature, normalize, ignore, _REDUCTION[reduction])
+
+
+_PLAIN = (torch.Tensor, torch.nn.Parameter)
+_PLAIN_OR_NONE = _PLAIN + (type(None),)
+
+
+def _labels_loss(x, weight, labels, cfg, reduction):
+    loss = _native(x, weight, labels, None, None, cfg, reduction)
+    if loss is not None:
+        return loss
+    dt = _rows(x, weight, reduction)
+    _index(labels, x.shape[:-1], "labels")
+    return _run(dt, x, weight, labels.reshape(-1).to(torch.int64).contiguous(), None, None, cfg, reduction)
+
+
 # ------------------------------------------------------------------ the losses
 def linear_cross_entropy(x, weight, labels, *, scale=1.0, ignore_index=-100, reduction="mean"):
     """``F.cross_entropy(scale * x @ weight.T, labels)`` without the logits.
@@ -151,18 +182,14 @@ def linear_cross_entropy(x, weight, labels, *, scale=1.0, ignore_index=-100, red
     them reaches the loss or a gradient, and no time goes into them; where no row counts the mean is 0. A label outside the classes makes
     its row's loss, and the gradients that depend on it, NaN (there is no synchronisation to raise an error from). ``reduction``: "mean" over
     the rows that count, "sum", or "none" (0 for the others). Differentiable once in ``x`` and ``weight``; same bits from run to run."""
-    dt = _rows(x, weight, reduction)
-    _index(labels, x.shape[:-1], "labels")
-    return _run(dt, x, weight, labels.reshape(-1).to(torch.int64).contiguous(), None, None, (int(ignore_index), float(scale), 0.0, 1.0, False), reduction)
+    return _labels_loss(x, weight, labels, (int(ignore_index), float(scale), 0.0, 1.0, False), reduction)
 
 
 def angular_cross_entropy(x, weight, labels, *, margin=0.2, scale=30.0, ignore_index=-100, reduction="mean"):
     """AAM-softmax: cross entropy of ``scale`` times the cosines of rows and classes, the label's angle widened by ``margin`` radians
     (``model.AAMSoftmax``; cos(a + m) as cos a cos m - sin a sin m, the squared sine at least 2e-7). A row or class of zeros has cosine 0 with
     all others and no gradient. Otherwise as ``linear_cross_entropy``."""
-    dt = _rows(x, weight, reduction)
-    _index(labels, x.shape[:-1], "labels")
-    return _run(dt, x, weight, labels.reshape(-1).to(torch.int64).contiguous(), None, None, (int(ignore_index), float(scale), float(margin), 1.0, True), reduction)
+    return _labels_loss(x, weight, labels, (int(ignore_index), float(scale), float(margin), 1.0, True), reduction)
 
 
 def linear_distillation(x, weight, teacher_logits, teacher_index, *, temperature=1.0, scale=1.0, normalize=False, reduction="mean"):
@@ -172,6 +199,11 @@ def linear_distillation(x, weight, teacher_logits, teacher_index, *, temperature
     ``teacher_logits`` (..., k) of any floating type, ``teacher_index`` (..., k) int64 or int32: the entries' classes, negative where there is
     no entry (its logit is not read). Rows without an entry do not count; a class may come twice. k is at most 1024. No gradient
     goes to the teacher. Otherwise as ``linear_cross_entropy``."""
+    cfg = (0, float(scale), 0.0, float(temperature), bool(normalize))
+    if teacher_index is not None and teacher_logits is not None:
+        loss = _native(x, weight, None, teacher_logits, teacher_index, cfg, reduction)
+        if loss is not None:
+            return loss
     dt = _rows(x, weight, reduction)
     if not isinstance(teacher_index, torch.Tensor) or teacher_index.dim() != x.dim() or teacher_index.shape[-1] == 0:
         raise ValueError("teacher_index is (..., k) for x (..., dim), k at least 1")
@@ -183,4 +215,4 @@ def linear_distillation(x, weight, teacher_logits, teacher_index, *, temperature
     k = teacher_index.shape[-1]
     logits = teacher_logits.detach().reshape(-1, k).to(torch.float32).contiguous()
     index = teacher_index.reshape(-1, k).to(torch.int64).contiguous()
-    return _run(dt, x, weight, None, logits, index, (0, float(scale), 0.0, float(temperature), bool(normalize)), reduction)
+    return _run(dt, x, weight, None, logits, index, cfg, reduction)

@@ -13,7 +13,7 @@ _L = _lib.lib()
 
 class _PythonRoutes:
     """Stands where the extension of C++ autograd nodes is missing: every call goes on to its Python route."""
-    fused = qk = av = packed = layer = valid_tokens = staticmethod(lambda *_: None)
+    fused = qk = av = packed = layer = valid_tokens = head = staticmethod(lambda *_: None)
     eager_mode = staticmethod(lambda: False)
 
 

@@ -355,3 +355,52 @@ def test_other_stream_and_graph():
     for _, out in graphs:
         assert all(torch.equal(a, b) for a, b in zip(ref, out))
     ops.device_status()
+
+
+@pytest.mark.parametrize("op", ["ce", "angular", "distill"])
+def test_python_route_gives_the_same_bits(op, monkeypatch):
+    N, D, V = 200, 57 if op == "ce" else 64, 500
+    x, w, y, t, i = make(N, D, V, torch.bfloat16, cosine=op == "angular", k=4)
+    f = {"ce": lambda x, w: b200.linear_cross_entropy(x, w, y, reduction="sum"), "angular": lambda x, w: b200.angular_cross_entropy(x, w, y),
+         "distill": lambda x, w: b200.linear_distillation(x, w, t, i)}[op]
+
+    def step():
+        x1, w1 = x.clone().requires_grad_(), w.clone().requires_grad_()
+        loss = f(x1, w1)
+        return (loss.detach(), f(x, w), type(loss.grad_fn).__name__) + torch.autograd.grad(loss, (x1, w1))
+    node = step()
+    monkeypatch.setattr(ops, "native", ops._PythonRoutes)
+    python = step()
+    assert node[2] != python[2]
+    assert all(torch.equal(a, b) for a, b in zip(node, python) if isinstance(a, torch.Tensor))
+
+
+@pytest.mark.parametrize("python", [False, True])
+def test_saved_tensors_moved_by_hooks(python, monkeypatch):
+    if python:
+        monkeypatch.setattr(ops, "native", ops._PythonRoutes)
+    x, w, y = make(200, 64, 500, torch.bfloat16)
+
+    def step():
+        x1, w1 = x.clone().requires_grad_(), w.clone().requires_grad_()
+        return torch.autograd.grad(b200.linear_cross_entropy(x1, w1, y), (x1, w1))
+    ref = step()
+
+    def unpack(t):        # off every boundary, and with other strides
+        if t.dim() == 1:
+            return torch.cat([t.new_zeros(2), t])[2:]
+        return torch.cat([t.new_zeros(t.shape[0], 3), t], 1)[:, 3:]
+    with torch.autograd.graph.saved_tensors_hooks(lambda t: t.clone(), unpack):
+        got = step()
+    assert all(torch.equal(a, b) for a, b in zip(ref, got))
+
+
+def test_weight_changed_between_the_passes():
+    """As with any saved tensor: an error, not another gradient."""
+    x, w, y = make(20, 64, 100, torch.bfloat16)
+    w.requires_grad_()
+    loss = b200.linear_cross_entropy(x, w, y)
+    with torch.no_grad():
+        w.mul_(2)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        loss.backward()
