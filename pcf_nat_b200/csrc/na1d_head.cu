@@ -15,8 +15,8 @@ Shape shape_of(const na1d_head& h) {
     s.parts = (s.V + kTile - 1) / kTile * (kTile / kPart);
     s.x_stride = h.x_stride; s.w_stride = h.weight_stride;
     s.norm = h.normalize != 0;
-    // the weight is read where it is if TMA can: 16-bit rows on 16-byte boundaries
-    s.copy_w = h.weight_type != h.dtype || h.weight_stride % 8 != 0 || h.weight_stride < s.D || (reinterpret_cast<uintptr_t>(h.weight) & 15) != 0;
+    // the weight is read where it is if its rows are whole 16-byte pieces
+    s.copy_w = h.weight_type != h.dtype || s.D % 8 != 0 || h.weight_stride % 8 != 0 || h.weight_stride < s.D || (reinterpret_cast<uintptr_t>(h.weight) & 15) != 0;
     s.cs = kLog2e * h.scale / (s.k ? h.temperature : 1.f);
     return s;
 }
@@ -68,18 +68,21 @@ Pieces pieces_of(const Shape& s, bool want_x, bool want_w) {
     p.pitch = p.piece_tiles * kTile;
     p.d_tiles = (int)((s.D + kTile - 1) / kTile);
     p.d_width = (int)round_up((s.D + p.d_tiles - 1) / p.d_tiles, 32);
-    // splits of the contractions: about as many steps to an item as a pair has in all
+    // Steps of 64 of the two contractions, and a pair's share of all of them. The weight's tiles are whole where that leaves no pair with more than
+    // its share; then their gradients leave at once, unless the way back through the normalisation needs more than one tile of a row. The
+    // rows' tiles fill up what the weight's leave of the pairs' shares, in items of about a third of a share.
     const int64_t steps_x = p.pitch / 64, steps_w = s.Np / 64;
     const int64_t items_x = want_x ? s.Np / kTile * p.d_tiles : 0, items_w = want_w ? p.piece_tiles * p.d_tiles : 0;
     int64_t share = (items_x * steps_x + items_w * steps_w + pairs - 1) / pairs;
-    share = share < 8 ? 8 : share;
-    auto splits = [&](int64_t steps, int64_t most_splits) {
-        int64_t n = (steps + share - 1) / share;
+    auto splits = [&](int64_t steps, int64_t item, int64_t least, int64_t most_splits) {
+        item = item < least ? least : item;
+        int64_t n = (steps + item - 1) / item;
         n = n > most_splits ? most_splits : n;
         return (int)(n < 1 ? 1 : n);
     };
-    p.splits_x = splits(steps_x, 32);
-    p.splits_w = splits(steps_w, 16);
+    p.splits_x = splits(steps_x, share / 3, 6, 32);
+    p.splits_w = splits(steps_w, share + share / 4, 16, 16);
+    p.direct_w = want_w && p.splits_w == 1 && (!s.norm || p.d_tiles == 1);
     return p;
 }
 
@@ -123,7 +126,7 @@ Forward forward_at(const Shape& s, void* base) {
         return static_cast<void*>(p);
     };
     f.part = static_cast<float2*>(take(s.parts * s.Np * 8));
-    f.block_sums = static_cast<float*>(take((s.N + 31) / 32 * 4));
+    f.block_sums = static_cast<float*>(take((s.N + 7) / 8 * 4));
     if (s.k) f.flags = static_cast<int*>(take(s.N * 4));
     f.bytes = at;
     return f;
@@ -144,7 +147,7 @@ Backward backward_at(const na1d_head& h, const Shape& s, const Pieces& p, bool w
     };
     b.grad = take(s.Np * p.pitch * 2);
     if (want_x) b.part_x = static_cast<float*>(take(p.splits_x * s.Np * s.Dp * 4));
-    if (want_w) b.part_w = static_cast<float*>(take(p.splits_w * p.pitch * s.Dp * 4));
+    if (want_w && !p.direct_w) b.part_w = static_cast<float*>(take(p.splits_w * p.pitch * s.Dp * 4));
     if (h.reduction == NA1D_HEAD_NONE) b.coef = static_cast<float*>(take((s.Np + 1) * 4));
     b.bytes = at;
     return b;
@@ -180,10 +183,10 @@ int backward(const na1d_head& h, void* dx, void* dw, const float* d_loss, void* 
     for (int64_t i = 0; i < p.count; ++i) {
         const int64_t v0 = i * p.pitch, cols = s.V - v0 < p.pitch ? s.V - v0 : p.pitch;
         NA1D_HEAD_TRY(gradients(h, s, sv, b.coef, b.grad, p.pitch, v0, (cols + kTile - 1) / kTile, w, ldw, st));
-        NA1D_HEAD_TRY(products(h, s, sv, b.grad, p, v0, cols, i > 0, b.part_x, b.part_w, w, ldw, st));
         const bool last = i + 1 == p.count;
-        if (dw || last)
-            NA1D_HEAD_TRY(finish(h, s, sv, last ? dx : nullptr, dw, b.part_x, b.part_w, d_loss, b.coef, p.splits_x, p.splits_w, v0, cols, p.pitch, w, ldw, st));
+        const FinishArgs f = finish_args(h, s, sv, last ? dx : nullptr, dw, b.part_x, b.part_w, d_loss, b.coef, p, v0, p.direct_w || !dw ? 0 : cols, w, ldw);
+        NA1D_HEAD_TRY(products(h, s, sv, b.grad, p, v0, cols, i > 0, b.part_x, b.part_w, f, w, ldw, st));
+        if (f.dx || f.cols) NA1D_HEAD_TRY(finish(h, f, st));
     }
     return NA1D_OK;
 }
@@ -217,7 +220,7 @@ int na1d_head_forward(const na1d_head* head, float* loss, void* saved, void* scr
 int na1d_head_backward(const na1d_head* head, void* d_x, void* d_weight, const float* d_loss, void* saved, void* scratch, void* stream) {
     if (int s = na1d::head::check(head)) return s;
     if (!d_loss || !saved || !scratch || (!d_x && !d_weight)) return NA1D_ERR_NULL_POINTER;
-    if (na1d::head::bad_align(saved, 256) || na1d::head::bad_align(scratch, 256) || na1d::head::bad_align(d_x, 16) || na1d::head::bad_align(d_weight, 16) ||
+    if (na1d::head::bad_align(saved, 256) || na1d::head::bad_align(scratch, 256) || na1d::head::bad_align(d_x, 32) || na1d::head::bad_align(d_weight, 32) ||
         na1d::head::bad_align(d_loss, 4))
         return NA1D_ERR_MISALIGNED;
     return na1d::head::backward(*head, d_x, d_weight, d_loss, saved, scratch, (cudaStream_t)stream);

@@ -17,7 +17,7 @@ int api_cuda_status(cudaError_t e);   // a status code, and the error kept for n
 namespace head {
 
 constexpr int kTile = 256;            // rows and classes of a product tile (a pair of CTAs)
-constexpr int kPart = 128;            // classes that one partial maximum and sum stand for
+constexpr int kPart = 64;             // classes that one partial maximum and sum stand for
 constexpr float kSineFloor = 2e-7f;   // of the squared sine in the margin's formula
 constexpr int kIgnored = -1, kBad = -2;
 constexpr int kNoClass = 0x7fffffff;  // behind a row's entries, which are sorted by class
@@ -66,7 +66,8 @@ Saved saved_at(const na1d_head& h, const Shape& s, void* base);
 struct Pieces {
     int64_t tiles, piece_tiles, count, pitch;   // tiles of classes; of a piece; pieces; row pitch of a piece's gradients
     int d_tiles, d_width;                       // tiles over D and their width
-    int splits_x, splits_w;
+    int splits_x, splits_w;                     // of the contractions
+    bool direct_w;                              // the weight's gradient leaves the products as it is: no partial sums
 };
 Pieces pieces_of(const Shape& s, bool want_x, bool want_w);
 
@@ -77,16 +78,31 @@ cudaError_t weight(const na1d_head& h, const Shape& s, const Saved& sv, cudaStre
 cudaError_t combine(const na1d_head& h, const Shape& s, const Saved& sv, const float2* part, float* block_sums, float* loss, const void* w, int64_t ldw,
                     cudaStream_t st);
 cudaError_t coefficients(const na1d_head& h, const Shape& s, const Saved& sv, const float* d_loss, float* coef, cudaStream_t st);
-// gradients of rows v0 .. v0 + cols of the weight (cols may be 0) and, where dx is given, of the rows
-cudaError_t finish(const na1d_head& h, const Shape& s, const Saved& sv, void* dx, void* dw, const float* part_x, const float* part_w, const float* d_loss,
-                   const float* coef, int splits_x, int splits_w, int64_t v0, int64_t cols, int64_t piece_rows, const void* w, int64_t ldw, cudaStream_t st);
+// What the last step of both gradients needs: sums times the common factor, what rounding took from a row's own class, the way back through
+// the normalisation.
+struct FinishArgs {
+    void *dx, *dw;
+    const float *part_x, *part_w, *d_loss, *coef;
+    const void *x, *w;
+    const float *ix, *iw, *slope;
+    const int *place, *target, *own_count, *own;
+    const Words* words;
+    long long Np, piece_rows, ldw;
+    int N, D, Dp, cols, v0, splits_x, splits_w, x_type, w_type, reduction;
+    float factor;
+    bool fp16, norm;
+};
+FinishArgs finish_args(const na1d_head& h, const Shape& s, const Saved& sv, void* dx, void* dw, const float* part_x, const float* part_w, const float* d_loss,
+                       const float* coef, const Pieces& p, int64_t v0, int64_t cols, const void* w, int64_t ldw);
+// the rows' gradients (dx) and, from partial sums, those of a piece of the weight (cols > 0)
+cudaError_t finish(const na1d_head& h, const FinishArgs& a, cudaStream_t st);
 
 // ---- products (na1d_head_logits.cu, na1d_head_grad.cu)
 cudaError_t stats(const na1d_head& h, const Shape& s, const Saved& sv, float2* part, const void* w, int64_t ldw, cudaStream_t st);
 cudaError_t gradients(const na1d_head& h, const Shape& s, const Saved& sv, const float* coef, void* grad, int64_t pitch, int64_t v0, int64_t tiles, const void* w,
                       int64_t ldw, cudaStream_t st);
 cudaError_t products(const na1d_head& h, const Shape& s, const Saved& sv, const void* grad, const Pieces& p, int64_t v0, int64_t cols, bool add, float* part_x,
-                     float* part_w, const void* w, int64_t ldw, cudaStream_t st);
+                     float* part_w, const FinishArgs& f, const void* w, int64_t ldw, cudaStream_t st);
 int logits_read_status();
 int grad_read_status();
 
@@ -106,6 +122,31 @@ __device__ __forceinline__ float gradient_scale(const Words* w, bool fp16, bool 
 // The gradient of a row's own class as it is rounded to 16 bits, in one order of operations: `out` = row_factor(..)
 __device__ __forceinline__ float row_factor(float up, float ix, float coef, bool norm) { return norm ? up * ix * coef : up * coef; }
 __device__ __forceinline__ float own_gradient(float slope, float out, float iw, bool norm) { return norm ? (slope * out) * iw : slope * out; }
+
+// element i of a tensor of one of the three types
+__device__ __forceinline__ float load_any(const void* p, int type, long long i) {
+    if (type == NA1D_FP32) return static_cast<const float*>(p)[i];
+    const unsigned short raw = static_cast<const unsigned short*>(p)[i];
+    return type == NA1D_BF16 ? Cvt<__nv_bfloat16>::from_bits(raw) : Cvt<__half>::from_bits(raw);
+}
+__device__ __forceinline__ void store_any(void* p, int type, long long i, float v) {
+    if (type == NA1D_FP32) static_cast<float*>(p)[i] = v;
+    else if (type == NA1D_BF16) static_cast<__nv_bfloat16*>(p)[i] = __float2bfloat16_rn(v);
+    else static_cast<__half*>(p)[i] = __float2half_rn(v);
+}
+// What rounding took from the gradient of row c's own class (the largest of the row, mostly): it is made good in fp32
+template <typename E>
+__device__ __forceinline__ float own_rest(const FinishArgs& a, int c, float up) {
+    const int v = a.target[c];
+    const float f = own_gradient(a.slope[c], row_factor(up, a.norm ? a.ix[c] : 1.f, a.coef ? a.coef[c] : 1.f, a.norm), a.norm ? a.iw[v] : 1.f, a.norm);
+    const float rest = f - (float)E(f);
+    return fabsf(rest) < INFINITY ? rest : 0.f;
+}
+// what both gradients are multiplied with
+__device__ __forceinline__ float common_factor(const FinishArgs& a, int counted, float up) {
+    const float f = a.factor / up;
+    return a.reduction == NA1D_HEAD_NONE ? f * a.coef[a.Np] : f * (a.d_loss[0] / (a.reduction == NA1D_HEAD_MEAN ? (float)max(counted, 1) : 1.f));
+}
 
 }  // namespace head
 }  // namespace na1d

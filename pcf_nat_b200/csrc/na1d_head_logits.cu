@@ -2,8 +2,8 @@
 //   stats      a running maximum and sum of 2^z per row, over 128 classes at a time
 //   gradient   the gradient of the logits in 16 bits, p minus the target's, for a piece of the classes
 // A pair takes 256 rows and 256 classes: each CTA stages its 128 rows of x and half of the tile's rows of w by TMA (six stages of 64
-// channels), the leader issues the products, and eight warps of each CTA read the accumulators back, a row per lane and half of the columns,
-// while the next tile's products fill the other half of tensor memory.
+// channels), the leader issues the products, and sixteen warps of each CTA read the accumulators back, a row per lane and a quarter of the
+// columns, while the next tile's products fill the other half of tensor memory.
 #include "na1d_head.cuh"
 #include "na1d_mlp.cuh"
 
@@ -13,7 +13,9 @@ namespace {
 
 __device__ int g_head_status = 0;
 
-constexpr int kThreads = 384;                       // warp 0: loads, 1: MMA issue, 2: tensor memory, 4-11: epilogue
+constexpr int kEpilogue = 16;                       // warps; each reaches 32 lanes of tensor memory, and takes a quarter of a tile's columns
+constexpr int kThreads = 128 + 32 * kEpilogue;      // warp 0: loads, 1: MMA issue, 2: tensor memory, from 4 on: epilogue
+constexpr int kWidth = kTile * 4 / kEpilogue;       // columns of a warp
 constexpr int kStep = 64, kHalf = 128;
 constexpr int kOperand = kHalf * kStep * 2;         // 16 KB: 128 rows of 64 channels
 constexpr int kStageBytes = 2 * kOperand;
@@ -21,6 +23,8 @@ constexpr int kStages = 6;
 constexpr int kSmem = kStages * kStageBytes + 1024;
 constexpr uint32_t kCols = 512;
 constexpr int kBand = 16;                           // row tiles that are walked together through the classes
+
+static_assert(kWidth == kPart, "a warp leaves one partial maximum and sum of a row");
 
 struct Barriers {
     uint64_t full[kStages], empty[kStages], acc_full[2], acc_empty[2];
@@ -33,9 +37,10 @@ struct Args {
     const int *row, *target, *index;
     const float *ix, *iw, *lse2, *slope, *coef;
     float* entry;
-    float2* part;               // stats: (classes / 128, Np)
+    float2* part;               // stats: (Np, parts)
     void* grad;                 // gradient: (Np, pitch)
-    long long Np, pitch;
+    long long pitch;
+    int parts;
     int V, v0, tiles, k, steps, tail;   // first class and tiles of classes of this launch; stages of a tile, products of 16 channels in the last one
     float cs;
     bool fp16;
@@ -68,7 +73,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) logits_
 
     if (warp == 0) {
         if (lane < kStages) { ptx::mbar_init(&bar.full[lane], 1); ptx::mbar_init(&bar.empty[lane], 1); }
-        else if (lane < kStages + 2) { ptx::mbar_init(&bar.acc_full[lane - kStages], 1); ptx::mbar_init(&bar.acc_empty[lane - kStages], 16); }
+        else if (lane < kStages + 2) { ptx::mbar_init(&bar.acc_full[lane - kStages], 1); ptx::mbar_init(&bar.acc_empty[lane - kStages], 2 * kEpilogue); }
         else if (lane == kStages + 2) bar.abort = 0;
         ptx::fence_mbar_init();
     } else if (warp == 1 && lane < 2) {
@@ -130,13 +135,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) logits_
             }
         }
     } else if (warp >= 4) {
-        const int q = warp & 3, h = (warp - 4) >> 2;   // tensor-memory lanes 32 q .. + 31 (those a warp reaches), half h of the columns
+        const int q = warp & 3, h = (warp - 4) >> 2;   // tensor-memory lanes 32 q .. + 31 (those a warp reaches), quarter h of the columns
         const uint32_t lanes = (uint32_t)(q * 32) << 16;
         const float up = GRAD ? gradient_scale(g.words, g.fp16, NORM) : 1.f;
         int it = 0;
         for (int i = first; i < items; i += step, ++it) {
             const Tile t = tile_at(i, row_tiles, g.tiles);
-            const int c = t.m * kTile + rank * kHalf + q * 32 + lane, v = g.v0 + t.n * kTile + h * kHalf;
+            const int c = t.m * kTile + rank * kHalf + q * 32 + lane, v = g.v0 + t.n * kTile + h * kWidth;
             const bool live = c < counted;
             const int target = !TOP && live ? g.target[c] : kIgnored;
             // (a row of zeros has no direction: its products are 0 whatever they are multiplied with, and it gets no gradient)
@@ -169,10 +174,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) logits_
             };
             if (!ptx::mbar_wait_relaxed(&bar.acc_full[it & 1], (it >> 1) & 1) || *abort_flag) { atomicExch(&g_head_status, 4); *abort_flag = 1; break; }
             ptx::tc_fence_after_sync();
-            const uint32_t acc = tmem + lanes + (it & 1) * kTile + h * kHalf;
+            const uint32_t acc = tmem + lanes + (it & 1) * kTile + h * kWidth;
             float most = -INFINITY, sum = 0.f;
 #pragma unroll 1
-            for (int n = 0; n < kHalf; n += 32) {
+            for (int n = 0; n < kWidth; n += 32) {
                 float d[32];
                 pair::tmem_ld32(acc + n, d);
                 ptx::tmem_ld_wait();
@@ -200,10 +205,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) logits_
                     if constexpr (TOP) {
                         while (__any_sync(0xffffffffu, next < col + 32)) {
                             if (next < col + 32) {
+                                // (by its bit: indexed, the row would go to local memory)
+                                const uint32_t bit = 1u << (next - col);
                                 float z = 0.f;
 #pragma unroll
-                                for (int j = 0; j < 32; ++j)
-                                    if (j == next - col) z = d[j];
+                                for (int j = 0; j < 32; ++j) z = bit & (1u << j) ? d[j] : z;
                                 entry[pos] = z * cs;
                                 advance();
                             }
@@ -249,9 +255,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) logits_
                         while (__any_sync(0xffffffffu, next < col + 32)) {
                             if (next < col + 32) {
                                 const float f = own_gradient(entry[pos], out, NORM ? __ldg(g.iw + next) : 1.f, NORM);
+                                const uint32_t bit = 1u << (next - col);
 #pragma unroll
-                                for (int j = 0; j < 32; ++j)
-                                    if (j == next - col) d[j] = f;
+                                for (int j = 0; j < 32; ++j) d[j] = bit & (1u << j) ? f : d[j];
                                 advance();
                             }
                         }
@@ -271,7 +277,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) logits_
             ptx::tc_fence_before_sync();
             __syncwarp();
             if (lane == 0) pair::arrive_cluster(pair::in_leader(&bar.acc_empty[it & 1]));
-            if (!GRAD && live) g.part[(size_t)(v / kPart) * g.Np + c] = make_float2(most, sum);
+            if (!GRAD && live) g.part[(size_t)c * g.parts + v / kPart] = make_float2(most, sum);
         }
     }
     __syncwarp();
@@ -297,7 +303,7 @@ template <bool GRAD>
 cudaError_t launch(const na1d_head& h, const Shape& s, const Saved& sv, Args a, const void* w, int64_t ldw, cudaStream_t st) {
     a.words = sv.words; a.row = sv.row; a.target = sv.target; a.index = sv.index; a.entry = sv.entry;
     a.ix = sv.ix; a.iw = sv.iw; a.lse2 = sv.lse2; a.slope = sv.slope;
-    a.Np = s.Np; a.V = (int)s.V; a.k = (int)s.k; a.cs = s.cs; a.fp16 = h.dtype == NA1D_FP16;
+    a.parts = (int)s.parts; a.V = (int)s.V; a.k = (int)s.k; a.cs = s.cs; a.fp16 = h.dtype == NA1D_FP16;
     a.steps = (int)((s.D + kStep - 1) / kStep);
     a.tail = (int)((s.D - (int64_t)(a.steps - 1) * kStep + 15) / 16);
     using B = __nv_bfloat16;

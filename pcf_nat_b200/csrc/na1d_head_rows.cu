@@ -7,17 +7,6 @@ namespace {
 
 constexpr int kWarps = 8, kThreads = 32 * kWarps;
 
-// element i of a tensor of one of the three types
-__device__ __forceinline__ float load_any(const void* p, int type, long long i) {
-    if (type == NA1D_FP32) return static_cast<const float*>(p)[i];
-    const unsigned short raw = static_cast<const unsigned short*>(p)[i];
-    return type == NA1D_BF16 ? Cvt<__nv_bfloat16>::from_bits(raw) : Cvt<__half>::from_bits(raw);
-}
-__device__ __forceinline__ void store_any(void* p, int type, long long i, float v) {
-    if (type == NA1D_FP32) static_cast<float*>(p)[i] = v;
-    else if (type == NA1D_BF16) static_cast<__nv_bfloat16*>(p)[i] = __float2bfloat16_rn(v);
-    else static_cast<__half*>(p)[i] = __float2half_rn(v);
-}
 __device__ __forceinline__ float warp_sum(float v) {
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
@@ -243,110 +232,98 @@ struct CombineArgs {
     int *target, *own_count, *own;
     const float *q, *entry;
     float *gradient, *lse2, *slope, *block_sums, *loss;
-    long long Np;
     int parts, k, reduction;
     float cos_m, sin_m, tau2;
     bool margin;
     Products p;
 };
-// A block takes 32 rows: its warps share out the partial sums (a lane to a row), then take four rows each for what belongs to the target
-// or the teacher's entries. The last block to finish adds up the blocks' sums in their order.
+// A warp takes a row: its partial sums, then what belongs to the target or the teacher's entries. The last block to finish adds up the
+// blocks' sums in their order.
 template <typename E>
 __global__ void __launch_bounds__(kThreads) combine_kernel(const __grid_constant__ CombineArgs a) {
-    __shared__ float top_s[kWarps][32], sum_s[kWarps][32], loss_s[32];
+    __shared__ float loss_s[kWarps];
     __shared__ int last;
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, counted = a.words->counted, c0 = blockIdx.x * 32;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, counted = a.words->counted, c = blockIdx.x * kWarps + warp;
     auto own_row = [&](int v, int c) {   // (in whatever order: they are sorted before they are added up)
         const int n = atomicAdd(a.own_count + v, 1);
         if (n < kOwn) a.own[(size_t)v * kOwn + n] = c;
     };
-    if (c0 < counted) {
-        float most = -INFINITY, sum = 0.f;
-        if (c0 + lane < counted)
-            for (int p = warp; p < a.parts; p += kWarps) {
-                const float2 v = a.part[(size_t)p * a.Np + c0 + lane];
-                const float to = fmaxf(most, v.x), by = to > -INFINITY ? to : 0.f;
-                sum = sum * exp2_fast(most - by) + v.y * exp2_fast(v.x - by);
-                most = to;
-            }
-        top_s[warp][lane] = most;
-        sum_s[warp][lane] = sum;
-        __syncthreads();
-        for (int j = warp; j < 32; j += kWarps) {
-            const int c = c0 + j;
-            float loss = 0.f;
-            if (c < counted) {
-                float m = -INFINITY, s = 0.f;
-#pragma unroll
-                for (int w = 0; w < kWarps; ++w) m = fmaxf(m, top_s[w][j]);
-                const float by = m > -INFINITY ? m : 0.f;
-#pragma unroll
-                for (int w = 0; w < kWarps; ++w) s += sum_s[w][j] * exp2_fast(top_s[w][j] - by);
-                if (a.k == 0) {
-                    const int target = a.target[c];
-                    if (target < 0) {
-                        loss = NAN;
-                        if (lane == 0) a.lse2[c] = NAN;
-                    } else {
-                        float z = logit_of<E>(a.p, c, target, lane), slope = 1.f;
-                        if (a.margin) {   // cos(angle + m) and its derivative
-                            const float sine2 = fmaf(-z, z, 1.f), sine = sqrtf(fmaxf(sine2, kSineFloor));
-                            slope = a.cos_m + (sine2 > kSineFloor ? z / sine : 0.f) * a.sin_m;
-                            z = z * a.cos_m - sine * a.sin_m;
-                        }
-                        z *= a.p.cs;
-                        // the other classes' sum against the target: others = sum 2^(z_v - top), top the largest of all
-                        const float top = fmaxf(m, z), others = s * exp2_fast((m > -INFINITY ? m : top) - top), own = exp2_fast(z - top);
-                        const float all = others + own;
-                        loss = z == top ? log1pf(others) : fmaf(top - z, kLn2, logf(all));
-                        if (lane == 0) {
-                            a.lse2[c] = top + log2f(all);
-                            a.slope[c] = -(others / all) * slope;
-                            own_row(target, c);
-                        }
-                    }
-                } else {
-                    const float lse2 = m + log2f(s);
-                    const size_t at = (size_t)a.row[c] * a.k;
-                    // (a class that comes twice has its entries side by side: all of them take the gradient of the class)
-                    float best = -1.f, own = 0.f;
-                    int own_class = kBad;
-                    for (int e = lane; e < a.k; e += 32) {
-                        const int v = a.index[at + e];
-                        const float q = a.q[at + e];
-                        if (q != q) loss = q;
-                        if (v == kNoClass) continue;
-                        const float z2 = a.entry[at + e] - lse2;
-                        if (q > 0.f) loss += q * (logf(q) - z2 * kLn2);
-                        float all = q;
-                        for (int o = e - 1; o >= 0 && a.index[at + o] == v; --o) all += a.q[at + o];
-                        for (int o = e + 1; o < a.k && a.index[at + o] == v; ++o) all += a.q[at + o];
-                        const float g = exp2_fast(z2) - all;
-                        if (fabsf(g) > best) { best = fabsf(g); own = g; own_class = v; }
-                        a.gradient[at + e] = g;
-                    }
-                    for (int o = 16; o > 0; o >>= 1) {   // the largest of all, the lowest class of equals
-                        const float b = __shfl_xor_sync(0xffffffffu, best, o), g = __shfl_xor_sync(0xffffffffu, own, o);
-                        const int v = __shfl_xor_sync(0xffffffffu, own_class, o);
-                        if (b > best || (b == best && v < own_class)) { best = b; own = g; own_class = v; }
-                    }
-                    if (lane == 0) {
-                        a.target[c] = own_class;
-                        a.slope[c] = own;
-                        if (own_class >= 0) own_row(own_class, c);
-                    }
-                    loss = warp_sum(loss) * a.tau2;
-                    if (lane == 0) a.lse2[c] = loss == loss ? lse2 : NAN;   // (an entry that is no class: nothing of the row counts)
-                }
-                if (a.reduction == NA1D_HEAD_NONE && lane == 0) a.loss[a.row[c]] = loss;
-            }
-            if (lane == 0) loss_s[j] = loss;
+    float loss = 0.f;
+    if (c < counted) {
+        float m = -INFINITY, s = 0.f;
+        const float2* part = a.part + (size_t)c * a.parts;
+        for (int p = lane; p < a.parts; p += 32) {
+            const float2 v = part[p];
+            const float to = fmaxf(m, v.x), by = to > -INFINITY ? to : 0.f;
+            s = s * exp2_fast(m - by) + v.y * exp2_fast(v.x - by);
+            m = to;
         }
-        __syncthreads();
+        const float top = warp_max(m), by = top > -INFINITY ? top : 0.f;
+        s = warp_sum(s * exp2_fast(m - by));
+        m = top;
+        if (a.k == 0) {
+            const int target = a.target[c];
+            if (target < 0) {
+                loss = NAN;
+                if (lane == 0) a.lse2[c] = NAN;
+            } else {
+                float z = logit_of<E>(a.p, c, target, lane), slope = 1.f;
+                if (a.margin) {   // cos(angle + m) and its derivative
+                    const float sine2 = fmaf(-z, z, 1.f), sine = sqrtf(fmaxf(sine2, kSineFloor));
+                    slope = a.cos_m + (sine2 > kSineFloor ? z / sine : 0.f) * a.sin_m;
+                    z = z * a.cos_m - sine * a.sin_m;
+                }
+                z *= a.p.cs;
+                // the other classes' sum against the target: others = sum 2^(z_v - top), top the largest of all
+                const float top = fmaxf(m, z), others = s * exp2_fast((m > -INFINITY ? m : top) - top), own = exp2_fast(z - top);
+                const float all = others + own;
+                loss = z == top ? log1pf(others) : fmaf(top - z, kLn2, logf(all));
+                if (lane == 0) {
+                    a.lse2[c] = top + log2f(all);
+                    a.slope[c] = -(others / all) * slope;
+                    own_row(target, c);
+                }
+            }
+        } else {
+            const float lse2 = m + log2f(s);
+            const size_t at = (size_t)a.row[c] * a.k;
+            // (a class that comes twice has its entries side by side: all of them take the gradient of the class)
+            float best = -1.f, own = 0.f;
+            int own_class = kBad;
+            for (int e = lane; e < a.k; e += 32) {
+                const int v = a.index[at + e];
+                const float q = a.q[at + e];
+                if (q != q) loss = q;
+                if (v == kNoClass) continue;
+                const float z2 = a.entry[at + e] - lse2;
+                if (q > 0.f) loss += q * (logf(q) - z2 * kLn2);
+                float all = q;
+                for (int o = e - 1; o >= 0 && a.index[at + o] == v; --o) all += a.q[at + o];
+                for (int o = e + 1; o < a.k && a.index[at + o] == v; ++o) all += a.q[at + o];
+                const float g = exp2_fast(z2) - all;
+                if (fabsf(g) > best) { best = fabsf(g); own = g; own_class = v; }
+                a.gradient[at + e] = g;
+            }
+            for (int o = 16; o > 0; o >>= 1) {   // the largest of all, the lowest class of equals
+                const float b = __shfl_xor_sync(0xffffffffu, best, o), g = __shfl_xor_sync(0xffffffffu, own, o);
+                const int v = __shfl_xor_sync(0xffffffffu, own_class, o);
+                if (b > best || (b == best && v < own_class)) { best = b; own = g; own_class = v; }
+            }
+            if (lane == 0) {
+                a.target[c] = own_class;
+                a.slope[c] = own;
+                if (own_class >= 0) own_row(own_class, c);
+            }
+            loss = warp_sum(loss) * a.tau2;
+            if (lane == 0) a.lse2[c] = loss == loss ? lse2 : NAN;   // (an entry that is no class: nothing of the row counts)
+        }
+        if (a.reduction == NA1D_HEAD_NONE && lane == 0) a.loss[a.row[c]] = loss;
     }
     if (a.reduction == NA1D_HEAD_NONE) return;
+    if (lane == 0) loss_s[warp] = loss;
+    __syncthreads();
     if (warp == 0) {
-        const float s = c0 < counted ? warp_sum(loss_s[lane]) : 0.f;
+        const float s = warp_sum(lane < kWarps ? loss_s[lane] : 0.f);
         if (lane == 0) {
             a.block_sums[blockIdx.x] = s;
             __threadfence();
@@ -359,11 +336,11 @@ __global__ void __launch_bounds__(kThreads) combine_kernel(const __grid_constant
     float s = 0.f;
     for (int b = threadIdx.x; b < (int)gridDim.x; b += kThreads) s += __ldcg(a.block_sums + b);
     s = warp_sum(s);
-    if (lane == 0) top_s[warp][0] = s;
+    if (lane == 0) loss_s[warp] = s;
     __syncthreads();
     if (threadIdx.x == 0) {
         s = 0.f;
-        for (int w = 0; w < kWarps; ++w) s += top_s[w][0];
+        for (int w = 0; w < kWarps; ++w) s += loss_s[w];
         *a.loss = a.reduction == NA1D_HEAD_MEAN ? s / (float)max(counted, 1) : s;
     }
 }
@@ -386,27 +363,6 @@ __global__ void __launch_bounds__(1024) coefficients_kernel(const float* __restr
     const float r = 1.f / most;
     for (int c = threadIdx.x; c < counted; c += 1024) coef[c] = relative ? d_loss[row[c]] * r : d_loss[row[c]];
     if (threadIdx.x == 0) coef[Np] = most;
-}
-struct FinishArgs {
-    void *dx, *dw;
-    const float *part_x, *part_w, *d_loss, *coef;
-    const void *x, *w;
-    const float *ix, *iw;
-    const float* slope;
-    const int *place, *target, *own_count, *own;
-    Words* words;
-    long long Np, piece_rows, ldw;
-    int N, D, Dp, cols, v0, splits_x, splits_w, x_type, w_type, reduction;
-    float factor;
-    bool fp16, norm;
-};
-// What rounding took from the gradient of row c's own class (the largest of the row, mostly): it is made good in fp32
-template <typename E>
-__device__ __forceinline__ float own_rest(const FinishArgs& a, int c, float up) {
-    const int v = a.target[c];
-    const float f = own_gradient(a.slope[c], row_factor(up, a.norm ? a.ix[c] : 1.f, a.coef ? a.coef[c] : 1.f, a.norm), a.norm ? a.iw[v] : 1.f, a.norm);
-    const float rest = f - (float)E(f);
-    return fabsf(rest) < INFINITY ? rest : 0.f;
 }
 template <typename E>
 __device__ __forceinline__ void unpack_row(const E* row, int j, float* f) { Cvt<E>::unpack(__ldg(reinterpret_cast<const uint4*>(row) + j), f); }
@@ -465,10 +421,7 @@ __device__ __forceinline__ void finish_row(void* out, int type, long long at, co
 template <typename E>
 __global__ void __launch_bounds__(kThreads) finish_kernel(const __grid_constant__ FinishArgs a) {
     const int lane = threadIdx.x & 31, counted = a.words->counted, n = (a.dx ? a.N : 0) + a.cols;
-    const float up = gradient_scale(a.words, a.fp16, a.norm);
-    float f = a.factor / up;
-    if (a.reduction == NA1D_HEAD_NONE) f *= a.coef[a.Np];
-    else f *= a.d_loss[0] / (a.reduction == NA1D_HEAD_MEAN ? (float)max(counted, 1) : 1.f);
+    const float up = gradient_scale(a.words, a.fp16, a.norm), f = common_factor(a, counted, up);
     const E *x = static_cast<const E*>(a.x), *w = static_cast<const E*>(a.w);
     for (int i = blockIdx.x * kWarps + (threadIdx.x >> 5); i < n; i += gridDim.x * kWarps) {
         float rest[kOwn];
@@ -548,12 +501,12 @@ cudaError_t combine(const na1d_head& h, const Shape& s, const Saved& sv, const f
     CombineArgs a = {};
     a.part = part; a.words = sv.words; a.row = sv.row; a.target = sv.target; a.own_count = sv.own_count; a.own = sv.own; a.index = sv.index; a.q = sv.q;
     a.entry = a.gradient = sv.entry; a.lse2 = sv.lse2; a.slope = sv.slope; a.block_sums = block_sums; a.loss = loss;
-    a.Np = s.Np; a.parts = (int)s.parts; a.k = (int)s.k; a.reduction = h.reduction;
+    a.parts = (int)s.parts; a.k = (int)s.k; a.reduction = h.reduction;
     a.margin = s.norm && h.margin != 0.f;
     a.cos_m = (float)cos((double)h.margin); a.sin_m = (float)sin((double)h.margin);
     a.tau2 = h.temperature * h.temperature;
     a.p = products_of(s, sv, w, ldw);
-    const unsigned blocks = (unsigned)((s.N + 31) / 32);
+    const unsigned blocks = (unsigned)((s.N + kWarps - 1) / kWarps);
     if (h.dtype == NA1D_BF16) combine_kernel<__nv_bfloat16><<<blocks, kThreads, 0, st>>>(a);
     else combine_kernel<__half><<<blocks, kThreads, 0, st>>>(a);
     return cudaGetLastError();
@@ -562,17 +515,20 @@ cudaError_t coefficients(const na1d_head& h, const Shape& s, const Saved& sv, co
     coefficients_kernel<<<1, 1024, 0, st>>>(d_loss, sv.words, sv.row, s.Np, h.dtype == NA1D_FP16, coef);
     return cudaGetLastError();
 }
-cudaError_t finish(const na1d_head& h, const Shape& s, const Saved& sv, void* dx, void* dw, const float* part_x, const float* part_w, const float* d_loss,
-                   const float* coef, int splits_x, int splits_w, int64_t v0, int64_t cols, int64_t piece_rows, const void* w, int64_t ldw, cudaStream_t st) {
+FinishArgs finish_args(const na1d_head& h, const Shape& s, const Saved& sv, void* dx, void* dw, const float* part_x, const float* part_w, const float* d_loss,
+                       const float* coef, const Pieces& p, int64_t v0, int64_t cols, const void* w, int64_t ldw) {
     FinishArgs a = {};
     a.dx = dx; a.dw = dw; a.part_x = part_x; a.part_w = part_w; a.d_loss = d_loss; a.coef = coef;
     a.x = sv.x; a.w = w; a.ix = sv.ix; a.iw = sv.iw; a.place = sv.place; a.words = sv.words;
     a.slope = sv.slope; a.target = sv.target; a.own_count = sv.own_count; a.own = sv.own;
-    a.Np = s.Np; a.piece_rows = piece_rows; a.ldw = ldw;
-    a.N = (int)s.N; a.D = (int)s.D; a.Dp = (int)s.Dp; a.cols = dw ? (int)cols : 0; a.v0 = (int)v0; a.splits_x = splits_x; a.splits_w = splits_w;
+    a.Np = s.Np; a.piece_rows = p.pitch; a.ldw = ldw;
+    a.N = (int)s.N; a.D = (int)s.D; a.Dp = (int)s.Dp; a.cols = (int)cols; a.v0 = (int)v0; a.splits_x = p.splits_x; a.splits_w = p.splits_w;
     a.x_type = h.x_type; a.w_type = h.weight_type; a.reduction = h.reduction; a.norm = s.norm; a.fp16 = h.dtype == NA1D_FP16;
     a.factor = s.k ? h.scale * h.temperature : h.scale;
-    const int blocks = blocks_for((dx ? s.N : 0) + a.cols, 148 * 8);
+    return a;
+}
+cudaError_t finish(const na1d_head& h, const FinishArgs& a, cudaStream_t st) {
+    const int blocks = blocks_for((a.dx ? a.N : 0) + a.cols);
     if (h.dtype == NA1D_BF16) finish_kernel<__nv_bfloat16><<<blocks, kThreads, 0, st>>>(a);
     else finish_kernel<__half><<<blocks, kThreads, 0, st>>>(a);
     return cudaGetLastError();

@@ -63,7 +63,7 @@ class _HeadFunction(torch.autograd.Function):
     def forward(ctx, x, weight, labels, teacher_logits, teacher_index, cfg):
         loss, saved, head = _forward(cfg, x, weight, labels, teacher_logits, teacher_index)
         # the weight is read again where it is, unless the forward pass made a copy of its own (then the copy is in `saved`)
-        ctx.in_place = weight.dtype != torch.float32 and weight.stride(0) % 8 == 0 and weight.stride(0) >= weight.shape[1] and weight.data_ptr() % 16 == 0
+        ctx.in_place = weight.dtype != torch.float32 and weight.shape[1] % 8 == 0 and weight.stride(0) % 8 == 0 and weight.stride(0) >= weight.shape[1] and weight.data_ptr() % 16 == 0
         ctx.save_for_backward(saved, weight if ctx.in_place else None)
         ctx.head, ctx.x_dtype, ctx.w_dtype = head, x.dtype, weight.dtype
         ctx.set_materialize_grads(False)

@@ -255,6 +255,16 @@ def test_forms_of_the_inputs(dtype, w_dtype):
         loss.backward()
         assert torch.equal(loss, ref[0]) and torch.equal(xs.grad.reshape(N, D), ref[1])
         assert ws.grad.dtype == ws.dtype and torch.equal(ws.grad.to(dtype), ref[2])
+    # rows of 57 channels in rows of 64, nothing but NaN between them, the last one at the end of its storage
+    gap = torch.full((V * 64 - 7,), float("nan"), dtype=dtype, device=DEV).as_strided((V, 57), (64, 1))
+    gap.copy_(w16[:, :57])
+    odd = gap.detach().requires_grad_()
+    loss = b200.angular_cross_entropy(x[:, :57], odd, y)
+    loss.backward()
+    tight = w16[:, :57].contiguous().requires_grad_()
+    ref57 = b200.angular_cross_entropy(x[:, :57].contiguous(), tight, y)
+    ref57.backward()
+    assert torch.equal(loss, ref57) and torch.equal(odd.grad, tight.grad)
     one = torch.randn(D, device=DEV).to(dtype)                    # a row broadcast to all: its gradient is the rows' sum
     a, b = one.clone().requires_grad_(), one.expand(N, D).contiguous().requires_grad_()
     b200.linear_cross_entropy(a.expand(N, D), w16, y, reduction="sum").backward()
