@@ -147,7 +147,7 @@ Backward backward_at(const na1d_head& h, const Shape& s, const Pieces& p, bool w
     };
     b.grad = take(s.Np * p.pitch * 2);
     if (want_x) b.part_x = static_cast<float*>(take(p.splits_x * s.Np * s.Dp * 4));
-    if (want_w && !p.direct_w) b.part_w = static_cast<float*>(take(p.splits_w * p.pitch * s.Dp * 4));
+    if (want_w) b.part_w = static_cast<float*>(take((p.direct_w ? s.Np : p.splits_w * p.pitch) * s.Dp * 4));   // (direct: rows' own classes alone)
     if (h.reduction == NA1D_HEAD_NONE) b.coef = static_cast<float*>(take((s.Np + 1) * 4));
     b.bytes = at;
     return b;
@@ -184,9 +184,10 @@ int backward(const na1d_head& h, void* dx, void* dw, const float* d_loss, void* 
         const int64_t v0 = i * p.pitch, cols = s.V - v0 < p.pitch ? s.V - v0 : p.pitch;
         NA1D_HEAD_TRY(gradients(h, s, sv, b.coef, b.grad, p.pitch, v0, (cols + kTile - 1) / kTile, w, ldw, st));
         const bool last = i + 1 == p.count;
-        const FinishArgs f = finish_args(h, s, sv, last ? dx : nullptr, dw, b.part_x, b.part_w, d_loss, b.coef, p, v0, p.direct_w || !dw ? 0 : cols, w, ldw);
+        FinishArgs f = finish_args(h, s, sv, last ? dx : nullptr, dw, b.part_x, b.part_w, d_loss, b.coef, p, v0, p.direct_w || !dw ? 0 : cols, w, ldw);
+        f.own_classes = p.direct_w && last;
         NA1D_HEAD_TRY(products(h, s, sv, b.grad, p, v0, cols, i > 0, b.part_x, b.part_w, f, w, ldw, st));
-        if (f.dx || f.cols) NA1D_HEAD_TRY(finish(h, f, st));
+        if (f.dx || f.cols || f.own_classes) NA1D_HEAD_TRY(finish(h, f, st));
     }
     return NA1D_OK;
 }

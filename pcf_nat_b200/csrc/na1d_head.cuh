@@ -91,6 +91,7 @@ struct FinishArgs {
     int N, D, Dp, cols, v0, splits_x, splits_w, x_type, w_type, reduction;
     float factor;
     bool fp16, norm;
+    bool own_classes;           // part_w has the sums of classes that are rows' own, at such a row
 };
 FinishArgs finish_args(const na1d_head& h, const Shape& s, const Saved& sv, void* dx, void* dw, const float* part_x, const float* part_w, const float* d_loss,
                        const float* coef, const Pieces& p, int64_t v0, int64_t cols, const void* w, int64_t ldw);

@@ -14,26 +14,28 @@ namespace {
 
 __device__ int g_head_status = 0;
 
-constexpr int kThreads = 384;                       // warp 0: loads, 1: MMA issue, 2: tensor memory, 4-11: results
+constexpr int kEpilogue = 16;                       // warps; each reaches 32 lanes of tensor memory, and takes every fourth 16 columns
+constexpr int kThreads = 128 + 32 * kEpilogue;      // warp 0: loads, 1: MMA issue, 2: tensor memory, 3: the plan, from 4 on: results
 constexpr int kStep = 64, kHalf = 128;              // contraction steps of a stage; rows of G's side in one CTA
 constexpr int kBox = 64 * kStep * 2;                // 64 columns of a stage
 constexpr int kOperand = 2 * kBox;
 constexpr int kStageBytes = 2 * kOperand;
-constexpr int kStages = 6;
-constexpr int kSmem = kStages * kStageBytes + 1024;
+constexpr int kOwnBox = 64 * kHalf * 2;             // 64 columns of the classes' own rows
+constexpr int kMostStages = 6;
+constexpr int kMostSmem = 232448 - 5 * 1024;        // (static: barriers, the plan, sums of four warps)
 constexpr uint32_t kCols = 512;
 
 struct Barriers {
-    uint64_t full[kStages], empty[kStages], acc_full[2], acc_empty[2];
+    uint64_t full[kMostStages], empty[kMostStages], acc_full[2], acc_empty[2], own_full, own_free, along;
     uint32_t tmem;
     int abort;
 };
-struct Maps { CUtensorMap g_rows, g_cols, x, w; };   // G with its contraction along and across its rows
+struct Maps { CUtensorMap g_rows, g_cols, x, w, own; };   // G with its contraction along and across its rows; w for a product, and as it is
 struct Args {
     const Words* words;
     float *part_x, *part_w;
     long long Np, Dq, piece_rows;                    // rows of a split's partial sums and their pitch
-    int D, d_tiles, d_width, v0, cols, tiles, splits_x, splits_w;
+    int D, d_tiles, d_width, v0, cols, tiles, splits_x, splits_w, stages;
     bool want_x, want_w, add, direct;
     FinishArgs f;
 };
@@ -104,118 +106,60 @@ __device__ __forceinline__ bool next_item(const Args& g, const Plan& p, Walk& w,
     return true;
 }
 
-// A class's gradient straight from the accumulators: what rounding took from the rows whose own class it is, the way back through the
-// normalisation (both warps of a row go through all of its columns for that), the common factor. Lane: a row of the tile.
+__device__ __forceinline__ void load_tile(void* dst, const CUtensorMap* map, uint64_t* bar, int c0, int c1) {   // this CTA's own
+    asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];"
+                 ::"r"(ptx::smem_u32(dst)), "l"(reinterpret_cast<uint64_t>(map)), "r"(ptx::smem_u32(bar)), "r"(c0), "r"(c1) : "memory");
+}
+// one addition to each of four places that nothing else in the launch touches: nothing waits for what was there
+__device__ __forceinline__ void add4(float* p, const float* d) {
+    asm volatile("red.relaxed.gpu.global.add.v4.f32 [%0], {%1, %2, %3, %4};" ::"l"(p), "f"(d[0]), "f"(d[1]), "f"(d[2]), "f"(d[3]) : "memory");
+}
+// sixteen columns of a class's gradient as they are wanted
 template <typename E>
-__device__ __forceinline__ void direct_rows(const Args& g, const Item& t, int r, bool live, float factor, float up, uint32_t acc, int n0, int n1, bool empty) {
-    const FinishArgs& f = g.f;
-    const int v = g.v0 + r;
-    const int count = live ? f.own_count[v] : 0, rows = count <= kOwn ? count : 0;   // (of many rows the roundings average out)
-    const E *x = static_cast<const E*>(f.x), *own = static_cast<const E*>(f.w) + (size_t)(live ? v : 0) * f.ldw;
-    const int* mine = f.own + (size_t)(live ? v : 0) * kOwn;
-    // sixteen columns of the sum, the rows' shares in the order of the rows
-    auto columns = [&](int n, float* d) {
-#pragma unroll
-        for (int j = 0; j < 16; ++j) d[j] = 0.f;
-        if (!empty) {
-            pair::tmem_ld16(acc + n, d);
-            ptx::tmem_ld_wait();
+__device__ __forceinline__ void store_columns(const FinishArgs& f, int v, int col, const float* d) {
+    const long long at = (long long)v * f.D + col;
+    if (f.w_type != NA1D_FP32 && f.D % 16 == 0) {
+        if (col < f.D) {
+            const uint4 a = Cvt<E>::pack(d), b = Cvt<E>::pack(d + 8);
+            const uint32_t s[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+            store_sector(static_cast<E*>(f.dw) + at, s);
         }
-        int before = -1;
-        for (int i = 0; i < rows; ++i) {
-            int c = kNoClass;
-            for (int o = 0; o < rows; ++o) {
-                const int m = __ldg(mine + o);
-                if (m > before && m < c) c = m;
+    } else if (f.D % 8 == 0) {
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
+            if (col + 8 * j < f.D) {
+                if (f.w_type == NA1D_FP32) store_sector(static_cast<float*>(f.dw) + at + 8 * j, reinterpret_cast<const uint32_t*>(d + 8 * j));
+                else *reinterpret_cast<uint4*>(static_cast<E*>(f.dw) + at + 8 * j) = Cvt<E>::pack(d + 8 * j);
             }
-            before = c;
-            const float rest = own_rest<E>(f, c, up);
+    } else {
 #pragma unroll
-            for (int j = 0; j < 2; ++j)
-                if (t.n0 + n + 8 * j < f.D) {
-                    float e[8];
-                    Cvt<E>::unpack(__ldg(reinterpret_cast<const uint4*>(x + (size_t)c * f.Dp + t.n0 + n) + j), e);
-#pragma unroll
-                    for (int k = 0; k < 8; ++k) d[8 * j + k] = fmaf(rest, e[k], d[8 * j + k]);
-                }
-        }
-    };
-    auto own_columns = [&](int n, float* e) {   // (rows of D up to a multiple of 8 are there, zeros behind D)
-#pragma unroll
-        for (int j = 0; j < 2; ++j) {
-            if (live && t.n0 + n + 8 * j < f.D) Cvt<E>::unpack(__ldg(reinterpret_cast<const uint4*>(own + t.n0 + n) + j), e + 8 * j);
-            else
-#pragma unroll
-                for (int k = 0; k < 8; ++k) e[8 * j + k] = 0.f;
-        }
-    };
-    float along = 0.f;
-    if (f.norm) {
-#pragma unroll 1
-        for (int n = 0; n < g.d_width; n += 16) {
-            float d[16], e[16];
-            columns(n, d);
-            own_columns(n, e);
-#pragma unroll
-            for (int j = 0; j < 16; ++j) along = fmaf(d[j], e[j], along);
-        }
-        const float iw = live ? f.iw[v] : 0.f;
-        along *= iw * iw;
-    }
-#pragma unroll 1
-    for (int n = n0; n < n1; n += 16) {
-        float d[16];
-        columns(n, d);
-        if (f.norm) {
-            float e[16];
-            own_columns(n, e);
-#pragma unroll
-            for (int j = 0; j < 16; ++j) d[j] = fmaf(-along, e[j], d[j]);
-        }
-#pragma unroll
-        for (int j = 0; j < 16; ++j) d[j] *= factor;
-        const int col = t.n0 + n;
-        const long long at = (long long)v * f.D + col;
-        if (!live) continue;
-        if (f.w_type != NA1D_FP32 && f.D % 16 == 0) {
-            if (col < f.D) {
-                const uint4 a = Cvt<E>::pack(d), b = Cvt<E>::pack(d + 8);
-                const uint32_t s[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
-                store_sector(static_cast<E*>(f.dw) + at, s);
-            }
-        } else if (f.D % 8 == 0) {
-#pragma unroll
-            for (int j = 0; j < 2; ++j)
-                if (col + 8 * j < f.D) {
-                    if (f.w_type == NA1D_FP32) store_sector(static_cast<float*>(f.dw) + at + 8 * j, reinterpret_cast<const uint32_t*>(d + 8 * j));
-                    else *reinterpret_cast<uint4*>(static_cast<E*>(f.dw) + at + 8 * j) = Cvt<E>::pack(d + 8 * j);
-                }
-        } else {
-#pragma unroll
-            for (int j = 0; j < 16; ++j)
-                if (col + j < f.D) store_any(f.dw, f.w_type, at + j, d[j]);
-        }
+        for (int j = 0; j < 16; ++j)
+            if (col + j < f.D) store_any(f.dw, f.w_type, at + j, d[j]);
     }
 }
 
-template <typename E>
+// PROJECT: the classes' own rows are staged too, for the way back through the normalisation
+template <typename E, bool PROJECT>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) grad_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Args g) {
+    const int kStages = PROJECT ? g.stages : kMostStages;   // (the staged classes take the others' place)
     extern __shared__ uint8_t raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~(uintptr_t)1023);
+    uint8_t* own_rows = smem + kStages * kStageBytes;
     __shared__ Barriers bar;
+    __shared__ Plan plan_s;
+    __shared__ float along_s[2][4][kHalf];
     const int warp = ptx::warp_index(), lane = threadIdx.x & 31;
     const uint32_t rank = pair::cta_rank();
-    __shared__ Plan plan_s;
     const int pair_index = blockIdx.x >> 1, pairs = gridDim.x >> 1;
     volatile int* abort_flag = &bar.abort;
 
     if (warp == 0) {
         if (lane < kStages) { ptx::mbar_init(&bar.full[lane], 1); ptx::mbar_init(&bar.empty[lane], 1); }
-        else if (lane < kStages + 2) { ptx::mbar_init(&bar.acc_full[lane - kStages], 1); ptx::mbar_init(&bar.acc_empty[lane - kStages], 16); }
-        else if (lane == kStages + 2) bar.abort = 0;
+        else if (lane < kStages + 2) { ptx::mbar_init(&bar.acc_full[lane - kStages], 1); ptx::mbar_init(&bar.acc_empty[lane - kStages], 2 * kEpilogue); }
+        else if (lane == kStages + 2) { ptx::mbar_init(&bar.own_full, 1); ptx::mbar_init(&bar.own_free, kEpilogue); ptx::mbar_init(&bar.along, kEpilogue); bar.abort = 0; }
         ptx::fence_mbar_init();
-    } else if (warp == 1 && lane < 4) {
-        ptx::prefetch_tensormap(lane == 0 ? &maps.g_rows : lane == 1 ? &maps.g_cols : lane == 2 ? &maps.x : &maps.w);
+    } else if (warp == 1 && lane < 5) {
+        ptx::prefetch_tensormap(lane == 0 ? &maps.g_rows : lane == 1 ? &maps.g_cols : lane == 2 ? &maps.x : lane == 3 ? &maps.w : &maps.own);
     }
     if (warp == 2) { pair::tmem_alloc(&bar.tmem, kCols); pair::tmem_relinquish(); }
     if (warp == 3 && lane == 0) plan_s = plan_of(g, pairs);
@@ -231,10 +175,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) grad_ke
 
     if (warp == 0) {
         if (ptx::elect_one()) {
-            int slot = 0, n = 0;
+            int slot = 0, n = 0, projected = 0;
             uint32_t phase = 1;   // the first round finds the slots empty
             bool ok = true;
             const bool two = half_width > 64;
+            const int own_boxes = (g.D + 63) / 64;
             while (ok && next_item(g, p, walk, pairs, t)) {
                 const CUtensorMap* mb = t.rows ? &maps.w : &maps.x;
                 const int m = t.m0 + rank * kHalf, d = t.n0 + rank * half_width, r0 = t.rows ? g.v0 : 0;
@@ -254,9 +199,18 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) grad_ke
                     ++n;
                     if (++slot == kStages) { slot = 0; phase ^= 1; }
                 }
+                if (PROJECT && ok && !t.rows) {   // (last: the epilogue of the item before may still read the rows that were there)
+                    if (!ptx::mbar_wait_relaxed(&bar.own_free, (projected & 1) ^ 1) || *abort_flag) { atomicExch(&g_head_status, 5); *abort_flag = 1; ok = false; break; }
+                    ptx::mbar_expect_tx(&bar.own_full, own_boxes * kOwnBox);
+                    for (int b = 0; b < own_boxes; ++b) load_tile(own_rows + b * kOwnBox, &maps.own, &bar.own_full, b * 64, g.v0 + m);
+                    ++projected;
+                }
             }
-            if (!ok && rank == 0)   // loads that are on their way arrive before the CTAs leave
-                for (int j = n - 1; j >= 0 && j >= n - kStages; --j) ptx::mbar_wait(&bar.full[j % kStages], (j / kStages) & 1, 1u << 14);
+            if (!ok) {   // loads that are on their way arrive before the CTAs leave
+                if (rank == 0)
+                    for (int j = n - 1; j >= 0 && j >= n - kStages; --j) ptx::mbar_wait(&bar.full[j % kStages], (j / kStages) & 1, 1u << 14);
+                if (projected > 0) ptx::mbar_wait(&bar.own_full, (projected - 1) & 1, 1u << 14);
+            }
         }
     } else if (warp == 1) {
         if (rank == 0 && ptx::elect_one()) {
@@ -285,49 +239,96 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) grad_ke
             }
         }
     } else if (warp >= 4) {
-        const int q = warp & 3, h = (warp - 4) >> 2;   // tensor-memory lanes 32 q .. + 31 (those a warp reaches), half h of the columns
+        const int q = warp & 3, h = (warp - 4) >> 2;   // tensor-memory lanes 32 q .. + 31 (those a warp reaches); columns 16 h, 16 h + 64, ..
         const uint32_t lanes = (uint32_t)(q * 32) << 16;
-        const int counted = g.words->counted;
-        const float up = gradient_scale(g.words, g.f.fp16, g.f.norm), factor = g.direct ? common_factor(g.f, counted, up) : 1.f;
-        int it = 0;
+        const int counted = g.words->counted, row = q * 32 + lane;
+        const float factor = g.direct ? common_factor(g.f, counted, gradient_scale(g.words, g.f.fp16, g.f.norm)) : 1.f;
+        const uint8_t* own_row = own_rows + row * 128;
+        int it = 0, projected = 0;
         while (next_item(g, p, walk, pairs, t)) {
             const bool empty = t.k0 == t.k1;           // a split without steps: zeros
             if (empty && t.rows && g.add) continue;
-            const int r = t.m0 + rank * kHalf + q * 32 + lane;
-            const bool live = r < (t.rows ? counted : g.cols);
-            float* dst = (t.rows ? g.part_x + (size_t)t.split * g.Np * g.Dq : g.part_w + (size_t)t.split * g.piece_rows * g.Dq) + (size_t)r * g.Dq + t.n0;
+            const int r = t.m0 + rank * kHalf + row, v = g.v0 + r;
+            const bool live = r < (t.rows ? counted : g.cols), direct = g.direct && !t.rows;
+            float* dst = t.rows ? g.part_x + (size_t)t.split * g.Np * g.Dq + (size_t)r * g.Dq : g.part_w + (size_t)t.split * g.piece_rows * g.Dq + (size_t)r * g.Dq;
+            bool whole = !direct;                      // an fp32 sum at dst
+            float iw = 0.f;
+            if (direct && live) {
+                // a class that is some rows' own (and not that of many, whose roundings average out) gets what rounding took in the last step
+                const int count = g.f.own_count[v];
+                whole = count > 0 && count <= kOwn;
+                if (whole) dst = g.part_w + (size_t)g.f.own[(size_t)v * kOwn] * g.Dq;
+                if (PROJECT) iw = g.f.iw[v];
+            }
             if (!empty) {
                 if (!ptx::mbar_wait_relaxed(&bar.acc_full[it & 1], (it >> 1) & 1) || *abort_flag) { atomicExch(&g_head_status, 4); *abort_flag = 1; break; }
                 ptx::tc_fence_after_sync();
             }
-            if (g.direct && !t.rows) {
-                direct_rows<E>(g, t, r, live, factor, up, tmem + lanes + (it & 1) * kTile, h * half_width, (h + 1) * half_width, empty);
-                if (!empty) {
-                    ptx::tc_fence_before_sync();
-                    __syncwarp();
-                    if (lane == 0) pair::arrive_cluster(pair::in_leader(&bar.acc_empty[it & 1]));
-                    ++it;
-                }
-                continue;
-            }
-#pragma unroll 1
-            for (int n = h * half_width; n < (h + 1) * half_width; n += 16) {
-                float d[16] = {};
-                if (!empty) {
-                    pair::tmem_ld16(tmem + lanes + (it & 1) * kTile + n, d);
+            const uint32_t acc = tmem + lanes + (it & 1) * kTile;
+            auto columns = [&](int n, float* d) {
+                if (empty) {
+#pragma unroll
+                    for (int j = 0; j < 16; ++j) d[j] = 0.f;
+                } else {
+                    pair::tmem_ld16(acc + n, d);
                     ptx::tmem_ld_wait();
                 }
+            };
+            auto own_columns = [&](int n, float* e) {   // of the staged row: 16-byte pieces, swizzled
+                const uint8_t* box = own_row + (n >> 6) * kOwnBox;
 #pragma unroll
-                for (int j = 0; j < 2; ++j)
-                    if (live && t.n0 + n + 8 * j < g.D) {
-                        float* at = dst + n + 8 * j;
-                        if (t.rows && g.add) {
-                            const float4 a = reinterpret_cast<const float4*>(at)[0], b = reinterpret_cast<const float4*>(at)[1];
-                            d[8 * j] += a.x; d[8 * j + 1] += a.y; d[8 * j + 2] += a.z; d[8 * j + 3] += a.w;
-                            d[8 * j + 4] += b.x; d[8 * j + 5] += b.y; d[8 * j + 6] += b.z; d[8 * j + 7] += b.w;
+                for (int j = 0; j < 2; ++j) Cvt<E>::unpack(*reinterpret_cast<const uint4*>(box + (((((n & 63) >> 3) + j) ^ (row & 7)) << 4)), e + 8 * j);
+            };
+            float along = 0.f;
+            if (PROJECT && direct) {
+                if (!ptx::mbar_wait_relaxed(&bar.own_full, projected & 1) || *abort_flag) { atomicExch(&g_head_status, 6); *abort_flag = 1; break; }
+#pragma unroll 1
+                for (int n = 16 * h; n < g.d_width; n += 64) {
+                    float d[16], e[16];
+                    columns(n, d);
+                    own_columns(n, e);
+#pragma unroll
+                    for (int j = 0; j < 16; ++j) along = fmaf(d[j], e[j], along);
+                }
+                along_s[projected & 1][h][row] = along;
+                __syncwarp();
+                if (lane == 0) ptx::mbar_arrive(&bar.along);
+                if (!ptx::mbar_wait(&bar.along, projected & 1) || *abort_flag) { atomicExch(&g_head_status, 7); *abort_flag = 1; break; }
+                const float(*sums)[kHalf] = along_s[projected & 1];
+                along = ((sums[0][row] + sums[1][row]) + (sums[2][row] + sums[3][row])) * iw * iw;
+            }
+#pragma unroll 1
+            for (int n = 16 * h; n < g.d_width; n += 64) {
+                float d[16];
+                columns(n, d);
+                const int col = t.n0 + n;
+                if (live && whole) {
+#pragma unroll
+                    for (int j = 0; j < 2; ++j)
+                        if (col + 8 * j < g.D) {
+                            if (t.rows && g.add) {
+                                add4(dst + col + 8 * j, d + 8 * j);
+                                add4(dst + col + 8 * j + 4, d + 8 * j + 4);
+                            } else {
+                                store_sector(dst + col + 8 * j, reinterpret_cast<const uint32_t*>(d + 8 * j));
+                            }
                         }
-                        store_sector(at, reinterpret_cast<const uint32_t*>(d + 8 * j));
+                } else if (live) {
+                    if (PROJECT) {
+                        float e[16];
+                        own_columns(n, e);
+#pragma unroll
+                        for (int j = 0; j < 16; ++j) d[j] = fmaf(-along, e[j], d[j]);
                     }
+#pragma unroll
+                    for (int j = 0; j < 16; ++j) d[j] *= factor;
+                    store_columns<E>(g.f, v, col, d);
+                }
+            }
+            if (PROJECT && direct) {
+                ++projected;
+                __syncwarp();
+                if (lane == 0) ptx::mbar_arrive(&bar.own_free);
             }
             if (!empty) {
                 ptx::tc_fence_before_sync();
@@ -344,19 +345,23 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) grad_ke
     if (warp == 2) pair::tmem_dealloc(tmem, kCols);
 }
 
-template <typename E>
-cudaError_t run(const Shape& s, const Saved& sv, const void* grad, const Args& a, int64_t pitch, const void* w, int64_t ldw, int dtype, cudaStream_t st) {
+template <typename E, bool PROJECT>
+cudaError_t run(const Shape& s, const Saved& sv, const void* grad, Args a, int64_t pitch, const void* w, int64_t ldw, int dtype, cudaStream_t st) {
     Maps maps;
     const int64_t dg[2] = {pitch, s.Np}, sg[1] = {pitch}, dx[2] = {s.D, s.Np}, sx[1] = {s.Dp}, dw[2] = {s.D, s.V}, sw[1] = {ldw};
     const int along[2] = {64, kHalf}, across[2] = {64, kStep};
     if (!make_matrix_map(&maps.g_rows, grad, dtype, 2, dg, sg, along) || !make_matrix_map(&maps.g_cols, grad, dtype, 2, dg, sg, across) ||
-        !make_matrix_map(&maps.x, sv.x, dtype, 2, dx, sx, across) || !make_matrix_map(&maps.w, w, dtype, 2, dw, sw, across))
+        !make_matrix_map(&maps.x, sv.x, dtype, 2, dx, sx, across) || !make_matrix_map(&maps.w, w, dtype, 2, dw, sw, across) ||
+        !make_matrix_map(&maps.own, w, dtype, 2, dw, sw, along))
         return cudaErrorInvalidValue;
-    auto* kern = grad_kernel<E>;
-    if (cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem)) return e;
+    auto* kern = grad_kernel<E, PROJECT>;
+    const int own_bytes = PROJECT ? (int)((s.D + 63) / 64) * kOwnBox : 0, fit = (kMostSmem - 1024 - own_bytes) / kStageBytes;
+    a.stages = fit < kMostStages ? fit : kMostStages;
+    const int smem = a.stages * kStageBytes + own_bytes + 1024;
+    if (cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem)) return e;
     const int64_t items = (a.want_x ? s.Np / kTile * a.d_tiles * a.splits_x : 0) + (a.want_w ? (int64_t)a.tiles * a.d_tiles * a.splits_w : 0);
     const int64_t pairs = device_sm_count() / 2;
-    kern<<<2 * (int)(items < pairs ? items : pairs), kThreads, kSmem, st>>>(maps, a);
+    kern<<<2 * (int)(items < pairs ? items : pairs), kThreads, smem, st>>>(maps, a);
     return cudaGetLastError();
 }
 
@@ -369,9 +374,11 @@ cudaError_t products(const na1d_head& h, const Shape& s, const Saved& sv, const 
     a.Np = s.Np; a.Dq = s.Dp; a.piece_rows = p.pitch;
     a.D = (int)s.D; a.d_tiles = p.d_tiles; a.d_width = p.d_width; a.v0 = (int)v0; a.cols = (int)cols;
     a.tiles = (int)((cols + kTile - 1) / kTile); a.splits_x = p.splits_x; a.splits_w = p.splits_w;
-    a.want_x = part_x != nullptr; a.want_w = p.direct_w || part_w != nullptr; a.add = add; a.direct = p.direct_w;
+    a.want_x = part_x != nullptr; a.want_w = part_w != nullptr; a.add = add; a.direct = p.direct_w;
     a.f = f;
-    return h.dtype == NA1D_BF16 ? run<__nv_bfloat16>(s, sv, grad, a, p.pitch, w, ldw, 0, st) : run<__half>(s, sv, grad, a, p.pitch, w, ldw, 1, st);
+    const bool project = p.direct_w && s.norm;
+    if (h.dtype == NA1D_BF16) return project ? run<__nv_bfloat16, true>(s, sv, grad, a, p.pitch, w, ldw, 0, st) : run<__nv_bfloat16, false>(s, sv, grad, a, p.pitch, w, ldw, 0, st);
+    return project ? run<__half, true>(s, sv, grad, a, p.pitch, w, ldw, 1, st) : run<__half, false>(s, sv, grad, a, p.pitch, w, ldw, 1, st);
 }
 int grad_read_status() {
     int v = 0, zero = 0;

@@ -63,13 +63,16 @@ __device__ __forceinline__ float copy_row(E* dst, const void* src, int type, lon
 // entry counts with a class in [0, V); one beyond (or a logit that is no number) makes the row's probabilities NaN.
 __global__ void __launch_bounds__(kThreads) teacher_kernel(const float* __restrict__ logits, const int64_t* __restrict__ index, int N, int k, long long V, float rt,
                                                            float* __restrict__ q, int* __restrict__ out, int* __restrict__ flags) {
+    extern __shared__ int classes_s[];   // a warp's row: kNoClass and behind it for what is no class
     const int i = blockIdx.x * kWarps + (threadIdx.x >> 5), lane = threadIdx.x & 31;
     if (i >= N) return;
+    int* classes = classes_s + (threadIdx.x >> 5) * k;
     const size_t at = (size_t)i * k;
     float most = -INFINITY;
     bool bad = false;
     for (int j = lane; j < k; j += 32) {
         const int64_t v = index[at + j];
+        classes[j] = v < 0 ? kNoClass : v < V ? (int)v : kNoClass - 1;
         if (v < 0) continue;
         const float t = logits[at + j] * rt;
         bad |= v >= V || t != t || t == INFINITY;
@@ -77,20 +80,22 @@ __global__ void __launch_bounds__(kThreads) teacher_kernel(const float* __restri
     }
     most = warp_max(most);
     bad = __any_sync(0xffffffffu, bad);
-    auto weight = [&](int j) { return index[at + j] >= 0 && most > -INFINITY ? expf(logits[at + j] * rt - most) : 0.f; };
+    auto weight = [&](int j) { return classes[j] != kNoClass && most > -INFINITY ? expf(logits[at + j] * rt - most) : 0.f; };
     float sum = 0.f;
     for (int j = lane; j < k; j += 32) sum += weight(j);
     sum = warp_sum(sum);
     const float r = 1.f / sum;
+    __syncwarp();
     for (int j = lane; j < k; j += 32) {
-        const int64_t v = index[at + j];
-        int rank = 0;   // entries without a class come last
+        const int v = classes[j];
+        int rank = 0;
+#pragma unroll 4
         for (int o = 0; o < k; ++o) {
-            const int64_t u = index[at + o];
-            rank += (v >= 0 ? u >= 0 && (u < v || (u == v && o < j)) : u >= 0 || o < j);
+            const int u = classes[o];
+            rank += u < v || (u == v && o < j);
         }
-        q[at + rank] = v < 0 ? 0.f : bad ? NAN : most > -INFINITY ? weight(j) * r : 0.f;
-        out[at + rank] = v >= 0 && v < V ? (int)v : kNoClass;
+        q[at + rank] = v == kNoClass ? 0.f : bad ? NAN : most > -INFINITY ? weight(j) * r : 0.f;
+        out[at + rank] = v < kNoClass - 1 ? v : kNoClass;
     }
     if (lane == 0) flags[i] = bad || most > -INFINITY;
 }
@@ -113,7 +118,7 @@ struct RowArgs {
 template <typename E>
 __global__ void __launch_bounds__(kThreads) rows_kernel(const __grid_constant__ RowArgs a) {
     __shared__ int sums[kWarps], places[kThreads], base_s;
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, r0 = blockIdx.x * a.per_block, r1 = min(a.N, r0 + a.per_block);
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, r0 = min(a.N, (int)blockIdx.x * a.per_block), r1 = min(a.N, r0 + a.per_block);
     auto counts = [&](int i) { return a.flags ? a.flags[i] != 0 : a.labels[i] != a.ignore; };
     int before = 0;
     for (int i = threadIdx.x; i < r0; i += kThreads) before += counts(i);
@@ -168,10 +173,11 @@ __global__ void __launch_bounds__(kThreads) rows_kernel(const __grid_constant__ 
         base += total;
         __syncthreads();
     }
-    for (int p = a.N + blockIdx.x; p < a.Np; p += gridDim.x)
-        for (int e = threadIdx.x; e < a.Dp / 8; e += kThreads) reinterpret_cast<uint4*>(out + (size_t)p * a.Dp)[e] = make_uint4(0, 0, 0, 0);
+    const long long pad = (long long)(a.Np - a.N) * (a.Dp / 8);   // 16-byte pieces behind the last row
+    for (long long e = (long long)blockIdx.x * kThreads + threadIdx.x; e < pad; e += (long long)gridDim.x * kThreads)
+        reinterpret_cast<uint4*>(out + (size_t)a.N * a.Dp)[e] = make_uint4(0, 0, 0, 0);
     if (a.norm && lane == 0 && most > 0.f) atomicMax(&a.words->most_ix, __float_as_int(most));   // (the largest, in whatever order)
-    if (r1 == a.N && threadIdx.x == 0) a.words->counted = base;
+    if (r0 < a.N && r1 == a.N && threadIdx.x == 0) a.words->counted = base;
 }
 
 // ---------------------------------------------------------------- the weight
@@ -420,39 +426,46 @@ __device__ __forceinline__ void finish_row(void* out, int type, long long at, co
 }
 template <typename E>
 __global__ void __launch_bounds__(kThreads) finish_kernel(const __grid_constant__ FinishArgs a) {
-    const int lane = threadIdx.x & 31, counted = a.words->counted, n = (a.dx ? a.N : 0) + a.cols;
+    const int lane = threadIdx.x & 31, counted = a.words->counted, n = (a.dx || a.own_classes ? a.N : 0) + a.cols;
     const float up = gradient_scale(a.words, a.fp16, a.norm), f = common_factor(a, counted, up);
     const E *x = static_cast<const E*>(a.x), *w = static_cast<const E*>(a.w);
-    for (int i = blockIdx.x * kWarps + (threadIdx.x >> 5); i < n; i += gridDim.x * kWarps) {
+    auto class_row = [&](int v, const float* part, long long split, int splits) {
         float rest[kOwn];
+        int rows_in_order[kOwn];
+        const int count = a.own_count[v], rows = count <= kOwn ? count : 0;   // (of many rows the roundings average out)
+        if (rows) {
+            const int mine = lane < rows ? a.own[(size_t)v * kOwn + lane] : kNoClass;
+            int rank = 0;
+#pragma unroll
+            for (int o = 0; o < kOwn; ++o) rank += __shfl_sync(0xffffffffu, mine, o) < mine;
+#pragma unroll
+            for (int o = 0; o < kOwn; ++o) {
+                const unsigned who = __ballot_sync(0xffffffffu, lane < rows && rank == o);
+                rows_in_order[o] = __shfl_sync(0xffffffffu, mine, who ? __ffs(who) - 1 : 0);
+                rest[o] = o < rows ? own_rest<E>(a, rows_in_order[o], up) : 0.f;
+            }
+        }
+        finish_row<E>(a.dw, a.w_type, (long long)v * a.D, part, split, splits, w + (size_t)v * a.ldw, a.norm ? a.iw[v] : 1.f, f, rows, rest,
+                      [&](int o) { return x + (size_t)rows_in_order[o] * a.Dp; }, a.norm, a.D, a.Dp, lane);
+    };
+    for (int i = blockIdx.x * kWarps + (threadIdx.x >> 5); i < n; i += gridDim.x * kWarps) {
         if (i < a.cols) {
-            const int v = a.v0 + i, count = a.own_count[v], rows = count <= kOwn ? count : 0;   // (of many rows the roundings average out)
-            int rows_in_order[kOwn];
-            if (rows) {
-                const int mine = lane < rows ? a.own[(size_t)v * kOwn + lane] : kNoClass;
-                int rank = 0;
-#pragma unroll
-                for (int o = 0; o < kOwn; ++o) rank += __shfl_sync(0xffffffffu, mine, o) < mine;
-#pragma unroll
-                for (int o = 0; o < kOwn; ++o) {
-                    const unsigned who = __ballot_sync(0xffffffffu, lane < rows && rank == o);
-                    rows_in_order[o] = __shfl_sync(0xffffffffu, mine, who ? __ffs(who) - 1 : 0);
-                    rest[o] = o < rows ? own_rest<E>(a, rows_in_order[o], up) : 0.f;
-                }
-            }
-            finish_row<E>(a.dw, a.w_type, (long long)v * a.D, a.part_w + (size_t)i * a.Dp, a.piece_rows * a.Dp, a.splits_w, w + (size_t)v * a.ldw,
-                          a.norm ? a.iw[v] : 1.f, f, rows, rest, [&](int o) { return x + (size_t)rows_in_order[o] * a.Dp; }, a.norm, a.D, a.Dp, lane);
-        } else {
-            const int r = i - a.cols, c = a.place[r];
-            if (c < 0) {
+            class_row(a.v0 + i, a.part_w + (size_t)i * a.Dp, a.piece_rows * a.Dp, a.splits_w);
+            continue;
+        }
+        const int r = i - a.cols, c = a.place[r];
+        if (c < 0) {
+            if (a.dx)
                 for (int j = lane; j < a.D; j += 32) store_any(a.dx, a.x_type, (long long)r * a.D + j, 0.f);
-                continue;
-            }
-            const int v = a.target[c];
-            rest[0] = v >= 0 ? own_rest<E>(a, c, up) : 0.f;
+            continue;
+        }
+        const int v = a.target[c];
+        if (a.dx) {
+            const float rest[kOwn] = {v >= 0 ? own_rest<E>(a, c, up) : 0.f};
             finish_row<E>(a.dx, a.x_type, (long long)r * a.D, a.part_x + (size_t)c * a.Dp, a.Np * a.Dp, a.splits_x, x + (size_t)c * a.Dp, a.norm ? a.ix[c] : 1.f, f,
                           v >= 0 ? 1 : 0, rest, [&](int) { return w + (size_t)v * a.ldw; }, a.norm, a.D, a.Dp, lane);
         }
+        if (a.own_classes && v >= 0 && a.own_count[v] <= kOwn && a.own[(size_t)v * kOwn] == c) class_row(v, a.part_w + (size_t)c * a.Dp, 0, 1);
     }
 }
 
@@ -467,7 +480,7 @@ Products products_of(const Shape& s, const Saved& sv, const void* w, int64_t ldw
 }  // namespace
 
 cudaError_t teacher(const na1d_head& h, const Shape& s, const Saved& sv, int* flags, cudaStream_t st) {
-    teacher_kernel<<<(unsigned)((s.N + kWarps - 1) / kWarps), kThreads, 0, st>>>(h.teacher_logits, h.teacher_index, (int)s.N, (int)s.k, s.V, 1.f / h.temperature, sv.q, sv.index,
+    teacher_kernel<<<(unsigned)((s.N + kWarps - 1) / kWarps), kThreads, kWarps * s.k * 4, st>>>(h.teacher_logits, h.teacher_index, (int)s.N, (int)s.k, s.V, 1.f / h.temperature, sv.q, sv.index,
                                                                                  flags);
     return cudaGetLastError();
 }
@@ -481,7 +494,8 @@ cudaError_t rows(const na1d_head& h, const Shape& s, const Saved& sv, const int*
     a.wide = s.D % 8 == 0 && h.x_stride % 8 == 0 && (reinterpret_cast<uintptr_t>(h.x) & 15) == 0;
     const int64_t per = round_up((s.N + 295) / 296, kWarps);
     a.per_block = (int)per;
-    const unsigned blocks = (unsigned)((s.N + per - 1) / per);
+    unsigned blocks = (unsigned)((s.N + per - 1) / per);
+    blocks = blocks < 16 ? 16 : blocks;   // (a few rows: the others fill up the tile with zeros)
     if (h.dtype == NA1D_BF16) rows_kernel<__nv_bfloat16><<<blocks, kThreads, 0, st>>>(a);
     else rows_kernel<__half><<<blocks, kThreads, 0, st>>>(a);
     return cudaGetLastError();
@@ -528,7 +542,7 @@ FinishArgs finish_args(const na1d_head& h, const Shape& s, const Saved& sv, void
     return a;
 }
 cudaError_t finish(const na1d_head& h, const FinishArgs& a, cudaStream_t st) {
-    const int blocks = blocks_for((a.dx ? a.N : 0) + a.cols);
+    const int blocks = blocks_for((a.dx || a.own_classes ? a.N : 0) + a.cols);
     if (h.dtype == NA1D_BF16) finish_kernel<__nv_bfloat16><<<blocks, kThreads, 0, st>>>(a);
     else finish_kernel<__half><<<blocks, kThreads, 0, st>>>(a);
     return cudaGetLastError();
