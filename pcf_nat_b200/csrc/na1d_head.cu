@@ -30,8 +30,7 @@ Saved saved_at(const na1d_head& h, const Shape& s, void* base) {
         return static_cast<void*>(p);
     };
     v.words = static_cast<Words*>(take(sizeof(Words)));
-    v.own_count = static_cast<int*>(take(round_up(s.V, kTile) * 4));   // (behind the words: both start as zeros)
-    v.zeros = at;
+    v.own_count = static_cast<int*>(take(round_up(s.V, kTile) * 4));
     v.place = static_cast<int*>(take(s.N * 4));
     v.row = static_cast<int*>(take(s.Np * 4));
     v.lse2 = static_cast<float*>(take(s.Np * 4));
@@ -55,7 +54,7 @@ Saved saved_at(const na1d_head& h, const Shape& s, void* base) {
 
 // A piece of the classes has gradients of at most kPieceBytes, so that they are still in L2 (or nearly) when the products read them, and
 // at least four tiles, below which the sums over pieces would cost more than the products.
-constexpr int64_t kPieceBytes = 96ll << 20;
+constexpr int64_t kPieceBytes = 256ll << 20;
 Pieces pieces_of(const Shape& s, bool want_x, bool want_w) {
     Pieces p = {};
     const int64_t pairs = device_sm_count() / 2;
@@ -162,7 +161,7 @@ int forward(const na1d_head& h, float* loss, void* saved, void* scratch, cudaStr
     const Forward f = forward_at(s, scratch);
     const void* w = s.copy_w ? sv.w : h.weight;
     const int64_t ldw = s.copy_w ? s.Dp : h.weight_stride;
-    NA1D_HEAD_TRY(cudaMemsetAsync(saved, 0, sv.zeros, st));
+    if (s.norm && h.dtype == NA1D_FP16) NA1D_HEAD_TRY(cudaMemsetAsync(sv.words, 0, sizeof(Words), st));   // (the largest inverse lengths; the rest the kernels set)
     if (s.k) NA1D_HEAD_TRY(teacher(h, s, sv, f.flags, st));
     NA1D_HEAD_TRY(rows(h, s, sv, f.flags, loss, st));
     NA1D_HEAD_TRY(weight(h, s, sv, st));
@@ -182,7 +181,7 @@ int backward(const na1d_head& h, void* dx, void* dw, const float* d_loss, void* 
     if (b.coef) NA1D_HEAD_TRY(coefficients(h, s, sv, d_loss, b.coef, st));
     for (int64_t i = 0; i < p.count; ++i) {
         const int64_t v0 = i * p.pitch, cols = s.V - v0 < p.pitch ? s.V - v0 : p.pitch;
-        NA1D_HEAD_TRY(gradients(h, s, sv, b.coef, b.grad, p.pitch, v0, (cols + kTile - 1) / kTile, w, ldw, st));
+        NA1D_HEAD_TRY(gradients(h, s, sv, b.coef, b.grad, p.pitch, v0, (cols + kTile - 1) / kTile, w, ldw, i > 0 || b.coef != nullptr, st));
         const bool last = i + 1 == p.count;
         FinishArgs f = finish_args(h, s, sv, last ? dx : nullptr, dw, b.part_x, b.part_w, d_loss, b.coef, p, v0, p.direct_w || !dw ? 0 : cols, w, ldw);
         f.own_classes = p.direct_w && last;

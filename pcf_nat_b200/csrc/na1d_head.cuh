@@ -10,11 +10,47 @@
 #include "na1d_tc_common.cuh"
 #include "na1d_internal.h"
 
+#include <atomic>
+#include <utility>
+
 namespace na1d {
 
 int api_cuda_status(cudaError_t e);   // a status code, and the error kept for na1d_last_cuda_error()
 
 namespace head {
+
+// Launch of one of a head's kernels. Each of them starts while its predecessor in the stream ends (programmatic dependent launch): it sets itself up, waits
+// until everything before it is done (ptx::grid_dependency_wait, before it reads or writes anything), and lets its own successor start. `after`: false for
+// the first kernel of a pass, whose predecessor is somebody else's.
+template <typename... P, typename... A>
+inline cudaError_t launch(void (*kern)(P...), int64_t blocks, int threads, size_t smem, cudaStream_t st, bool after, A&&... args) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)blocks);
+    cfg.blockDim = dim3((unsigned)threads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = st;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = after ? 1 : 0;
+    return cudaLaunchKernelEx(&cfg, kern, std::forward<A>(args)...);
+}
+// dynamic shared memory beyond the default for a kernel, once for each device
+template <typename K>
+inline cudaError_t allow_smem(K kern, int bytes, std::atomic<uint64_t>& done) {
+    int dev = 0;
+    if (cudaError_t e = cudaGetDevice(&dev)) return e;
+    const uint64_t bit = 1ull << (dev & 63);
+    if (dev < 64 && (done.load(std::memory_order_relaxed) & bit)) return cudaSuccess;
+    if (cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes)) return e;
+    done.fetch_or(bit, std::memory_order_relaxed);
+    return cudaSuccess;
+}
+__device__ __forceinline__ void wait_for_predecessor() {
+    ptx::grid_dependency_wait();
+    ptx::grid_launch_dependents();
+}
 
 constexpr int kTile = 256;            // rows and classes of a product tile (a pair of CTAs)
 constexpr int kPart = 64;             // classes that one partial maximum and sum stand for
@@ -49,7 +85,7 @@ struct Saved {
     float* entry;      // (N, k) the entry's logit as a power of two, then its gradient p - q
     void* x;           // (Np, Dp) 16 bits, zeros behind the rows that count
     void* w;           // (V, Dp) 16 bits, where the weight is not used in its place
-    int64_t zeros, bytes;   // the first of them start as zeros
+    int64_t bytes;
 };
 
 struct Shape {
@@ -101,7 +137,7 @@ cudaError_t finish(const na1d_head& h, const FinishArgs& a, cudaStream_t st);
 // ---- products (na1d_head_logits.cu, na1d_head_grad.cu)
 cudaError_t stats(const na1d_head& h, const Shape& s, const Saved& sv, float2* part, const void* w, int64_t ldw, cudaStream_t st);
 cudaError_t gradients(const na1d_head& h, const Shape& s, const Saved& sv, const float* coef, void* grad, int64_t pitch, int64_t v0, int64_t tiles, const void* w,
-                      int64_t ldw, cudaStream_t st);
+                      int64_t ldw, bool after, cudaStream_t st);
 cudaError_t products(const na1d_head& h, const Shape& s, const Saved& sv, const void* grad, const Pieces& p, int64_t v0, int64_t cols, bool add, float* part_x,
                      float* part_w, const FinishArgs& f, const void* w, int64_t ldw, cudaStream_t st);
 int logits_read_status();

@@ -48,6 +48,7 @@ struct Item {
 struct Plan {
     int items_x, items_w, steps_x, steps_w, more, fill0, fill1;
 };
+// (a warp)
 __device__ __forceinline__ Plan plan_of(const Args& g, int pairs) {
     const int counted = g.words->counted;
     Plan p;
@@ -56,19 +57,18 @@ __device__ __forceinline__ Plan plan_of(const Args& g, int pairs) {
     p.steps_x = (g.cols + kStep - 1) / kStep;
     p.steps_w = (counted + kStep - 1) / kStep;
     p.more = p.items_w % pairs;
-    // a pair's end: the smallest by which all of the rows' items are done, each of them taking the longest one's time
+    // a pair's end: the smallest by which all of the rows' items are done, each of them taking the longest one's time. It lies a whole number of
+    // them behind the weight's items of some pairs, and within one of the average: each lane tries one such end.
     const int item_x = (p.steps_x + g.splits_x - 1) / g.splits_x, item_w = (p.steps_w + g.splits_w - 1) / g.splits_w;
-    const int busy1 = p.items_w / pairs * item_w, busy0 = busy1 + item_w;
-    auto fill = [&](int end, int busy) { return end > busy ? (end - busy) / item_x : 0; };
-    int low = 0, high = busy0 + (p.items_x / pairs + 1) * item_x;      // (enough: every pair could take its share)
-    while (low < high) {
-        const int mid = (low + high) >> 1;
-        const long long n = (long long)p.more * fill(mid, busy0) + (long long)(pairs - p.more) * fill(mid, busy1);
-        if (n >= p.items_x) high = mid;
-        else low = mid + 1;
-    }
-    p.fill0 = fill(low, busy0);
-    p.fill1 = fill(low, busy1);
+    const int busy1 = p.items_w / pairs * item_w, busy0 = busy1 + item_w, lane = threadIdx.x & 31;
+    const int average = (int)(((long long)p.items_w * item_w + (long long)p.items_x * item_x) / pairs), busy = lane & 1 ? busy1 : busy0;
+    const int end = busy + (max(average - busy, 0) / item_x + (lane >> 1)) * item_x;
+    const int fill0 = max(end - busy0, 0) / item_x, fill1 = max(end - busy1, 0) / item_x;
+    const bool enough = (long long)p.more * fill0 + (long long)(pairs - p.more) * fill1 >= p.items_x;
+    const unsigned best = __reduce_min_sync(0xffffffffu, enough ? (unsigned)end : 0xffffffffu);
+    const int who = __ffs(__ballot_sync(0xffffffffu, enough && (unsigned)end == best)) - 1;
+    p.fill0 = __shfl_sync(0xffffffffu, fill0, who);
+    p.fill1 = __shfl_sync(0xffffffffu, fill1, who);
     return p;
 }
 // a pair's items, one after the other: the weight's, then the rows'
@@ -162,7 +162,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) grad_ke
         ptx::prefetch_tensormap(lane == 0 ? &maps.g_rows : lane == 1 ? &maps.g_cols : lane == 2 ? &maps.x : lane == 3 ? &maps.w : &maps.own);
     }
     if (warp == 2) { pair::tmem_alloc(&bar.tmem, kCols); pair::tmem_relinquish(); }
-    if (warp == 3 && lane == 0) plan_s = plan_of(g, pairs);
+    wait_for_predecessor();
+    if (warp == 3) {
+        const Plan made = plan_of(g, pairs);
+        if (lane == 0) plan_s = made;
+    }
     ptx::tc_fence_before_sync();
     __syncthreads();
     pair::cluster_sync();
@@ -358,11 +362,11 @@ cudaError_t run(const Shape& s, const Saved& sv, const void* grad, Args a, int64
     const int own_bytes = PROJECT ? (int)((s.D + 63) / 64) * kOwnBox : 0, fit = (kMostSmem - 1024 - own_bytes) / kStageBytes;
     a.stages = fit < kMostStages ? fit : kMostStages;
     const int smem = a.stages * kStageBytes + own_bytes + 1024;
-    if (cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem)) return e;
+    static std::atomic<uint64_t> allowed{0};
+    if (cudaError_t e = allow_smem(kern, kMostSmem, allowed)) return e;
     const int64_t items = (a.want_x ? s.Np / kTile * a.d_tiles * a.splits_x : 0) + (a.want_w ? (int64_t)a.tiles * a.d_tiles * a.splits_w : 0);
     const int64_t pairs = device_sm_count() / 2;
-    kern<<<2 * (int)(items < pairs ? items : pairs), kThreads, smem, st>>>(maps, a);
-    return cudaGetLastError();
+    return launch(kern, 2 * (items < pairs ? items : pairs), kThreads, smem, st, true, maps, a);
 }
 
 }  // namespace

@@ -85,6 +85,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) logits_
     pair::cluster_sync();
     ptx::tc_fence_after_sync();
     const uint32_t tmem = bar.tmem;
+    wait_for_predecessor();
     const int counted = g.words->counted, row_tiles = (counted + kTile - 1) / kTile, items = row_tiles * g.tiles;
 
     if (warp == 0) {
@@ -288,19 +289,19 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) logits_
 }
 
 template <typename E, bool GRAD, bool NORM, bool TOP>
-cudaError_t run(const Shape& s, const Saved& sv, const Args& a, const void* w, int64_t ldw, int dtype, cudaStream_t st) {
+cudaError_t run(const Shape& s, const Saved& sv, const Args& a, const void* w, int64_t ldw, bool after, int dtype, cudaStream_t st) {
     Maps maps;
     const int64_t dx[2] = {s.D, s.Np}, sx[1] = {s.Dp}, dw[2] = {s.D, s.V}, sw[1] = {ldw};
     const int box[2] = {kStep, kHalf};
     if (!make_matrix_map(&maps.x, sv.x, dtype, 2, dx, sx, box) || !make_matrix_map(&maps.w, w, dtype, 2, dw, sw, box)) return cudaErrorInvalidValue;
     auto* kern = logits_kernel<E, GRAD, NORM, TOP>;
-    if (cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem)) return e;
+    static std::atomic<uint64_t> allowed{0};
+    if (cudaError_t e = allow_smem(kern, kSmem, allowed)) return e;
     const int64_t items = s.Np / kTile * a.tiles, pairs = device_sm_count() / 2;
-    kern<<<2 * (int)(items < pairs ? items : pairs), kThreads, kSmem, st>>>(maps, a);
-    return cudaGetLastError();
+    return launch(kern, 2 * (items < pairs ? items : pairs), kThreads, kSmem, st, after, maps, a);
 }
 template <bool GRAD>
-cudaError_t launch(const na1d_head& h, const Shape& s, const Saved& sv, Args a, const void* w, int64_t ldw, cudaStream_t st) {
+cudaError_t start(const na1d_head& h, const Shape& s, const Saved& sv, Args a, const void* w, int64_t ldw, bool after, cudaStream_t st) {
     a.words = sv.words; a.row = sv.row; a.target = sv.target; a.index = sv.index; a.entry = sv.entry;
     a.ix = sv.ix; a.iw = sv.iw; a.lse2 = sv.lse2; a.slope = sv.slope;
     a.parts = (int)s.parts; a.V = (int)s.V; a.k = (int)s.k; a.cs = s.cs; a.fp16 = h.dtype == NA1D_FP16;
@@ -308,11 +309,11 @@ cudaError_t launch(const na1d_head& h, const Shape& s, const Saved& sv, Args a, 
     a.tail = (int)((s.D - (int64_t)(a.steps - 1) * kStep + 15) / 16);
     using B = __nv_bfloat16;
     if (s.k) {
-        if (h.dtype == NA1D_BF16) return s.norm ? run<B, GRAD, true, true>(s, sv, a, w, ldw, 0, st) : run<B, GRAD, false, true>(s, sv, a, w, ldw, 0, st);
-        return s.norm ? run<__half, GRAD, true, true>(s, sv, a, w, ldw, 1, st) : run<__half, GRAD, false, true>(s, sv, a, w, ldw, 1, st);
+        if (h.dtype == NA1D_BF16) return s.norm ? run<B, GRAD, true, true>(s, sv, a, w, ldw, after, 0, st) : run<B, GRAD, false, true>(s, sv, a, w, ldw, after, 0, st);
+        return s.norm ? run<__half, GRAD, true, true>(s, sv, a, w, ldw, after, 1, st) : run<__half, GRAD, false, true>(s, sv, a, w, ldw, after, 1, st);
     }
-    if (h.dtype == NA1D_BF16) return s.norm ? run<B, GRAD, true, false>(s, sv, a, w, ldw, 0, st) : run<B, GRAD, false, false>(s, sv, a, w, ldw, 0, st);
-    return s.norm ? run<__half, GRAD, true, false>(s, sv, a, w, ldw, 1, st) : run<__half, GRAD, false, false>(s, sv, a, w, ldw, 1, st);
+    if (h.dtype == NA1D_BF16) return s.norm ? run<B, GRAD, true, false>(s, sv, a, w, ldw, after, 0, st) : run<B, GRAD, false, false>(s, sv, a, w, ldw, after, 0, st);
+    return s.norm ? run<__half, GRAD, true, false>(s, sv, a, w, ldw, after, 1, st) : run<__half, GRAD, false, false>(s, sv, a, w, ldw, after, 1, st);
 }
 
 }  // namespace
@@ -321,13 +322,13 @@ cudaError_t stats(const na1d_head& h, const Shape& s, const Saved& sv, float2* p
     Args a = {};
     a.part = part;
     a.tiles = (int)((s.V + kTile - 1) / kTile);
-    return launch<false>(h, s, sv, a, w, ldw, st);
+    return start<false>(h, s, sv, a, w, ldw, true, st);
 }
 cudaError_t gradients(const na1d_head& h, const Shape& s, const Saved& sv, const float* coef, void* grad, int64_t pitch, int64_t v0, int64_t tiles, const void* w,
-                      int64_t ldw, cudaStream_t st) {
+                      int64_t ldw, bool after, cudaStream_t st) {
     Args a = {};
     a.coef = coef; a.grad = grad; a.pitch = pitch; a.v0 = (int)v0; a.tiles = (int)tiles;
-    return launch<true>(h, s, sv, a, w, ldw, st);
+    return start<true>(h, s, sv, a, w, ldw, after, st);
 }
 int logits_read_status() {
     int v = 0, zero = 0;

@@ -63,6 +63,7 @@ __device__ __forceinline__ float copy_row(E* dst, const void* src, int type, lon
 // entry counts with a class in [0, V); one beyond (or a logit that is no number) makes the row's probabilities NaN.
 __global__ void __launch_bounds__(kThreads) teacher_kernel(const float* __restrict__ logits, const int64_t* __restrict__ index, int N, int k, long long V, float rt,
                                                            float* __restrict__ q, int* __restrict__ out, int* __restrict__ flags) {
+    wait_for_predecessor();
     extern __shared__ int classes_s[];   // a warp's row: kNoClass and behind it for what is no class
     const int i = blockIdx.x * kWarps + (threadIdx.x >> 5), lane = threadIdx.x & 31;
     if (i >= N) return;
@@ -112,12 +113,16 @@ struct RowArgs {
     void* out;
     long long x_stride, ignore, V;
     int N, Np, D, Dp, type, per_block;
-    bool wide, norm;
+    bool wide, norm, relative;   // relative: the largest inverse length is wanted
+    int* own_count;
 };
 // A block takes `per_block` rows. It counts the rows before its own itself: labels are few bytes, and no block waits for another.
 template <typename E>
 __global__ void __launch_bounds__(kThreads) rows_kernel(const __grid_constant__ RowArgs a) {
     __shared__ int sums[kWarps], places[kThreads], base_s;
+    wait_for_predecessor();
+    if (blockIdx.x == 0 && threadIdx.x == 0) a.words->ticket = 0;
+    for (int v = blockIdx.x * kThreads + threadIdx.x; v < a.V; v += gridDim.x * kThreads) a.own_count[v] = 0;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, r0 = min(a.N, (int)blockIdx.x * a.per_block), r1 = min(a.N, r0 + a.per_block);
     auto counts = [&](int i) { return a.flags ? a.flags[i] != 0 : a.labels[i] != a.ignore; };
     int before = 0;
@@ -176,7 +181,7 @@ __global__ void __launch_bounds__(kThreads) rows_kernel(const __grid_constant__ 
     const long long pad = (long long)(a.Np - a.N) * (a.Dp / 8);   // 16-byte pieces behind the last row
     for (long long e = (long long)blockIdx.x * kThreads + threadIdx.x; e < pad; e += (long long)gridDim.x * kThreads)
         reinterpret_cast<uint4*>(out + (size_t)a.N * a.Dp)[e] = make_uint4(0, 0, 0, 0);
-    if (a.norm && lane == 0 && most > 0.f) atomicMax(&a.words->most_ix, __float_as_int(most));   // (the largest, in whatever order)
+    if (a.relative && lane == 0 && most > 0.f) atomicMax(&a.words->most_ix, __float_as_int(most));   // (the largest, in whatever order)
     if (r0 < a.N && r1 == a.N && threadIdx.x == 0) a.words->counted = base;
 }
 
@@ -188,10 +193,11 @@ struct WeightArgs {
     Words* words;
     long long stride;
     int V, D, Dp, type;
-    bool wide, norm;
+    bool wide, norm, relative;
 };
 template <typename E>
 __global__ void __launch_bounds__(kThreads) weight_kernel(const __grid_constant__ WeightArgs a) {
+    wait_for_predecessor();
     const int lane = threadIdx.x & 31;
     float most = 0.f;
     for (int v = blockIdx.x * kWarps + (threadIdx.x >> 5); v < a.V; v += gridDim.x * kWarps) {
@@ -199,7 +205,7 @@ __global__ void __launch_bounds__(kThreads) weight_kernel(const __grid_constant_
         if (a.norm && lane == 0) a.iw[v] = iw;
         most = fmaxf(most, iw);
     }
-    if (a.norm && lane == 0 && most > 0.f) atomicMax(&a.words->most_iw, __float_as_int(most));
+    if (a.relative && lane == 0 && most > 0.f) atomicMax(&a.words->most_iw, __float_as_int(most));
 }
 
 // ---------------------------------------------------------------- single logits
@@ -249,6 +255,7 @@ template <typename E>
 __global__ void __launch_bounds__(kThreads) combine_kernel(const __grid_constant__ CombineArgs a) {
     __shared__ float loss_s[kWarps];
     __shared__ int last;
+    wait_for_predecessor();
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, counted = a.words->counted, c = blockIdx.x * kWarps + warp;
     auto own_row = [&](int v, int c) {   // (in whatever order: they are sorted before they are added up)
         const int n = atomicAdd(a.own_count + v, 1);
@@ -356,6 +363,7 @@ __global__ void __launch_bounds__(kThreads) combine_kernel(const __grid_constant
 __global__ void __launch_bounds__(1024) coefficients_kernel(const float* __restrict__ d_loss, const Words* __restrict__ words, const int* __restrict__ row, long long Np,
                                                             bool relative, float* __restrict__ coef) {
     __shared__ float most_s[32];
+    wait_for_predecessor();
     const int counted = words->counted;
     float most = 0.f;
     if (relative) {
@@ -426,6 +434,7 @@ __device__ __forceinline__ void finish_row(void* out, int type, long long at, co
 }
 template <typename E>
 __global__ void __launch_bounds__(kThreads) finish_kernel(const __grid_constant__ FinishArgs a) {
+    wait_for_predecessor();
     const int lane = threadIdx.x & 31, counted = a.words->counted, n = (a.dx || a.own_classes ? a.N : 0) + a.cols;
     const float up = gradient_scale(a.words, a.fp16, a.norm), f = common_factor(a, counted, up);
     const E *x = static_cast<const E*>(a.x), *w = static_cast<const E*>(a.w);
@@ -480,9 +489,8 @@ Products products_of(const Shape& s, const Saved& sv, const void* w, int64_t ldw
 }  // namespace
 
 cudaError_t teacher(const na1d_head& h, const Shape& s, const Saved& sv, int* flags, cudaStream_t st) {
-    teacher_kernel<<<(unsigned)((s.N + kWarps - 1) / kWarps), kThreads, kWarps * s.k * 4, st>>>(h.teacher_logits, h.teacher_index, (int)s.N, (int)s.k, s.V, 1.f / h.temperature, sv.q, sv.index,
+    return launch(teacher_kernel, (s.N + kWarps - 1) / kWarps, kThreads, kWarps * s.k * 4, st, false, h.teacher_logits, h.teacher_index, (int)s.N, (int)s.k, s.V, 1.f / h.temperature, sv.q, sv.index,
                                                                                  flags);
-    return cudaGetLastError();
 }
 cudaError_t rows(const na1d_head& h, const Shape& s, const Saved& sv, const int* flags, float* loss, cudaStream_t st) {
     RowArgs a = {};
@@ -490,25 +498,22 @@ cudaError_t rows(const na1d_head& h, const Shape& s, const Saved& sv, const int*
     a.loss = h.reduction == NA1D_HEAD_NONE ? loss : nullptr;
     a.words = sv.words; a.place = sv.place; a.row = sv.row; a.target = sv.target; a.ix = sv.ix; a.out = sv.x;
     a.x_stride = h.x_stride; a.ignore = h.ignore_index; a.V = s.V;
-    a.N = (int)s.N; a.Np = (int)s.Np; a.D = (int)s.D; a.Dp = (int)s.Dp; a.type = h.x_type; a.norm = s.norm;
+    a.N = (int)s.N; a.Np = (int)s.Np; a.D = (int)s.D; a.Dp = (int)s.Dp; a.type = h.x_type; a.norm = s.norm; a.own_count = sv.own_count;
+    a.relative = s.norm && h.dtype == NA1D_FP16;
     a.wide = s.D % 8 == 0 && h.x_stride % 8 == 0 && (reinterpret_cast<uintptr_t>(h.x) & 15) == 0;
     const int64_t per = round_up((s.N + 295) / 296, kWarps);
     a.per_block = (int)per;
     unsigned blocks = (unsigned)((s.N + per - 1) / per);
     blocks = blocks < 16 ? 16 : blocks;   // (a few rows: the others fill up the tile with zeros)
-    if (h.dtype == NA1D_BF16) rows_kernel<__nv_bfloat16><<<blocks, kThreads, 0, st>>>(a);
-    else rows_kernel<__half><<<blocks, kThreads, 0, st>>>(a);
-    return cudaGetLastError();
+    return launch(h.dtype == NA1D_BF16 ? rows_kernel<__nv_bfloat16> : rows_kernel<__half>, blocks, kThreads, 0, st, s.k > 0, a);
 }
 cudaError_t weight(const na1d_head& h, const Shape& s, const Saved& sv, cudaStream_t st) {
     if (!s.copy_w && !s.norm) return cudaSuccess;
     WeightArgs a = {};
     a.w = h.weight; a.out = s.copy_w ? sv.w : nullptr; a.iw = sv.iw; a.words = sv.words; a.stride = h.weight_stride;
-    a.V = (int)s.V; a.D = (int)s.D; a.Dp = (int)s.Dp; a.type = h.weight_type; a.norm = s.norm;
+    a.V = (int)s.V; a.D = (int)s.D; a.Dp = (int)s.Dp; a.type = h.weight_type; a.norm = s.norm; a.relative = s.norm && h.dtype == NA1D_FP16;
     a.wide = s.D % 8 == 0 && h.weight_stride % 8 == 0 && (reinterpret_cast<uintptr_t>(h.weight) & 15) == 0;
-    if (h.dtype == NA1D_BF16) weight_kernel<__nv_bfloat16><<<blocks_for(s.V), kThreads, 0, st>>>(a);
-    else weight_kernel<__half><<<blocks_for(s.V), kThreads, 0, st>>>(a);
-    return cudaGetLastError();
+    return launch(h.dtype == NA1D_BF16 ? weight_kernel<__nv_bfloat16> : weight_kernel<__half>, blocks_for(s.V), kThreads, 0, st, true, a);
 }
 cudaError_t combine(const na1d_head& h, const Shape& s, const Saved& sv, const float2* part, float* block_sums, float* loss, const void* w, int64_t ldw,
                     cudaStream_t st) {
@@ -521,13 +526,10 @@ cudaError_t combine(const na1d_head& h, const Shape& s, const Saved& sv, const f
     a.tau2 = h.temperature * h.temperature;
     a.p = products_of(s, sv, w, ldw);
     const unsigned blocks = (unsigned)((s.N + kWarps - 1) / kWarps);
-    if (h.dtype == NA1D_BF16) combine_kernel<__nv_bfloat16><<<blocks, kThreads, 0, st>>>(a);
-    else combine_kernel<__half><<<blocks, kThreads, 0, st>>>(a);
-    return cudaGetLastError();
+    return launch(h.dtype == NA1D_BF16 ? combine_kernel<__nv_bfloat16> : combine_kernel<__half>, blocks, kThreads, 0, st, true, a);
 }
 cudaError_t coefficients(const na1d_head& h, const Shape& s, const Saved& sv, const float* d_loss, float* coef, cudaStream_t st) {
-    coefficients_kernel<<<1, 1024, 0, st>>>(d_loss, sv.words, sv.row, s.Np, h.dtype == NA1D_FP16, coef);
-    return cudaGetLastError();
+    return launch(coefficients_kernel, 1, 1024, 0, st, false, d_loss, sv.words, sv.row, s.Np, h.dtype == NA1D_FP16, coef);
 }
 FinishArgs finish_args(const na1d_head& h, const Shape& s, const Saved& sv, void* dx, void* dw, const float* part_x, const float* part_w, const float* d_loss,
                        const float* coef, const Pieces& p, int64_t v0, int64_t cols, const void* w, int64_t ldw) {
@@ -543,9 +545,7 @@ FinishArgs finish_args(const na1d_head& h, const Shape& s, const Saved& sv, void
 }
 cudaError_t finish(const na1d_head& h, const FinishArgs& a, cudaStream_t st) {
     const int blocks = blocks_for((a.dx || a.own_classes ? a.N : 0) + a.cols);
-    if (h.dtype == NA1D_BF16) finish_kernel<__nv_bfloat16><<<blocks, kThreads, 0, st>>>(a);
-    else finish_kernel<__half><<<blocks, kThreads, 0, st>>>(a);
-    return cudaGetLastError();
+    return launch(h.dtype == NA1D_BF16 ? finish_kernel<__nv_bfloat16> : finish_kernel<__half>, blocks, kThreads, 0, st, true, a);
 }
 
 }  // namespace head

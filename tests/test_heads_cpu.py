@@ -104,5 +104,5 @@ def test_buffers_stay_far_below_the_logits(rows, dim, classes):
     saved, back = L.na1d_head_saved_bytes(h), L.na1d_head_backward_scratch(h, 1, 1)
     padded = (rows + 255) // 256 * 256
     assert saved <= padded * (2 * (dim + 8) + 64) + 64 * (classes + 256) + 4096   # (a copy of the rows, a few words for each row and class)
-    # a piece's gradients (at most 96 MB, or 1024 classes of them), and both products' partial sums
-    assert back <= max(96 << 20, padded * 1024 * 2) + 33 * 4 * (dim + 8) * padded + 17 * 4 * (dim + 8) * (classes + 256) + 4096
+    # a piece's gradients (at most 256 MB, or 1024 classes of them), and both products' partial sums
+    assert back <= max(256 << 20, padded * 1024 * 2) + 33 * 4 * (dim + 8) * padded + 17 * 4 * (dim + 8) * (classes + 256) + 4096
