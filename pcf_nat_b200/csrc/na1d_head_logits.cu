@@ -61,7 +61,8 @@ __device__ __forceinline__ Tile tile_at(int t, int row_tiles, int tiles) {
 
 // TOP: the rows have a teacher's entries, sorted by class, instead of a label. A lane has the place of its row's next entry at hand, and the
 // class of the one after it.
-template <typename E, bool GRAD, bool NORM, bool TOP>
+// FIXED: scaled cosines whose whole range fits fp32's exponents: the scale stands for the maximum.
+template <typename E, bool GRAD, bool NORM, bool TOP, bool FIXED>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) logits_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Args g) {
     extern __shared__ uint8_t raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~(uintptr_t)1023);
@@ -147,10 +148,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) logits_
             const int target = !TOP && live ? g.target[c] : kIgnored;
             // (a row of zeros has no direction: its products are 0 whatever they are multiplied with, and it gets no gradient)
             const float ix = NORM ? (live ? g.ix[c] : 0.f) : 1.f, cs = ix > 0.f ? g.cs * ix : g.cs;
-            float lse2 = 0.f, out = 0.f, at_target = 0.f;
+            // the gradient's factor goes into the exponent, but for its sign
+            float shift = 0.f, out = 0.f, at_target = 0.f;
+            bool negative = false;
             if (GRAD && live) {
-                lse2 = g.lse2[c];
                 out = row_factor(up, ix, g.coef ? g.coef[c] : 1.f, NORM);
+                shift = log2f(fabsf(out)) - g.lse2[c];
+                negative = out < 0.f;
                 if (!TOP && target >= 0) at_target = own_gradient(g.slope[c], out, NORM ? g.iw[target] : 1.f, NORM);
             }
             const int* classes = nullptr;
@@ -176,20 +180,29 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) logits_
             if (!ptx::mbar_wait_relaxed(&bar.acc_full[it & 1], (it >> 1) & 1) || *abort_flag) { atomicExch(&g_head_status, 4); *abort_flag = 1; break; }
             ptx::tc_fence_after_sync();
             const uint32_t acc = tmem + lanes + (it & 1) * kTile + h * kWidth;
-            float most = -INFINITY, sum = 0.f;
+            float most = FIXED ? g.cs : -INFINITY, sum = 0.f;
 #pragma unroll 1
             for (int n = 0; n < kWidth; n += 32) {
                 float d[32];
-                pair::tmem_ld32(acc + n, d);
-                ptx::tmem_ld_wait();
+                float2 iw[NORM ? 16 : 1];
                 const int col = v + n;
-                const bool hit = !TOP && (unsigned)(target - col) < 32u;
                 if constexpr (NORM) {
-                    const float4* iw = reinterpret_cast<const float4*>(g.iw + col);
 #pragma unroll
                     for (int j = 0; j < 8; ++j) {
-                        const float4 f = __ldg(iw + j);
-                        d[4 * j] *= f.x; d[4 * j + 1] *= f.y; d[4 * j + 2] *= f.z; d[4 * j + 3] *= f.w;
+                        const float4 f = __ldg(reinterpret_cast<const float4*>(g.iw + col) + j);
+                        iw[2 * j] = make_float2(f.x, f.y);
+                        iw[2 * j + 1] = make_float2(f.z, f.w);
+                    }
+                }
+                pair::tmem_ld32(acc + n, d);
+                ptx::tmem_ld_wait();
+                const bool hit = !TOP && (unsigned)(target - col) < 32u;
+                if constexpr (NORM) {
+#pragma unroll
+                    for (int j = 0; j < 16; ++j) {
+                        const float2 z = mul2(make_float2(d[2 * j], d[2 * j + 1]), iw[j]);
+                        d[2 * j] = z.x;
+                        d[2 * j + 1] = z.y;
                     }
                 }
                 if constexpr (!GRAD) {
@@ -216,41 +229,44 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) logits_
                             }
                         }
                     }
-                    float m[8];
+                    float by = most;
+                    if constexpr (!FIXED) {
+                        float m[8];
 #pragma unroll
-                    for (int j = 0; j < 8; ++j) m[j] = fmaxf(fmaxf(d[j], d[j + 8]), fmaxf(d[j + 16], d[j + 24]));
-                    const float top = fmaxf(fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3])), fmaxf(fmaxf(m[4], m[5]), fmaxf(m[6], m[7])));
-                    const float to = fmaxf(most, top * cs), by = to > -INFINITY ? to : 0.f;
-                    float s[4] = {};
+                        for (int j = 0; j < 8; ++j) m[j] = fmaxf(fmaxf(d[j], d[j + 8]), fmaxf(d[j + 16], d[j + 24]));
+                        const float top = fmaxf(fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3])), fmaxf(fmaxf(m[4], m[5]), fmaxf(m[6], m[7])));
+                        const float to = fmaxf(most, top * cs);
+                        by = to > -INFINITY ? to : 0.f;
+                        sum *= exp2_fast(most - by);
+                        most = to;
+                    }
+                    float2 s0 = both(0.f), s1 = both(0.f);
 #pragma unroll
-                    for (int j = 0; j < 32; ++j) s[j & 3] += exp2_fast(fmaf(d[j], cs, -by));
-                    sum = sum * exp2_fast(most - by) + ((s[0] + s[1]) + (s[2] + s[3]));
-                    most = to;
+                    for (int j = 0; j < 16; ++j) {
+                        const float2 z = fma2(make_float2(d[2 * j], d[2 * j + 1]), both(cs), both(-by)), e = make_float2(exp2_fast(z.x), exp2_fast(z.y));
+                        if (j & 1) s1 = add2(s1, e);
+                        else s0 = add2(s0, e);
+                    }
+                    s0 = add2(s0, s1);
+                    sum += s0.x + s0.y;
                 } else {
                     uint32_t packed[16];
-                    if constexpr (NORM) {
-                        const float4* iw = reinterpret_cast<const float4*>(g.iw + col);
 #pragma unroll
-                        for (int j = 0; j < 8; ++j) {
-                            const float4 f = __ldg(iw + j);
-                            d[4 * j] = exp2_fast(fmaf(d[4 * j], cs, -lse2)) * (out * f.x);
-                            d[4 * j + 1] = exp2_fast(fmaf(d[4 * j + 1], cs, -lse2)) * (out * f.y);
-                            d[4 * j + 2] = exp2_fast(fmaf(d[4 * j + 2], cs, -lse2)) * (out * f.z);
-                            d[4 * j + 3] = exp2_fast(fmaf(d[4 * j + 3], cs, -lse2)) * (out * f.w);
-                        }
-                        if (hit) {
+                    for (int j = 0; j < 16; ++j) {
+                        const float2 z = fma2(make_float2(d[2 * j], d[2 * j + 1]), both(cs), both(shift));
+                        float2 e = make_float2(exp2_fast(z.x), exp2_fast(z.y));
+                        if constexpr (NORM) e = mul2(e, iw[j]);
+                        d[2 * j] = e.x;
+                        d[2 * j + 1] = e.y;
+                    }
+                    if (negative) {
 #pragma unroll
-                            for (int j = 0; j < 32; ++j)
-                                if (j == target - col) d[j] = at_target;
-                        }
-                    } else {
+                        for (int j = 0; j < 32; ++j) d[j] = -d[j];
+                    }
+                    if (hit) {
 #pragma unroll
-                        for (int j = 0; j < 32; ++j) d[j] = exp2_fast(fmaf(d[j], cs, -lse2)) * out;
-                        if (hit) {
-#pragma unroll
-                            for (int j = 0; j < 32; ++j)
-                                if (j == target - col) d[j] = at_target;
-                        }
+                        for (int j = 0; j < 32; ++j)
+                            if (j == target - col) d[j] = at_target;
                     }
                     if constexpr (TOP) {
                         while (__any_sync(0xffffffffu, next < col + 32)) {
@@ -288,13 +304,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) logits_
     if (warp == 2) pair::tmem_dealloc(tmem, kCols);
 }
 
-template <typename E, bool GRAD, bool NORM, bool TOP>
+template <typename E, bool GRAD, bool NORM, bool TOP, bool FIXED = false>
 cudaError_t run(const Shape& s, const Saved& sv, const Args& a, const void* w, int64_t ldw, bool after, int dtype, cudaStream_t st) {
     Maps maps;
     const int64_t dx[2] = {s.D, s.Np}, sx[1] = {s.Dp}, dw[2] = {s.D, s.V}, sw[1] = {ldw};
     const int box[2] = {kStep, kHalf};
     if (!make_matrix_map(&maps.x, sv.x, dtype, 2, dx, sx, box) || !make_matrix_map(&maps.w, w, dtype, 2, dw, sw, box)) return cudaErrorInvalidValue;
-    auto* kern = logits_kernel<E, GRAD, NORM, TOP>;
+    auto* kern = logits_kernel<E, GRAD, NORM, TOP, FIXED>;
     static std::atomic<uint64_t> allowed{0};
     if (cudaError_t e = allow_smem(kern, kSmem, allowed)) return e;
     const int64_t items = s.Np / kTile * a.tiles, pairs = device_sm_count() / 2;
@@ -307,13 +323,22 @@ cudaError_t start(const na1d_head& h, const Shape& s, const Saved& sv, Args a, c
     a.parts = (int)s.parts; a.V = (int)s.V; a.k = (int)s.k; a.cs = s.cs; a.fp16 = h.dtype == NA1D_FP16;
     a.steps = (int)((s.D + kStep - 1) / kStep);
     a.tail = (int)((s.D - (int64_t)(a.steps - 1) * kStep + 15) / 16);
+    // scaled cosines of at most +-48 powers of two: the smallest term is 2^-96 of the one that the scale stands for
+    const bool fixed = !GRAD && s.norm && s.cs <= 48.f;
+#define NA1D_HEAD_RUN(E, NORM, TOP, code) \
+    return fixed && NORM ? run<E, GRAD, NORM, TOP, !GRAD && NORM>(s, sv, a, w, ldw, after, code, st) : run<E, GRAD, NORM, TOP>(s, sv, a, w, ldw, after, code, st)
+    const bool bf16 = h.dtype == NA1D_BF16, top = s.k > 0;
     using B = __nv_bfloat16;
-    if (s.k) {
-        if (h.dtype == NA1D_BF16) return s.norm ? run<B, GRAD, true, true>(s, sv, a, w, ldw, after, 0, st) : run<B, GRAD, false, true>(s, sv, a, w, ldw, after, 0, st);
-        return s.norm ? run<__half, GRAD, true, true>(s, sv, a, w, ldw, after, 1, st) : run<__half, GRAD, false, true>(s, sv, a, w, ldw, after, 1, st);
-    }
-    if (h.dtype == NA1D_BF16) return s.norm ? run<B, GRAD, true, false>(s, sv, a, w, ldw, after, 0, st) : run<B, GRAD, false, false>(s, sv, a, w, ldw, after, 0, st);
-    return s.norm ? run<__half, GRAD, true, false>(s, sv, a, w, ldw, after, 1, st) : run<__half, GRAD, false, false>(s, sv, a, w, ldw, after, 1, st);
+    using H = __half;
+    if (bf16 && s.norm && top) NA1D_HEAD_RUN(B, true, true, 0);
+    if (bf16 && s.norm) NA1D_HEAD_RUN(B, true, false, 0);
+    if (bf16 && top) NA1D_HEAD_RUN(B, false, true, 0);
+    if (bf16) NA1D_HEAD_RUN(B, false, false, 0);
+    if (s.norm && top) NA1D_HEAD_RUN(H, true, true, 1);
+    if (s.norm) NA1D_HEAD_RUN(H, true, false, 1);
+    if (top) NA1D_HEAD_RUN(H, false, true, 1);
+    NA1D_HEAD_RUN(H, false, false, 1);
+#undef NA1D_HEAD_RUN
 }
 
 }  // namespace
