@@ -736,6 +736,8 @@ def main():
     ap.add_argument("--quick", action="store_true", help="with --sweep: a bf16, D=64 subset")
     ap.add_argument("--scaling", default="strong", choices=["strong", "weak"], help="model workloads: split or replicate the batch")
     ap.add_argument("--attention", default="fused", choices=["fused", "unfused"], help="model workloads: operator variant")
+    ap.add_argument("--head", default="plain", choices=["plain", "fused"], help="cfg5_train: AAM-softmax in fp32 passes or without its cosines")
+    ap.add_argument("--teacher-top", type=int, default=0, metavar="K", help="cfg5_train: also learn from a teacher's K top logits")
     ap.add_argument("--precision", default="autocast", choices=["bf16", "autocast"],
                     help="model workloads: bf16 weights/activations with fp32 master weights, or bf16 autocast over fp32 parameters")
     ap.add_argument("--crop-batches", action="store_true",

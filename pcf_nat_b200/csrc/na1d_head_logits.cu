@@ -51,13 +51,37 @@ __device__ __forceinline__ float exp2_fast(float x) {
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
-// tile t: bands of kBand row tiles, in a band the classes outside and its row tiles inside, so that the pairs at work share both operands in L2
-struct Tile { int m, n; };
-__device__ __forceinline__ Tile tile_at(int t, int row_tiles, int tiles) {
-    const int band = t / (kBand * tiles), first = band * kBand, height = min(kBand, row_tiles - first);
-    t -= band * kBand * tiles;
-    return Tile{first + t % height, t / height};
-}
+__device__ __forceinline__ void prefetch_line(const void* p) { asm volatile("prefetch.global.L1 [%0];" ::"l"(p)); }
+// Tiles in the order in which the pairs take them: bands of kBand row tiles, in a band the classes outside and its row tiles inside, so that the pairs
+// at work share both operands in L2. A pair takes every `step`-th; from one to its next inside a band there is nothing to divide.
+struct Walk {
+    int m, n, left;             // this tile; tiles behind it that are in the list
+    int first, height, dm, dn;  // its band; the step in it
+    int index, step, row_tiles, tiles;
+    __device__ __forceinline__ Walk(int index_, int step_, int row_tiles_, int tiles_) : index(index_), step(step_), row_tiles(row_tiles_), tiles(tiles_) {
+        left = row_tiles * tiles - index;
+        find();
+    }
+    __device__ __forceinline__ void find() {
+        if (left <= 0) return;
+        const int band = index / (kBand * tiles), r = index - band * kBand * tiles;
+        first = band * kBand;
+        height = min(kBand, row_tiles - first);
+        n = r / height;
+        m = first + (r - n * height);
+        dn = step / height;
+        dm = step - dn * height;
+    }
+    __device__ __forceinline__ bool any() const { return left > 0; }
+    __device__ __forceinline__ void next() {
+        left -= step;
+        index += step;
+        m += dm;
+        n += dn;
+        if (m >= first + height) { m -= height; ++n; }
+        if (n >= tiles) find();
+    }
+};
 
 // TOP: the rows have a teacher's entries, sorted by class, instead of a label. A lane has the place of its row's next entry at hand, and the
 // class of the one after it.
@@ -94,8 +118,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) logits_
             int slot = 0, n = 0;
             uint32_t phase = 1;   // the first round finds the slots empty
             bool ok = true;
-            for (int i = first; ok && i < items; i += step) {
-                const Tile t = tile_at(i, row_tiles, g.tiles);
+            for (Walk t(first, step, row_tiles, g.tiles); ok && t.any(); t.next()) {
                 const int m = t.m * kTile + rank * kHalf, v = g.v0 + t.n * kTile + rank * kHalf;
                 for (int k = 0; k < g.steps; ++k) {
                     if (!ptx::mbar_wait_relaxed(&bar.empty[slot], phase) || *abort_flag) { atomicExch(&g_head_status, 1); *abort_flag = 1; ok = false; break; }
@@ -140,31 +163,55 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) logits_
         const int q = warp & 3, h = (warp - 4) >> 2;   // tensor-memory lanes 32 q .. + 31 (those a warp reaches), quarter h of the columns
         const uint32_t lanes = (uint32_t)(q * 32) << 16;
         const float up = GRAD ? gradient_scale(g.words, g.fp16, NORM) : 1.f;
+        // what belongs to a tile's row: asked for while the tile before is worked on
+        struct Row {
+            int target, place;
+            float ix, lse2, coef, slope;
+        };
+        auto row_of = [&](const Walk& t) {
+            Row r = {kIgnored, 0, 0.f, 0.f, 1.f, 0.f};
+            const int c = t.m * kTile + rank * kHalf + q * 32 + lane;
+            if (t.any() && c < counted) {
+                if (TOP) r.place = g.row[c];
+                else r.target = g.target[c];
+                if (NORM) r.ix = g.ix[c];
+                if (GRAD) {
+                    r.lse2 = g.lse2[c];
+                    if (!TOP) r.slope = g.slope[c];
+                    if (g.coef) r.coef = g.coef[c];
+                }
+            }
+            if (NORM && t.any() && lane < kWidth * 4 / 128) prefetch_line(g.iw + g.v0 + t.n * kTile + h * kWidth + lane * 32);
+            return r;
+        };
         int it = 0;
-        for (int i = first; i < items; i += step, ++it) {
-            const Tile t = tile_at(i, row_tiles, g.tiles);
-            const int c = t.m * kTile + rank * kHalf + q * 32 + lane, v = g.v0 + t.n * kTile + h * kWidth;
+        Walk ahead(first, step, row_tiles, g.tiles);
+        Row next_row = row_of(ahead);
+        while (ahead.any()) {
+            const int c = ahead.m * kTile + rank * kHalf + q * 32 + lane, v = g.v0 + ahead.n * kTile + h * kWidth;
+            const Row row = next_row;
+            ahead.next();
+            next_row = row_of(ahead);
             const bool live = c < counted;
-            const int target = !TOP && live ? g.target[c] : kIgnored;
+            const int target = row.target;
             // (a row of zeros has no direction: its products are 0 whatever they are multiplied with, and it gets no gradient)
-            const float ix = NORM ? (live ? g.ix[c] : 0.f) : 1.f, cs = ix > 0.f ? g.cs * ix : g.cs;
+            const float ix = NORM ? row.ix : 1.f, cs = ix > 0.f ? g.cs * ix : g.cs;
             // the gradient's factor goes into the exponent, but for its sign
             float shift = 0.f, out = 0.f, at_target = 0.f;
             bool negative = false;
             if (GRAD && live) {
-                out = row_factor(up, ix, g.coef ? g.coef[c] : 1.f, NORM);
-                shift = log2f(fabsf(out)) - g.lse2[c];
+                out = row_factor(up, ix, row.coef, NORM);
+                shift = log2f(fabsf(out)) - row.lse2;
                 negative = out < 0.f;
-                if (!TOP && target >= 0) at_target = own_gradient(g.slope[c], out, NORM ? g.iw[target] : 1.f, NORM);
+                if (!TOP && target >= 0) at_target = own_gradient(row.slope, out, NORM ? g.iw[target] : 1.f, NORM);
             }
             const int* classes = nullptr;
             float* entry = nullptr;
             int next = kNoClass, after = kNoClass, pos = 0;
             if (TOP && live) {
-                classes = g.index + (size_t)g.row[c] * g.k;
-                entry = g.entry + (size_t)g.row[c] * g.k;
-                int end = g.k;
-                while (pos < end) {   // the first entry whose class is v or more
+                classes = g.index + (size_t)row.place * g.k;
+                entry = g.entry + (size_t)row.place * g.k;
+                for (int end = g.k; pos < end;) {   // the first entry whose class is v or more
                     const int mid = (pos + end) >> 1;
                     if (__ldg(classes + mid) < v) pos = mid + 1;
                     else end = mid;
@@ -177,7 +224,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) logits_
                 next = after;
                 after = pos + 1 < g.k ? __ldg(classes + pos + 1) : kNoClass;
             };
-            if (!ptx::mbar_wait_relaxed(&bar.acc_full[it & 1], (it >> 1) & 1) || *abort_flag) { atomicExch(&g_head_status, 4); *abort_flag = 1; break; }
+            if (!ptx::mbar_wait(&bar.acc_full[it & 1], (it >> 1) & 1) || *abort_flag) { atomicExch(&g_head_status, 4); *abort_flag = 1; break; }
             ptx::tc_fence_after_sync();
             const uint32_t acc = tmem + lanes + (it & 1) * kTile + h * kWidth;
             float most = FIXED ? g.cs : -INFINITY, sum = 0.f;
@@ -295,6 +342,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) logits_
             __syncwarp();
             if (lane == 0) pair::arrive_cluster(pair::in_leader(&bar.acc_empty[it & 1]));
             if (!GRAD && live) g.part[(size_t)c * g.parts + v / kPart] = make_float2(most, sum);
+            ++it;
         }
     }
     __syncwarp();

@@ -11,13 +11,15 @@ with it: weights are random-init, which is all a throughput benchmark needs. The
 
 ``attention="unfused"`` swaps in the reference's own operator sequence -- ``q*scale -> QK -> +rpb -> softmax -> AV`` through
 the drop-in ``getNA1dFunction`` pair with the fp32 ``(N*heads, T, win)`` tensor in HBM -- for an A/B of the fused layer
-inside a whole training step.
+inside a whole training step. ``head="fused"`` runs the loss without its (utterances, classes) cosines (``heads.py``), and ``distill`` lets an extractor
+learn from another one's ``top_logits``.
 """
 import torch
 import torch.nn as nn
 import torch.nn.functional as F
 
 from . import block
+from .heads import angular_cross_entropy, linear_distillation
 from .nattention import NAttention, _merge_heads, _plain_linear, _split_heads, _valid_tokens
 from .nattn import getNA1dFunction
 
@@ -89,17 +91,36 @@ class AttentiveStatsPool(nn.Module):
         return block.weighted_stats(logits, x, 1e-5) if out is None else out
 
 
-class AAMSoftmax(nn.Module):
-    """Additive angular margin softmax loss over `classes` (cos(theta + m) on the target logit, scale s)."""
+def _half(emb):
+    """Embeddings as the 16-bit losses take them: fp32 ones outside autocast are rounded to bfloat16."""
+    return emb if emb.dtype != torch.float32 or torch.is_autocast_enabled(emb.device.type) else emb.to(torch.bfloat16)
 
-    def __init__(self, dim, classes, margin=0.2, scale=30.0):
+
+class AAMSoftmax(nn.Module):
+    """Additive angular margin softmax loss over `classes` (cos(theta + m) on the target logit, scale s).
+
+    ``fused``: ``heads.angular_cross_entropy`` -- the same loss of 16-bit embeddings and weights (fp32 ones are rounded, to autocast's type or
+    bfloat16) without the (rows, classes) cosines, for many rows or classes. The default computes in fp32 as before."""
+
+    def __init__(self, dim, classes, margin=0.2, scale=30.0, fused=False):
         super().__init__()
         self.weight = nn.Parameter(torch.randn(classes, dim) * 0.01)
-        self.m, self.s = margin, scale
+        self.m, self.s, self.fused = margin, scale, fused
 
     def forward(self, emb, labels):
+        if self.fused:
+            return angular_cross_entropy(_half(emb), self.weight, labels, margin=self.m, scale=self.s)
         with torch.autocast(emb.device.type, enabled=False):  # the margin arithmetic stays in fp32
             return self._loss(emb.float(), labels)
+
+    def distill(self, emb, teacher_logits, teacher_index, temperature=1.0):
+        """Divergence from a teacher's top logits over the same classes (``heads.linear_distillation`` of the scaled cosines)."""
+        return linear_distillation(_half(emb), self.weight, teacher_logits, teacher_index, temperature=temperature, scale=self.s, normalize=True)
+
+    def top_logits(self, emb, k):
+        """The k largest scaled cosines of each row and their classes, largest first: what a teacher keeps for ``distill``."""
+        with torch.no_grad(), torch.autocast(emb.device.type, enabled=False):
+            return (F.linear(F.normalize(emb.float()), F.normalize(self.weight.float())) * self.s).topk(k, dim=1)
 
     def _loss(self, emb, labels):
         cos = F.linear(F.normalize(emb.float()), F.normalize(self.weight.float())).clamp(-1 + 1e-7, 1 - 1e-7)
@@ -110,10 +131,12 @@ class AAMSoftmax(nn.Module):
 
 class PCFNATExtractor(nn.Module):
     def __init__(self, frames=300, feat=80, dim=256, heads=4, win=7, stages=6, blocks=4, mlp_ratio=4, emb=192,
-                 classes=5994, attention="fused"):
+                 classes=5994, attention="fused", head="plain"):
         super().__init__()
         if attention not in ("fused", "unfused"):
             raise ValueError("attention must be 'fused' or 'unfused'")
+        if head not in ("plain", "fused"):
+            raise ValueError("head must be 'plain' or 'fused'")
         self.front = nn.Conv1d(feat, dim, kernel_size=5, padding=2)
         self.stages = nn.ModuleList(nn.ModuleList(NABlock(frames, dim, heads, win, mlp_ratio, attention) for _ in range(blocks))
                                     for _ in range(stages))
@@ -122,7 +145,7 @@ class PCFNATExtractor(nn.Module):
         self.pool = AttentiveStatsPool(stages * dim)
         self.bn = nn.BatchNorm1d(2 * stages * dim)
         self.embed = nn.Linear(2 * stages * dim, emb)
-        self.loss = AAMSoftmax(emb, classes)
+        self.loss = AAMSoftmax(emb, classes, fused=head == "fused")
 
     def embedding(self, fbank, padding=None):
         x = self.front(fbank).transpose(1, 2).contiguous()  # (N, T, C)
@@ -159,6 +182,16 @@ class PCFNATExtractor(nn.Module):
 
     def forward(self, fbank, labels, padding=None):
         return self.loss(self.embedding(fbank, padding), labels)
+
+    def distill(self, fbank, labels, teacher_logits, teacher_index, temperature=1.0, weight=1.0, padding=None):
+        """The head's own loss plus ``weight`` times the divergence from a teacher's top logits (``top_logits`` of a larger extractor)."""
+        emb = self.embedding(fbank, padding)
+        return self.loss(emb, labels) + weight * self.loss.distill(emb, teacher_logits, teacher_index, temperature)
+
+    def top_logits(self, fbank, k, padding=None):
+        """A teacher's k largest logits for each utterance and their classes."""
+        with torch.no_grad():
+            return self.loss.top_logits(self.embedding(fbank, padding), k)
 
 
 def model_flops_per_utterance(frames=300, feat=80, dim=256, stages=6, blocks=4, mlp_ratio=4, emb=192, classes=5994, win=7):

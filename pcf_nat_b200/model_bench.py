@@ -92,18 +92,26 @@ class TrainStep:
 
     precision "bf16" (default): bf16 weights and activations in the body with fp32 master weights, fp32 gradients for the
     all-reduce and the update (no autocast: no per-call weight and activation casts); "autocast": fp32 parameters under
-    ``torch.autocast(bfloat16)`` as the reference's ``train_main.py`` runs."""
+    ``torch.autocast(bfloat16)`` as the reference's ``train_main.py`` runs. ``head``: the extractor's; ``teacher_top``: a teacher's top logits
+    (that many for each utterance) are learned from beside the labels."""
 
-    def __init__(self, per_gpu, dev, world, rank, attention="fused", frames=FRAMES, use_graphs=True, precision="autocast"):
+    def __init__(self, per_gpu, dev, world, rank, attention="fused", frames=FRAMES, use_graphs=True, precision="autocast", head="plain", teacher_top=0):
         import torch.distributed as dist
         from . import parallel
         from .model import PCFNATExtractor
         self.dist, self.world, self.dev, self.parallel, self.precision = dist, world, dev, parallel, precision
         torch.manual_seed(4)
-        self.model = PCFNATExtractor(frames=frames, attention=attention).to(dev)
+        self.model = PCFNATExtractor(frames=frames, attention=attention, head=head).to(dev)
         g = torch.Generator(device=dev).manual_seed(4 + rank)
         self.fbank = torch.randn(per_gpu, FEAT, frames, device=dev, generator=g)
         self.labels = torch.randint(0, CLASSES, (per_gpu,), device=dev, generator=g)
+        self.teacher = None
+        if teacher_top:     # an extractor of the same kind (other weights) has seen the batch before
+            torch.manual_seed(5)
+            teacher = PCFNATExtractor(frames=frames, attention=attention).to(dev).eval()
+            with torch.autocast("cuda", dtype=torch.bfloat16, cache_enabled=False):
+                self.teacher = tuple(teacher.top_logits(self.fbank, teacher_top))
+            del teacher
         if precision == "bf16":
             self.master, self.flat_w, self.nb, body, tail = _bf16_body(self.model, dev)
             self.n_params = self.master.numel()
@@ -149,16 +157,21 @@ class TrainStep:
             self.launch = "graph A (zero grads, forward, backward) -> eager NCCL all-reduce -> graph B (AdamW)" if world > 1 else \
                 "graph A (zero grads, forward, backward) -> graph B (AdamW)"
 
+    def _loss(self, fbank):
+        if self.teacher is None:
+            return self.model(fbank, self.labels)
+        return self.model.distill(fbank, self.labels, *self.teacher, temperature=2.0)
+
     def _forward_backward(self):
         self.flat.zero_()
         if self.precision == "bf16":
             self.body_grad.zero_()
-            loss = self.model(self.fbank.to(torch.bfloat16), self.labels)
+            loss = self._loss(self.fbank.to(torch.bfloat16))
             loss.backward()
             self.flat[:self.nb].copy_(self.body_grad)
         else:
             with torch.autocast("cuda", dtype=torch.bfloat16, cache_enabled=False):
-                loss = self.model(self.fbank, self.labels)
+                loss = self._loss(self.fbank)
             loss.backward()
         self.loss = loss.detach()
 
@@ -205,7 +218,7 @@ def run_train(args):
     global_batch = 256
     lo, hi = parallel.shard_range(global_batch, world, rank) if args.scaling == "strong" else (0, global_batch)
     per_gpu = hi - lo
-    ts = TrainStep(per_gpu, dev, world, rank, attention=args.attention, precision=args.precision)
+    ts = TrainStep(per_gpu, dev, world, rank, attention=args.attention, precision=args.precision, head=args.head, teacher_top=args.teacher_top)
     for _ in range(max(args.warmup, 3)):
         ts()
     ops.device_status()
@@ -236,7 +249,7 @@ def run_train(args):
             "scaling": args.scaling, "vs_baseline": None, "dtype": "bf16", "data": "synthetic",
             "config": {"workload": "cfg5_train", "model": "conv 80->256, 6 stages x 4 NA blocks (dim 256, 4 heads, window 7, MLP x4), "
                        "progressive channel fusion, attentive statistics pooling, 192-d embedding, AAM-softmax over 5994 classes",
-                       "global_batch": total, "per_gpu_batch": per_gpu, "frames": FRAMES, "attention": args.attention,
+                       "global_batch": total, "per_gpu_batch": per_gpu, "frames": FRAMES, "attention": args.attention, "head": args.head, "teacher_top": args.teacher_top,
                        "parameters": ts.n_params, "launch": ts.launch, "parallelism": "dp%d" % world,
                        "batchnorm": "per-GPU statistics", "optimizer": "AdamW (fused)",
                        "precision": "bf16 weights and activations in the body, fp32 master weights, fp32 gradient all-reduce and update"
