@@ -162,9 +162,7 @@ int forward(const na1d_head& h, float* loss, void* saved, void* scratch, cudaStr
     const void* w = s.copy_w ? sv.w : h.weight;
     const int64_t ldw = s.copy_w ? s.Dp : h.weight_stride;
     if (s.norm && h.dtype == NA1D_FP16) NA1D_HEAD_TRY(cudaMemsetAsync(sv.words, 0, sizeof(Words), st));   // (the largest inverse lengths; the rest the kernels set)
-    if (s.k) NA1D_HEAD_TRY(teacher(h, s, sv, f.flags, st));
-    NA1D_HEAD_TRY(rows(h, s, sv, f.flags, loss, st));
-    NA1D_HEAD_TRY(weight(h, s, sv, st));
+    NA1D_HEAD_TRY(prepare(h, s, sv, f.flags, loss, st));
     NA1D_HEAD_TRY(stats(h, s, sv, f.part, w, ldw, st));
     NA1D_HEAD_TRY(combine(h, s, sv, f.part, f.block_sums, loss, w, ldw, st));
     return NA1D_OK;

@@ -1,10 +1,10 @@
 // The losses of a classification head (na1d_head*.cu): what a call is made of, and where its pieces lie in the caller's buffers.
 //
 // Rows x (N, D) and weight w (V, D), products s = x w^T, logits z = scale s (or scale s / (|x| |w|)). The (N, V) logits are never stored:
-//   forward   rows that count side by side (head_rows) -> s tile by tile, a running maximum and sum per row and 128 classes (head_stats)
-//             -> log-sum-exp, the target's terms, the loss (head_combine)
-//   backward  for a piece of the classes at a time: s again, its gradient in 16 bits (head_logits, gradient form) -> the products with
-//             w and x (head_grad) -> sums over splits, the way back through the normalisation (head_finish)
+//   forward   rows that count side by side (prepare) -> s tile by tile, a running maximum and sum per row and 64 classes (stats)
+//             -> log-sum-exp, the target's terms, the loss (combine)
+//   backward  for a piece of the classes at a time: s again, its gradient in 16 bits (gradients) -> the products with
+//             w and x (products) -> sums over splits, the way back through the normalisation (finish)
 #pragma once
 #include "../../include/na1d_b200.h"
 #include "na1d_tc_common.cuh"
@@ -57,7 +57,7 @@ constexpr int kPart = 64;             // classes that one partial maximum and su
 constexpr float kSineFloor = 2e-7f;   // of the squared sine in the margin's formula
 constexpr int kIgnored = -1, kBad = -2;
 constexpr int kNoClass = 0x7fffffff;  // behind a row's entries, which are sorted by class
-constexpr int kOwn = 8;               // rows of a class whose own gradients' roundings are made good
+constexpr int kOwn = 4;               // rows of a class whose own gradients' roundings are made good
 
 inline int64_t round_up(int64_t x, int64_t m) { return (x + m - 1) / m * m; }
 
@@ -108,9 +108,7 @@ struct Pieces {
 Pieces pieces_of(const Shape& s, bool want_x, bool want_w);
 
 // ---- passes (na1d_head_rows.cu)
-cudaError_t teacher(const na1d_head& h, const Shape& s, const Saved& sv, int* flags, cudaStream_t st);
-cudaError_t rows(const na1d_head& h, const Shape& s, const Saved& sv, const int* flags, float* loss, cudaStream_t st);
-cudaError_t weight(const na1d_head& h, const Shape& s, const Saved& sv, cudaStream_t st);
+cudaError_t prepare(const na1d_head& h, const Shape& s, const Saved& sv, int* flags, float* loss, cudaStream_t st);
 cudaError_t combine(const na1d_head& h, const Shape& s, const Saved& sv, const float2* part, float* block_sums, float* loss, const void* w, int64_t ldw,
                     cudaStream_t st);
 cudaError_t coefficients(const na1d_head& h, const Shape& s, const Saved& sv, const float* d_loss, float* coef, cudaStream_t st);

@@ -23,6 +23,17 @@ __device__ __forceinline__ float exp2_fast(float x) {
     return y;
 }
 
+template <typename E> __device__ __forceinline__ float squares(const uint4& v, float ss) {
+    float f[8];
+    Cvt<E>::unpack(v, f);
+#pragma unroll
+    for (int k = 0; k < 8; ++k) ss = fmaf(f[k], f[k], ss);
+    return ss;
+}
+__device__ __forceinline__ float inverse_of(float ss) {   // of a row whose squares the lanes have
+    ss = warp_sum(ss);
+    return ss > 0.f ? rsqrtf(ss) : ss == 0.f ? 0.f : ss;   // (NaN stays)
+}
 // One row of D elements to 16 bits at dst (Dp of them, zeros behind D; null: not stored), returns 1 / its length (0 where that is 0).
 // wide: rows start on 16 bytes, D is a multiple of 8.
 template <typename E>
@@ -46,87 +57,131 @@ __device__ __forceinline__ float copy_row(E* dst, const void* src, int type, lon
             v = Cvt<E>::pack(f);
         }
         if (dst) reinterpret_cast<uint4*>(dst)[j] = v;
-        if (norm) {
-            float f[8];
-            Cvt<E>::unpack(v, f);
-#pragma unroll
-            for (int k = 0; k < 8; ++k) ss = fmaf(f[k], f[k], ss);
-        }
+        if (norm) ss = squares<E>(v, ss);
     }
-    if (!norm) return 1.f;
-    ss = warp_sum(ss);
-    return ss > 0.f ? rsqrtf(ss) : ss == 0.f ? 0.f : ss;   // (NaN stays)
+    return norm ? inverse_of(ss) : 1.f;
 }
+template <typename E> __device__ __forceinline__ float inverse_length(const uint4& v, float ss) { return inverse_of(squares<E>(v, ss)); }
 
 // ---------------------------------------------------------------- a teacher's probabilities
-// Softmax over a row's entries, and the entries in the order of their classes, so that a tile of classes finds its own; a warp to a row. An
-// entry counts with a class in [0, V); one beyond (or a logit that is no number) makes the row's probabilities NaN.
-__global__ void __launch_bounds__(kThreads) teacher_kernel(const float* __restrict__ logits, const int64_t* __restrict__ index, int N, int k, long long V, float rt,
-                                                           float* __restrict__ q, int* __restrict__ out, int* __restrict__ flags) {
-    wait_for_predecessor();
-    extern __shared__ int classes_s[];   // a warp's row: kNoClass and behind it for what is no class
-    const int i = blockIdx.x * kWarps + (threadIdx.x >> 5), lane = threadIdx.x & 31;
-    if (i >= N) return;
-    int* classes = classes_s + (threadIdx.x >> 5) * k;
-    const size_t at = (size_t)i * k;
+struct TeacherArgs {
+    const float* logits;
+    const int64_t* index;
+    float* q;
+    int *out, *flags;          // flags (N): rows that count; null where the rows' kernel finds out by itself
+    long long V;
+    int N, k;
+    float rt;                  // 1 / temperature
+};
+// Softmax over row i's entries, and the entries in the order of their classes, so that a tile of classes finds its own; a warp, `classes`: k ints of its
+// own. An entry counts with a class in [0, V); one beyond (or a logit that is no number) makes the row's probabilities NaN.
+__device__ __forceinline__ bool teacher_row(const TeacherArgs& a, int i, int* classes, int lane) {
+    const size_t at = (size_t)i * a.k;
     float most = -INFINITY;
     bool bad = false;
-    for (int j = lane; j < k; j += 32) {
-        const int64_t v = index[at + j];
-        classes[j] = v < 0 ? kNoClass : v < V ? (int)v : kNoClass - 1;
+    for (int j = lane; j < a.k; j += 32) {
+        const int64_t v = a.index[at + j];
+        classes[j] = v < 0 ? kNoClass : v < a.V ? (int)v : kNoClass - 1;
         if (v < 0) continue;
-        const float t = logits[at + j] * rt;
-        bad |= v >= V || t != t || t == INFINITY;
+        const float t = a.logits[at + j] * a.rt;
+        bad |= v >= a.V || t != t || t == INFINITY;
         most = fmaxf(most, t);
     }
     most = warp_max(most);
     bad = __any_sync(0xffffffffu, bad);
-    auto weight = [&](int j) { return classes[j] != kNoClass && most > -INFINITY ? expf(logits[at + j] * rt - most) : 0.f; };
+    auto weight = [&](int j) { return classes[j] != kNoClass && most > -INFINITY ? expf(a.logits[at + j] * a.rt - most) : 0.f; };
     float sum = 0.f;
-    for (int j = lane; j < k; j += 32) sum += weight(j);
+    for (int j = lane; j < a.k; j += 32) sum += weight(j);
     sum = warp_sum(sum);
     const float r = 1.f / sum;
     __syncwarp();
-    for (int j = lane; j < k; j += 32) {
+    for (int j = lane; j < a.k; j += 32) {
         const int v = classes[j];
         int rank = 0;
 #pragma unroll 4
-        for (int o = 0; o < k; ++o) {
+        for (int o = 0; o < a.k; ++o) {
             const int u = classes[o];
             rank += u < v || (u == v && o < j);
         }
-        q[at + rank] = v == kNoClass ? 0.f : bad ? NAN : most > -INFINITY ? weight(j) * r : 0.f;
-        out[at + rank] = v < kNoClass - 1 ? v : kNoClass;
+        a.q[at + rank] = v == kNoClass ? 0.f : bad ? NAN : most > -INFINITY ? weight(j) * r : 0.f;
+        a.out[at + rank] = v < kNoClass - 1 ? v : kNoClass;
     }
-    if (lane == 0) flags[i] = bad || most > -INFINITY;
+    __syncwarp();
+    return bad || most > -INFINITY;
+}
+__global__ void __launch_bounds__(kThreads) teacher_kernel(const __grid_constant__ TeacherArgs a) {
+    extern __shared__ int classes_s[];
+    wait_for_predecessor();
+    const int i = blockIdx.x * kWarps + (threadIdx.x >> 5), lane = threadIdx.x & 31;
+    if (i >= a.N) return;
+    const bool on = teacher_row(a, i, classes_s + (threadIdx.x >> 5) * a.k, lane);
+    if (lane == 0) a.flags[i] = on;
 }
 
-// ---------------------------------------------------------------- rows that count, side by side
-struct RowArgs {
-    const void* x;
+// ---------------------------------------------------------------- rows that count, side by side; the weight
+struct PrepareArgs {
+    const void *x, *w;
     const int64_t* labels;
-    const int* flags;
     float* loss;               // (N) zeros for rows that do not count; null where the loss is one number
     Words* words;
-    int *place, *row, *target;
-    float* ix;
-    void* out;
-    long long x_stride, ignore, V;
-    int N, Np, D, Dp, type, per_block;
-    bool wide, norm, relative;   // relative: the largest inverse length is wanted
-    int* own_count;
+    int *place, *row, *target, *own_count;
+    float *ix, *iw;
+    void *out, *w_out;         // w_out: null where the weight stays where it is
+    long long x_stride, w_stride, ignore;
+    int N, Np, V, D, Dp, x_type, w_type, per_block, row_blocks;
+    bool wide, w_wide, norm, relative;   // relative: the largest inverse lengths are wanted
+    TeacherArgs t;
+    bool top;
 };
-// A block takes `per_block` rows. It counts the rows before its own itself: labels are few bytes, and no block waits for another.
+// whether row i counts: by its label, or by an entry with a class and a logit above minus infinity (as teacher_row finds)
+__device__ __forceinline__ bool row_counts(const PrepareArgs& a, int i) {
+    if (!a.top) return a.labels[i] != a.ignore;
+    if (a.t.flags) return a.t.flags[i] != 0;
+    for (int j = 0; j < a.t.k; ++j) {
+        const size_t at = (size_t)i * a.t.k + j;
+        if (a.t.index[at] >= 0 && (a.t.index[at] >= a.t.V || !(a.t.logits[at] * a.t.rt <= -INFINITY))) return true;
+    }
+    return false;
+}
+// Blocks below row_blocks take `per_block` rows each. Such a block counts the rows before its own itself: labels are few bytes, and no block waits for
+// another. The others take the weight: a copy in 16 bits where the products cannot read it as it is, and its rows' lengths.
 template <typename E>
-__global__ void __launch_bounds__(kThreads) rows_kernel(const __grid_constant__ RowArgs a) {
+__global__ void __launch_bounds__(kThreads) prepare_kernel(const __grid_constant__ PrepareArgs a) {
     __shared__ int sums[kWarps], places[kThreads], base_s;
+    extern __shared__ int classes_s[];
     wait_for_predecessor();
     if (blockIdx.x == 0 && threadIdx.x == 0) a.words->ticket = 0;
     for (int v = blockIdx.x * kThreads + threadIdx.x; v < a.V; v += gridDim.x * kThreads) a.own_count[v] = 0;
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, r0 = min(a.N, (int)blockIdx.x * a.per_block), r1 = min(a.N, r0 + a.per_block);
-    auto counts = [&](int i) { return a.flags ? a.flags[i] != 0 : a.labels[i] != a.ignore; };
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    float most = 0.f;
+    if ((int)blockIdx.x >= a.row_blocks) {
+        const int step = (gridDim.x - a.row_blocks) * kWarps;
+        int v = (blockIdx.x - a.row_blocks) * kWarps + warp;
+        if (!a.w_out && a.D <= 256) {   // lengths alone: four rows' loads at a time
+            for (; v + 3 * step < a.V; v += 4 * step) {
+                uint4 r[4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    r[i] = lane < a.D / 8 ? __ldg(reinterpret_cast<const uint4*>(static_cast<const E*>(a.w) + (v + i * step) * a.w_stride) + lane) : make_uint4(0, 0, 0, 0);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const float iw = inverse_length<E>(r[i], 0.f);
+                    if (lane == 0) a.iw[v + i * step] = iw;
+                    most = fmaxf(most, iw);
+                }
+            }
+        }
+        for (; v < a.V; v += step) {
+            const float iw = copy_row<E>(a.w_out ? static_cast<E*>(a.w_out) + (size_t)v * a.Dp : nullptr, a.w, a.w_type, v * a.w_stride, a.D, a.Dp, a.w_wide, a.norm, lane);
+            if (a.norm && lane == 0) a.iw[v] = iw;
+            most = fmaxf(most, iw);
+        }
+        if (a.relative && lane == 0 && most > 0.f) atomicMax(&a.words->most_iw, __float_as_int(most));   // (the largest, in whatever order)
+        return;
+    }
+    const int r0 = min(a.N, (int)blockIdx.x * a.per_block), r1 = min(a.N, r0 + a.per_block);
     int before = 0;
-    for (int i = threadIdx.x; i < r0; i += kThreads) before += counts(i);
+    for (int i = threadIdx.x; i < r0; i += kThreads) before += row_counts(a, i);
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) before += __shfl_xor_sync(0xffffffffu, before, o);
     if (lane == 0) sums[warp] = before;
@@ -139,10 +194,9 @@ __global__ void __launch_bounds__(kThreads) rows_kernel(const __grid_constant__ 
     __syncthreads();
     int base = base_s;
     E* out = static_cast<E*>(a.out);
-    float most = 0.f;
     for (int c0 = r0; c0 < r1; c0 += kThreads) {
         const int i = c0 + threadIdx.x;
-        const bool in = i < r1, on = in && counts(i);
+        const bool in = i < r1, on = in && row_counts(a, i);
         const unsigned mask = __ballot_sync(0xffffffffu, on);
         __syncthreads();
         if (lane == 0) sums[warp] = __popc(mask);
@@ -157,7 +211,7 @@ __global__ void __launch_bounds__(kThreads) rows_kernel(const __grid_constant__ 
             a.place[i] = on ? c : kIgnored;
             if (on) {
                 a.row[c] = i;
-                if (a.labels) {
+                if (!a.top) {
                     const int64_t v = a.labels[i];
                     a.target[c] = v >= 0 && v < a.V ? (int)v : kBad;
                 }
@@ -168,9 +222,10 @@ __global__ void __launch_bounds__(kThreads) rows_kernel(const __grid_constant__ 
         for (int j = warp; j < n; j += kWarps) {
             const int p = places[j];
             if (p >= 0) {
-                const float ix = copy_row<E>(out + (size_t)p * a.Dp, a.x, a.type, (c0 + j) * a.x_stride, a.D, a.Dp, a.wide, a.norm, lane);
+                const float ix = copy_row<E>(out + (size_t)p * a.Dp, a.x, a.x_type, (c0 + j) * a.x_stride, a.D, a.Dp, a.wide, a.norm, lane);
                 if (a.norm && lane == 0) a.ix[p] = ix;
                 most = fmaxf(most, ix);
+                if (a.top && !a.t.flags) teacher_row(a.t, c0 + j, classes_s + warp * a.t.k, lane);
             } else {
                 for (int e = lane; e < a.Dp / 8; e += 32) reinterpret_cast<uint4*>(out + (size_t)(-1 - p) * a.Dp)[e] = make_uint4(0, 0, 0, 0);
             }
@@ -179,33 +234,10 @@ __global__ void __launch_bounds__(kThreads) rows_kernel(const __grid_constant__ 
         __syncthreads();
     }
     const long long pad = (long long)(a.Np - a.N) * (a.Dp / 8);   // 16-byte pieces behind the last row
-    for (long long e = (long long)blockIdx.x * kThreads + threadIdx.x; e < pad; e += (long long)gridDim.x * kThreads)
+    for (long long e = (long long)blockIdx.x * kThreads + threadIdx.x; e < pad; e += (long long)a.row_blocks * kThreads)
         reinterpret_cast<uint4*>(out + (size_t)a.N * a.Dp)[e] = make_uint4(0, 0, 0, 0);
-    if (a.relative && lane == 0 && most > 0.f) atomicMax(&a.words->most_ix, __float_as_int(most));   // (the largest, in whatever order)
+    if (a.relative && lane == 0 && most > 0.f) atomicMax(&a.words->most_ix, __float_as_int(most));
     if (r0 < a.N && r1 == a.N && threadIdx.x == 0) a.words->counted = base;
-}
-
-// ---------------------------------------------------------------- the weight
-struct WeightArgs {
-    const void* w;
-    void* out;
-    float* iw;
-    Words* words;
-    long long stride;
-    int V, D, Dp, type;
-    bool wide, norm, relative;
-};
-template <typename E>
-__global__ void __launch_bounds__(kThreads) weight_kernel(const __grid_constant__ WeightArgs a) {
-    wait_for_predecessor();
-    const int lane = threadIdx.x & 31;
-    float most = 0.f;
-    for (int v = blockIdx.x * kWarps + (threadIdx.x >> 5); v < a.V; v += gridDim.x * kWarps) {
-        const float iw = copy_row<E>(a.out ? static_cast<E*>(a.out) + (size_t)v * a.Dp : nullptr, a.w, a.type, v * a.stride, a.D, a.Dp, a.wide, a.norm, lane);
-        if (a.norm && lane == 0) a.iw[v] = iw;
-        most = fmaxf(most, iw);
-    }
-    if (a.relative && lane == 0 && most > 0.f) atomicMax(&a.words->most_iw, __float_as_int(most));
 }
 
 // ---------------------------------------------------------------- single logits
@@ -433,7 +465,7 @@ __device__ __forceinline__ void finish_row(void* out, int type, long long at, co
     }
 }
 template <typename E>
-__global__ void __launch_bounds__(kThreads) finish_kernel(const __grid_constant__ FinishArgs a) {
+__global__ void __launch_bounds__(kThreads, 3) finish_kernel(const __grid_constant__ FinishArgs a) {
     wait_for_predecessor();
     const int lane = threadIdx.x & 31, counted = a.words->counted, n = (a.dx || a.own_classes ? a.N : 0) + a.cols;
     const float up = gradient_scale(a.words, a.fp16, a.norm), f = common_factor(a, counted, up);
@@ -488,32 +520,38 @@ Products products_of(const Shape& s, const Saved& sv, const void* w, int64_t ldw
 
 }  // namespace
 
-cudaError_t teacher(const na1d_head& h, const Shape& s, const Saved& sv, int* flags, cudaStream_t st) {
-    return launch(teacher_kernel, (s.N + kWarps - 1) / kWarps, kThreads, kWarps * s.k * 4, st, false, h.teacher_logits, h.teacher_index, (int)s.N, (int)s.k, s.V, 1.f / h.temperature, sv.q, sv.index,
-                                                                                 flags);
+namespace {
+TeacherArgs teacher_args(const na1d_head& h, const Shape& s, const Saved& sv, int* flags) {
+    return TeacherArgs{h.teacher_logits, h.teacher_index, sv.q, sv.index, flags, (long long)s.V, (int)s.N, (int)s.k, 1.f / h.temperature};
 }
-cudaError_t rows(const na1d_head& h, const Shape& s, const Saved& sv, const int* flags, float* loss, cudaStream_t st) {
-    RowArgs a = {};
-    a.x = h.x; a.labels = s.k ? nullptr : h.labels; a.flags = flags;
+bool whole_pieces(const void* p, int64_t stride, int64_t D) { return D % 8 == 0 && stride % 8 == 0 && (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+}  // namespace
+cudaError_t prepare(const na1d_head& h, const Shape& s, const Saved& sv, int* flags, float* loss, cudaStream_t st) {
+    PrepareArgs a = {};
+    a.x = h.x; a.w = h.weight; a.labels = h.labels; a.top = s.k > 0;
     a.loss = h.reduction == NA1D_HEAD_NONE ? loss : nullptr;
-    a.words = sv.words; a.place = sv.place; a.row = sv.row; a.target = sv.target; a.ix = sv.ix; a.out = sv.x;
-    a.x_stride = h.x_stride; a.ignore = h.ignore_index; a.V = s.V;
-    a.N = (int)s.N; a.Np = (int)s.Np; a.D = (int)s.D; a.Dp = (int)s.Dp; a.type = h.x_type; a.norm = s.norm; a.own_count = sv.own_count;
-    a.relative = s.norm && h.dtype == NA1D_FP16;
-    a.wide = s.D % 8 == 0 && h.x_stride % 8 == 0 && (reinterpret_cast<uintptr_t>(h.x) & 15) == 0;
-    const int64_t per = round_up((s.N + 295) / 296, kWarps);
-    a.per_block = (int)per;
-    unsigned blocks = (unsigned)((s.N + per - 1) / per);
-    blocks = blocks < 16 ? 16 : blocks;   // (a few rows: the others fill up the tile with zeros)
-    return launch(h.dtype == NA1D_BF16 ? rows_kernel<__nv_bfloat16> : rows_kernel<__half>, blocks, kThreads, 0, st, s.k > 0, a);
-}
-cudaError_t weight(const na1d_head& h, const Shape& s, const Saved& sv, cudaStream_t st) {
-    if (!s.copy_w && !s.norm) return cudaSuccess;
-    WeightArgs a = {};
-    a.w = h.weight; a.out = s.copy_w ? sv.w : nullptr; a.iw = sv.iw; a.words = sv.words; a.stride = h.weight_stride;
-    a.V = (int)s.V; a.D = (int)s.D; a.Dp = (int)s.Dp; a.type = h.weight_type; a.norm = s.norm; a.relative = s.norm && h.dtype == NA1D_FP16;
-    a.wide = s.D % 8 == 0 && h.weight_stride % 8 == 0 && (reinterpret_cast<uintptr_t>(h.weight) & 15) == 0;
-    return launch(h.dtype == NA1D_BF16 ? weight_kernel<__nv_bfloat16> : weight_kernel<__half>, blocks_for(s.V), kThreads, 0, st, true, a);
+    a.words = sv.words; a.place = sv.place; a.row = sv.row; a.target = sv.target; a.own_count = sv.own_count; a.ix = sv.ix; a.iw = sv.iw;
+    a.out = sv.x; a.w_out = s.copy_w ? sv.w : nullptr;
+    a.x_stride = h.x_stride; a.w_stride = h.weight_stride; a.ignore = h.ignore_index;
+    a.N = (int)s.N; a.Np = (int)s.Np; a.V = (int)s.V; a.D = (int)s.D; a.Dp = (int)s.Dp; a.x_type = h.x_type; a.w_type = h.weight_type;
+    a.norm = s.norm; a.relative = s.norm && h.dtype == NA1D_FP16;
+    a.wide = whole_pieces(h.x, h.x_stride, s.D);
+    a.w_wide = whole_pieces(h.weight, h.weight_stride, s.D);
+    a.per_block = (int)round_up((s.N + 295) / 296, kWarps);
+    a.row_blocks = (int)((s.N + a.per_block - 1) / a.per_block);
+    a.row_blocks = a.row_blocks < 16 ? 16 : a.row_blocks;   // (a few rows: the others fill up the tile with zeros)
+    // Few rows find out by themselves which of them have a teacher (a row's first entry tells, mostly): a launch less. Many would look at all rows
+    // before theirs once for each block (1003 rows of up to 20 entries: 12 us more).
+    const bool early = s.N * s.k > 8192;
+    size_t smem = 0;
+    if (s.k) {
+        a.t = teacher_args(h, s, sv, early ? flags : nullptr);
+        smem = (size_t)kWarps * s.k * 4;
+        if (early)
+            if (cudaError_t e = launch(teacher_kernel, (s.N + kWarps - 1) / kWarps, kThreads, smem, st, false, a.t)) return e;
+    }
+    const int64_t blocks = a.row_blocks + (s.copy_w || s.norm ? blocks_for(s.V) : 0);
+    return launch(h.dtype == NA1D_BF16 ? prepare_kernel<__nv_bfloat16> : prepare_kernel<__half>, blocks, kThreads, early ? 0 : smem, st, early, a);
 }
 cudaError_t combine(const na1d_head& h, const Shape& s, const Saved& sv, const float2* part, float* block_sums, float* loss, const void* w, int64_t ldw,
                     cudaStream_t st) {

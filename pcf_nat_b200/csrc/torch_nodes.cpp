@@ -15,6 +15,7 @@
 
 #include <ATen/autocast_mode.h>
 #include <ATen/cuda/CUDAContext.h>
+#include <ATen/cuda/EmptyTensor.h>
 #include <ATen/cuda/tunable/Tunable.h>
 #include <c10/core/impl/LocalDispatchKeySet.h>
 #include <c10/core/impl/TorchDispatchModeTLS.h>
@@ -1092,7 +1093,9 @@ int64_t head_bytes(int64_t bytes, const char* where) {
     if (bytes < 0) check((int)bytes, where);
     return bytes;
 }
-Tensor head_buffer(int64_t bytes, const Tensor& like) { return at::empty({bytes}, like.options().dtype(at::kByte)); }
+// (past the dispatcher: a call allocates five or six tensors)
+Tensor head_empty(at::IntArrayRef shape, at::ScalarType type, const Tensor& like) { return at::detail::empty_cuda(shape, type, like.device(), std::nullopt); }
+Tensor head_buffer(int64_t bytes, const Tensor& like) { return head_empty({bytes}, at::kByte, like); }
 
 // x with its rows one after the other, `x_stride` elements apart
 struct HeadForward {
@@ -1106,10 +1109,14 @@ struct HeadForward {
             h.teacher_logits = fptr(*logits);
             h.teacher_index = static_cast<const int64_t*>(ptr(*index));
         }
-        saved = head_buffer(head_bytes(na1d_head_saved_bytes(&h), "na1d_head_saved_bytes"), x);
-        const Tensor scratch = head_buffer(head_bytes(na1d_head_forward_scratch(&h), "na1d_head_forward_scratch"), x);
-        loss = c.reduction == NA1D_HEAD_NONE ? empty_f32(x.sizes().slice(0, x.dim() - 1), x) : empty_f32({}, x);
-        check(na1d_head_forward(&h, fptr(loss), ptr(saved), ptr(scratch), stream()), "na1d_head_forward");
+        const int64_t kept = (head_bytes(na1d_head_saved_bytes(&h), "na1d_head_saved_bytes") + 255) / 256 * 256;
+        const int64_t needed = head_bytes(na1d_head_forward_scratch(&h), "na1d_head_forward_scratch");
+        const bool together = needed <= 1 << 18;   // a little more is kept for the backward pass, and one allocation less
+        saved = head_buffer(together ? kept + needed : kept, x);
+        const Tensor more = together ? Tensor() : head_buffer(needed, x);
+        void* scratch = together ? static_cast<char*>(ptr(saved)) + kept : ptr(more);
+        loss = c.reduction == NA1D_HEAD_NONE ? head_empty(x.sizes().slice(0, x.dim() - 1), at::kFloat, x) : head_empty({}, at::kFloat, x);
+        check(na1d_head_forward(&h, fptr(loss), ptr(saved), scratch, stream()), "na1d_head_forward");
     }
 };
 // whether the forward pass reads the weight where it is: then the backward pass does so too, else it has a copy of its own
@@ -1157,9 +1164,9 @@ struct NA1dHead : public torch::autograd::Function<NA1dHead> {
                 h.weight_stride = w.stride(0);
             }
             const bool want_x = ctx->needs_input_grad(0), want_w = ctx->needs_input_grad(1);
-            const Tensor d_loss = grads[0].to(at::kFloat).contiguous();
-            if (want_x) out[0] = at::empty(d["x"].toIntVector(), saved.options().dtype((at::ScalarType)d["x_type"].toInt()));
-            if (want_w) out[1] = at::empty({h.classes, h.dim}, saved.options().dtype((at::ScalarType)d["w_type"].toInt()));
+            const Tensor d_loss = grads[0].scalar_type() == at::kFloat && grads[0].is_contiguous() ? grads[0] : grads[0].to(at::kFloat).contiguous();
+            if (want_x) out[0] = head_empty(d["x"].toIntVector(), (at::ScalarType)d["x_type"].toInt(), saved);
+            if (want_w) out[1] = head_empty({h.classes, h.dim}, (at::ScalarType)d["w_type"].toInt(), saved);
             const Tensor scratch = head_buffer(head_bytes(na1d_head_backward_scratch(&h, want_x, want_w), "na1d_head_backward_scratch"), saved);
             check(na1d_head_backward(&h, ptr(out[0]), ptr(out[1]), fptr(d_loss), ptr(saved), ptr(scratch), stream()), "na1d_head_backward");
         }

@@ -152,26 +152,15 @@ def _run(dt, x, weight, labels, teacher_logits, teacher_index, cfg, reduction):
     return loss.view(shape) if reduction == "none" else loss
 
 
-def _native(x, weight, labels, teacher_logits, teacher_index, cfg, reduction):
-    """The call as one C++ node, or None where it is not of the forms that this takes."""
-    if (type(x) not in _PLAIN or type(weight) not in _PLAIN or torch.compiler.is_compiling() or reduction not in _REDUCTION or
-            type(labels) not in _PLAIN_OR_NONE or type(teacher_logits) not in _PLAIN_OR_NONE or type(teacher_index) not in _PLAIN_OR_NONE):
-        return None
-    ignore, scale, margin, temperature, normalize = cfg
-    return ops.native.head(x, weight, labels, teacher_logits, teacher_index, scale, margin, temperature, normalize, ignore, _REDUCTION[reduction])
-
-
-_PLAIN = (torch.Tensor, torch.nn.Parameter)
-_PLAIN_OR_NONE = _PLAIN + (type(None),)
-
-
 def _labels_loss(x, weight, labels, cfg, reduction):
-    loss = _native(x, weight, labels, None, None, cfg, reduction)
-    if loss is not None:
-        return loss
+    """What the C++ node (``ops.native.head``) did not take: checks, conversions, the Python route."""
     dt = _rows(x, weight, reduction)
     _index(labels, x.shape[:-1], "labels")
     return _run(dt, x, weight, labels.reshape(-1).to(torch.int64).contiguous(), None, None, cfg, reduction)
+
+
+def _tensors(*ts):
+    return all(isinstance(t, torch.Tensor) for t in ts) and not torch.compiler.is_compiling()
 
 
 # ------------------------------------------------------------------ the losses
@@ -182,14 +171,20 @@ def linear_cross_entropy(x, weight, labels, *, scale=1.0, ignore_index=-100, red
     them reaches the loss or a gradient, and no time goes into them; where no row counts the mean is 0. A label outside the classes makes
     its row's loss, and the gradients that depend on it, NaN (there is no synchronisation to raise an error from). ``reduction``: "mean" over
     the rows that count, "sum", or "none" (0 for the others). Differentiable once in ``x`` and ``weight``; same bits from run to run."""
-    return _labels_loss(x, weight, labels, (int(ignore_index), float(scale), 0.0, 1.0, False), reduction)
+    loss = None
+    if _tensors(x, weight, labels):
+        loss = ops.native.head(x, weight, labels, None, None, scale, 0.0, 1.0, False, ignore_index, _REDUCTION.get(reduction, -1))
+    return _labels_loss(x, weight, labels, (int(ignore_index), float(scale), 0.0, 1.0, False), reduction) if loss is None else loss
 
 
 def angular_cross_entropy(x, weight, labels, *, margin=0.2, scale=30.0, ignore_index=-100, reduction="mean"):
     """AAM-softmax: cross entropy of ``scale`` times the cosines of rows and classes, the label's angle widened by ``margin`` radians
     (``model.AAMSoftmax``; cos(a + m) as cos a cos m - sin a sin m, the squared sine at least 2e-7). A row or class of zeros has cosine 0 with
     all others and no gradient. Otherwise as ``linear_cross_entropy``."""
-    return _labels_loss(x, weight, labels, (int(ignore_index), float(scale), float(margin), 1.0, True), reduction)
+    loss = None
+    if _tensors(x, weight, labels):
+        loss = ops.native.head(x, weight, labels, None, None, scale, margin, 1.0, True, ignore_index, _REDUCTION.get(reduction, -1))
+    return _labels_loss(x, weight, labels, (int(ignore_index), float(scale), float(margin), 1.0, True), reduction) if loss is None else loss
 
 
 def linear_distillation(x, weight, teacher_logits, teacher_index, *, temperature=1.0, scale=1.0, normalize=False, reduction="mean"):
@@ -199,11 +194,11 @@ def linear_distillation(x, weight, teacher_logits, teacher_index, *, temperature
     ``teacher_logits`` (..., k) of any floating type, ``teacher_index`` (..., k) int64 or int32: the entries' classes, negative where there is
     no entry (its logit is not read). Rows without an entry do not count; a class may come twice. k is at most 1024. No gradient
     goes to the teacher. Otherwise as ``linear_cross_entropy``."""
-    cfg = (0, float(scale), 0.0, float(temperature), bool(normalize))
-    if teacher_index is not None and teacher_logits is not None:
-        loss = _native(x, weight, None, teacher_logits, teacher_index, cfg, reduction)
+    if _tensors(x, weight, teacher_logits, teacher_index):
+        loss = ops.native.head(x, weight, None, teacher_logits, teacher_index, scale, 0.0, temperature, normalize, 0, _REDUCTION.get(reduction, -1))
         if loss is not None:
             return loss
+    cfg = (0, float(scale), 0.0, float(temperature), bool(normalize))
     dt = _rows(x, weight, reduction)
     if not isinstance(teacher_index, torch.Tensor) or teacher_index.dim() != x.dim() or teacher_index.shape[-1] == 0:
         raise ValueError("teacher_index is (..., k) for x (..., dim), k at least 1")
