@@ -55,6 +55,7 @@ Saved saved_at(const na1d_head& h, const Shape& s, void* base) {
 // A piece of the classes has gradients of at most kPieceBytes, so that they are still in L2 (or nearly) when the products read them, and
 // at least four tiles, below which the sums over pieces would cost more than the products.
 constexpr int64_t kPieceBytes = 256ll << 20;
+constexpr int64_t kBothTiles = 1;
 Pieces pieces_of(const Shape& s, bool want_x, bool want_w) {
     Pieces p = {};
     const int64_t pairs = device_sm_count() / 2;
@@ -64,6 +65,10 @@ Pieces pieces_of(const Shape& s, bool want_x, bool want_w) {
     p.count = (p.tiles + most - 1) / most;
     p.piece_tiles = (p.tiles + p.count - 1) / p.count;
     p.count = (p.tiles + p.piece_tiles - 1) / p.piece_tiles;
+    if (p.piece_tiles > pairs && p.count > 1) {   // whole rounds of the pairs
+        p.piece_tiles = round_up(p.piece_tiles, pairs);
+        p.count = (p.tiles + p.piece_tiles - 1) / p.piece_tiles;
+    }
     p.pitch = p.piece_tiles * kTile;
     p.d_tiles = (int)((s.D + kTile - 1) / kTile);
     p.d_width = (int)round_up((s.D + p.d_tiles - 1) / p.d_tiles, 32);
@@ -82,6 +87,13 @@ Pieces pieces_of(const Shape& s, bool want_x, bool want_w) {
     p.splits_x = splits(steps_x, share / 3, 6, 32);
     p.splits_w = splits(steps_w, share + share / 4, 16, 16);
     p.direct_w = want_w && p.splits_w == 1 && (!s.norm || p.d_tiles == 1);
+    p.both = want_w && p.d_tiles == 1 && s.k == 0 && p.piece_tiles >= kBothTiles;
+    if (p.both) {
+        p.direct_w = true;
+        p.splits_w = 1;
+        share = (items_x * steps_x + pairs - 1) / pairs;
+        p.splits_x = splits(steps_x, share / 3, 6, 32);
+    }
     return p;
 }
 
@@ -151,8 +163,10 @@ Backward backward_at(const na1d_head& h, const Shape& s, const Pieces& p, bool w
     b.bytes = at;
     return b;
 }
-#define NA1D_HEAD_TRY(call) \
-    if (cudaError_t e = (call)) return api_cuda_status(e)
+#define NA1D_HEAD_TRY(call)                                   \
+    do {                                                      \
+        if (cudaError_t e = (call)) return api_cuda_status(e); \
+    } while (0)
 
 int forward(const na1d_head& h, float* loss, void* saved, void* scratch, cudaStream_t st) {
     bind_primary_context();
@@ -179,11 +193,16 @@ int backward(const na1d_head& h, void* dx, void* dw, const float* d_loss, void* 
     if (b.coef) NA1D_HEAD_TRY(coefficients(h, s, sv, d_loss, b.coef, st));
     for (int64_t i = 0; i < p.count; ++i) {
         const int64_t v0 = i * p.pitch, cols = s.V - v0 < p.pitch ? s.V - v0 : p.pitch;
-        NA1D_HEAD_TRY(gradients(h, s, sv, b.coef, b.grad, p.pitch, v0, (cols + kTile - 1) / kTile, w, ldw, i > 0 || b.coef != nullptr, st));
         const bool last = i + 1 == p.count;
         FinishArgs f = finish_args(h, s, sv, last ? dx : nullptr, dw, b.part_x, b.part_w, d_loss, b.coef, p, v0, p.direct_w || !dw ? 0 : cols, w, ldw);
         f.own_classes = p.direct_w && last;
-        NA1D_HEAD_TRY(products(h, s, sv, b.grad, p, v0, cols, i > 0, b.part_x, b.part_w, f, w, ldw, st));
+        const bool after = i > 0 || b.coef != nullptr;
+        if (p.both) {
+            NA1D_HEAD_TRY(gradients_and_weight(h, s, sv, b.coef, dx ? b.grad : nullptr, s.Np, v0, cols, b.part_w, f, w, ldw, after, st));
+        } else {
+            NA1D_HEAD_TRY(gradients(h, s, sv, b.coef, b.grad, p.pitch, v0, (cols + kTile - 1) / kTile, w, ldw, after, st));
+        }
+        if (dx || !p.both) NA1D_HEAD_TRY(products(h, s, sv, b.grad, p, v0, cols, i > 0, b.part_x, b.part_w, f, w, ldw, st));
         if (f.dx || f.cols || f.own_classes) NA1D_HEAD_TRY(finish(h, f, st));
     }
     return NA1D_OK;
