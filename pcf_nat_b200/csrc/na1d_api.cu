@@ -372,7 +372,7 @@ int na1d_tensor_map_cache_stats(int64_t* hits, int64_t* misses) {
 
 int na1d_device_status(void) {
     // every word is read (and cleared) before anything is reported; an expired wait in any kernel wins over a failed read
-    const int words[14] = {na1d::head::both_read_status(), na1d::head::logits_read_status(), na1d::head::grad_read_status(), na1d::mlp_read_status(), na1d::mlp_bwd_read_status(), na1d::wgrad_read_status(), na1d::tc_read_status(), na1d::tc_bwd_read_status(), na1d::tc_seg_read_status(),
+    const int words[13] = {na1d::head::logits_read_status(), na1d::head::grad_read_status(), na1d::mlp_read_status(), na1d::mlp_bwd_read_status(), na1d::wgrad_read_status(), na1d::tc_read_status(), na1d::tc_bwd_read_status(), na1d::tc_seg_read_status(),
                           na1d::tc_bwd_seg_read_status(), na1d::tc_unfused_read_status(), na1d::tc_unfused_t_read_status(),
                           na1d::tc_drop_read_status(), na1d::tc_bwd_drop_read_status()};
     int v = 0, w = 0;

@@ -55,7 +55,17 @@ Saved saved_at(const na1d_head& h, const Shape& s, void* base) {
 // A piece of the classes has gradients of at most kPieceBytes, so that they are still in L2 (or nearly) when the products read them, and
 // at least four tiles, below which the sums over pieces would cost more than the products.
 constexpr int64_t kPieceBytes = 256ll << 20;
-constexpr int64_t kBothTiles = 1;
+// when the last pair is through with its items, in steps (as the products' kernel shares them out)
+static int64_t last_end(int64_t items_x, int64_t item_x, int64_t items_w, int64_t item_w, int64_t pairs) {
+    const int64_t more = items_w % pairs, busy1 = items_w / pairs * item_w, busy0 = busy1 + item_w, average = (items_w * item_w + items_x * item_x) / pairs;
+    auto fill = [&](int64_t end, int64_t busy) { return end > busy ? (end - busy) / item_x : 0; };
+    int64_t best = -1;
+    for (int k = 0; k < 32; ++k) {
+        const int64_t busy = k & 1 ? busy1 : busy0, end = busy + ((average > busy ? average - busy : 0) / item_x + (k >> 1)) * item_x;
+        if (more * fill(end, busy0) + (pairs - more) * fill(end, busy1) >= items_x && (best < 0 || end < best)) best = end;
+    }
+    return best > (more ? busy0 : busy1) ? best : more ? busy0 : busy1;
+}
 Pieces pieces_of(const Shape& s, bool want_x, bool want_w) {
     Pieces p = {};
     const int64_t pairs = device_sm_count() / 2;
@@ -72,27 +82,22 @@ Pieces pieces_of(const Shape& s, bool want_x, bool want_w) {
     p.pitch = p.piece_tiles * kTile;
     p.d_tiles = (int)((s.D + kTile - 1) / kTile);
     p.d_width = (int)round_up((s.D + p.d_tiles - 1) / p.d_tiles, 32);
-    // Steps of 64 of the two contractions, and a pair's share of all of them. The weight's tiles are whole where that leaves no pair with more than
-    // its share; then their gradients leave at once, unless the way back through the normalisation needs more than one tile of a row. The
-    // rows' tiles fill up what the weight's leave of the pairs' shares, in items of about a third of a share.
+    // Steps of 64 of the two contractions, and a pair's share of all of them. The weight's tiles are whole where that leaves no pair with much more
+    // than its share; then their gradients leave at once, unless the way back through the normalisation needs more than one tile of a row.
     const int64_t steps_x = p.pitch / 64, steps_w = s.Np / 64;
-    const int64_t items_x = want_x ? s.Np / kTile * p.d_tiles : 0, items_w = want_w ? p.piece_tiles * p.d_tiles : 0;
-    int64_t share = (items_x * steps_x + items_w * steps_w + pairs - 1) / pairs;
-    auto splits = [&](int64_t steps, int64_t item, int64_t least, int64_t most_splits) {
-        item = item < least ? least : item;
-        int64_t n = (steps + item - 1) / item;
-        n = n > most_splits ? most_splits : n;
-        return (int)(n < 1 ? 1 : n);
-    };
-    p.splits_x = splits(steps_x, share / 3, 6, 32);
-    p.splits_w = splits(steps_w, share + share / 4, 16, 16);
+    const int64_t items_x = want_x ? s.Np / kTile * p.d_tiles : 0, tiles_w = want_w ? p.piece_tiles * p.d_tiles : 0;
+    const int64_t share = (items_x * steps_x + tiles_w * steps_w + pairs - 1) / pairs, most = share + share / 4 < 16 ? 16 : share + share / 4;
+    p.splits_w = (int)(most >= steps_w ? 1 : (steps_w + most - 1) / most < 16 ? (steps_w + most - 1) / most : 16);
     p.direct_w = want_w && p.splits_w == 1 && (!s.norm || p.d_tiles == 1);
-    p.both = want_w && p.d_tiles == 1 && s.k == 0 && p.piece_tiles >= kBothTiles;
-    if (p.both) {
-        p.direct_w = true;
-        p.splits_w = 1;
-        share = (items_x * steps_x + pairs - 1) / pairs;
-        p.splits_x = splits(steps_x, share / 3, 6, 32);
+    // Splits of the rows' contraction, which fill up what the weight's items leave of the pairs' time: the end of the last pair (a step takes about
+    // half a microsecond) against the partial sums' way to memory and back (4 TB/s; the normalised ones of wide rows are read twice).
+    const int64_t items_w = tiles_w * p.splits_w, item_w = (steps_w + p.splits_w - 1) / p.splits_w;
+    const double each = (double)s.Np * s.Dp * 4 * (s.norm && s.Dp > 256 ? 3 : 2) / 4e6;
+    double best = 0;
+    p.splits_x = 1;
+    for (int n = 1; items_x && n <= 32 && n <= steps_x / 4 + 1; ++n) {
+        const double cost = 0.5 * last_end(items_x * n, (steps_x + n - 1) / n, items_w, item_w, pairs) + n * each;
+        if (n == 1 || cost < best) { best = cost; p.splits_x = n; }
     }
     return p;
 }
@@ -197,12 +202,8 @@ int backward(const na1d_head& h, void* dx, void* dw, const float* d_loss, void* 
         FinishArgs f = finish_args(h, s, sv, last ? dx : nullptr, dw, b.part_x, b.part_w, d_loss, b.coef, p, v0, p.direct_w || !dw ? 0 : cols, w, ldw);
         f.own_classes = p.direct_w && last;
         const bool after = i > 0 || b.coef != nullptr;
-        if (p.both) {
-            NA1D_HEAD_TRY(gradients_and_weight(h, s, sv, b.coef, dx ? b.grad : nullptr, s.Np, v0, cols, b.part_w, f, w, ldw, after, st));
-        } else {
-            NA1D_HEAD_TRY(gradients(h, s, sv, b.coef, b.grad, p.pitch, v0, (cols + kTile - 1) / kTile, w, ldw, after, st));
-        }
-        if (dx || !p.both) NA1D_HEAD_TRY(products(h, s, sv, b.grad, p, v0, cols, i > 0, b.part_x, b.part_w, f, w, ldw, st));
+        NA1D_HEAD_TRY(gradients(h, s, sv, b.coef, b.grad, p.pitch, v0, (cols + kTile - 1) / kTile, w, ldw, after, st));
+        NA1D_HEAD_TRY(products(h, s, sv, b.grad, p, v0, cols, i > 0, b.part_x, b.part_w, f, w, ldw, st));
         if (f.dx || f.cols || f.own_classes) NA1D_HEAD_TRY(finish(h, f, st));
     }
     return NA1D_OK;

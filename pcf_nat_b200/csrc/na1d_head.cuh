@@ -104,7 +104,6 @@ struct Pieces {
     int d_tiles, d_width;                       // tiles over D and their width
     int splits_x, splits_w;                     // of the contractions
     bool direct_w;                              // the weight's gradient leaves the products as it is: no partial sums
-    bool both;                                  // one kernel forms the gradients of the logits and the weight's (na1d_head_both.cu); the former lie transposed
 };
 Pieces pieces_of(const Shape& s, bool want_x, bool want_w);
 
@@ -139,9 +138,6 @@ cudaError_t gradients(const na1d_head& h, const Shape& s, const Saved& sv, const
                       int64_t ldw, bool after, cudaStream_t st);
 cudaError_t products(const na1d_head& h, const Shape& s, const Saved& sv, const void* grad, const Pieces& p, int64_t v0, int64_t cols, bool add, float* part_x,
                      float* part_w, const FinishArgs& f, const void* w, int64_t ldw, cudaStream_t st);
-cudaError_t gradients_and_weight(const na1d_head& h, const Shape& s, const Saved& sv, const float* coef, void* grad, int64_t pitch, int64_t v0, int64_t cols, float* part_w,
-                                 const FinishArgs& f, const void* w, int64_t ldw, bool after, cudaStream_t st);
-int both_read_status();
 int logits_read_status();
 int grad_read_status();
 

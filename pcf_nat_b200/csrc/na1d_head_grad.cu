@@ -36,7 +36,7 @@ struct Args {
     float *part_x, *part_w;
     long long Np, Dq, piece_rows;                    // rows of a split's partial sums and their pitch
     int D, d_tiles, d_width, v0, cols, tiles, splits_x, splits_w, stages;
-    bool want_x, want_w, add, direct, transposed;    // transposed: G lies with a class to a row
+    bool want_x, want_w, add, direct;
     FinishArgs f;
 };
 struct Item {
@@ -192,7 +192,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) grad_ke
                     const uint32_t full = pair::in_leader(&bar.full[slot]);
                     uint8_t* s = smem + slot * kStageBytes;
                     if (rank == 0) ptx::mbar_expect_tx(&bar.full[slot], 2 * (kOperand + (two ? 2 : 1) * kBox));
-                    if (t.rows && !g.transposed) {
+                    if (t.rows) {
                         pair::load_2d(s, &maps.g_rows, full, k * kStep, m);
                     } else {
                         pair::load_2d(s, &maps.g_cols, full, m, k * kStep);
@@ -224,15 +224,14 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) grad_ke
             bool ok = true;
             while (ok && next_item(g, p, walk, pairs, t)) {
                 if (t.k0 == t.k1) continue;
-                const bool along = t.rows && !g.transposed;
-                const uint32_t d = tmem + (it & 1) * kTile, idesc = along ? rows_desc : cols_desc, a_step = along ? 32 : 2048;
+                const uint32_t d = tmem + (it & 1) * kTile, idesc = t.rows ? rows_desc : cols_desc, a_step = t.rows ? 32 : 2048;
                 if (!ptx::mbar_wait(&bar.acc_empty[it & 1], ((it >> 1) & 1) ^ 1) || *abort_flag) { atomicExch(&g_head_status, 2); *abort_flag = 1; break; }
                 ptx::tc_fence_after_sync();
                 for (int k = t.k0; k < t.k1; ++k) {
                     if (!ptx::mbar_wait(&bar.full[slot], phase) || *abort_flag) { atomicExch(&g_head_status, 3); *abort_flag = 1; ok = false; break; }
                     ptx::tc_fence_after_sync();
                     const uint32_t s = ptx::smem_u32(smem + slot * kStageBytes);
-                    const uint64_t a = along ? pair::k_major(s) : pair::mn_major(s, kBox), b = pair::mn_major(s + kOperand, kBox);
+                    const uint64_t a = t.rows ? pair::k_major(s) : pair::mn_major(s, kBox), b = pair::mn_major(s + kOperand, kBox);
 #pragma unroll
                     for (int j = 0; j < kStep / 16; ++j)
                         pair::mma_ss(d, tc::desc_advance(a, j * a_step), tc::desc_advance(b, j * 2048), idesc, k > t.k0 || j > 0);
@@ -353,7 +352,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) grad_ke
 template <typename E, bool PROJECT>
 cudaError_t run(const Shape& s, const Saved& sv, const void* grad, Args a, int64_t pitch, const void* w, int64_t ldw, int dtype, cudaStream_t st) {
     Maps maps;
-    const int64_t dg[2] = {a.transposed ? s.Np : pitch, a.transposed ? pitch : s.Np}, sg[1] = {dg[0]}, dx[2] = {s.D, s.Np}, sx[1] = {s.Dp}, dw[2] = {s.D, s.V}, sw[1] = {ldw};
+    const int64_t dg[2] = {pitch, s.Np}, sg[1] = {pitch}, dx[2] = {s.D, s.Np}, sx[1] = {s.Dp}, dw[2] = {s.D, s.V}, sw[1] = {ldw};
     const int along[2] = {64, kHalf}, across[2] = {64, kStep};
     if (!make_matrix_map(&maps.g_rows, grad, dtype, 2, dg, sg, along) || !make_matrix_map(&maps.g_cols, grad, dtype, 2, dg, sg, across) ||
         !make_matrix_map(&maps.x, sv.x, dtype, 2, dx, sx, across) || !make_matrix_map(&maps.w, w, dtype, 2, dw, sw, across) ||
@@ -379,9 +378,9 @@ cudaError_t products(const na1d_head& h, const Shape& s, const Saved& sv, const 
     a.Np = s.Np; a.Dq = s.Dp; a.piece_rows = p.pitch;
     a.D = (int)s.D; a.d_tiles = p.d_tiles; a.d_width = p.d_width; a.v0 = (int)v0; a.cols = (int)cols;
     a.tiles = (int)((cols + kTile - 1) / kTile); a.splits_x = p.splits_x; a.splits_w = p.splits_w;
-    a.want_x = part_x != nullptr; a.want_w = part_w != nullptr && !p.both; a.transposed = p.both; a.add = add; a.direct = p.direct_w;
+    a.want_x = part_x != nullptr; a.want_w = part_w != nullptr; a.add = add; a.direct = p.direct_w;
     a.f = f;
-    const bool project = a.want_w && p.direct_w && s.norm;
+    const bool project = p.direct_w && s.norm;
     if (h.dtype == NA1D_BF16) return project ? run<__nv_bfloat16, true>(s, sv, grad, a, p.pitch, w, ldw, 0, st) : run<__nv_bfloat16, false>(s, sv, grad, a, p.pitch, w, ldw, 0, st);
     return project ? run<__half, true>(s, sv, grad, a, p.pitch, w, ldw, 1, st) : run<__half, false>(s, sv, grad, a, p.pitch, w, ldw, 1, st);
 }

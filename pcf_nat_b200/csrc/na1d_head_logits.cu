@@ -56,6 +56,11 @@ __device__ __forceinline__ float exp2_fast(float x) {
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
+__device__ __forceinline__ float log2_fast(float x) {   // (2^-22 of the logarithm: less than 16 bits of a gradient show)
+    float y;
+    asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
 __device__ __forceinline__ void store_tile(const CUtensorMap* map, const void* src, int c0, int c1) {
     asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.tile.bulk_group [%0, {%2, %3}], [%1];"
                  ::"l"(reinterpret_cast<uint64_t>(map)), "r"(ptx::smem_u32(src)), "r"(c0), "r"(c1) : "memory");
@@ -213,7 +218,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) logits_
             bool negative = false;
             if (GRAD && live) {
                 out = row_factor(up, ix, row.coef, NORM);
-                shift = log2f(fabsf(out)) - row.lse2;
+                shift = log2_fast(fabsf(out)) - row.lse2;
                 negative = out < 0.f;
                 if (!TOP && target >= 0) at_target = own_gradient(row.slope, out, NORM ? g.iw[target] : 1.f, NORM);
             }

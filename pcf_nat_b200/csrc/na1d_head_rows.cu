@@ -143,11 +143,21 @@ __device__ __forceinline__ bool row_counts(const PrepareArgs& a, int i) {
     }
     return false;
 }
+// the largest of a block's warps' values (the same in all lanes) into *word, as bits (one atomic a block, in whatever order)
+__device__ __forceinline__ void block_most(float most, int* word, float* most_s) {
+    if ((threadIdx.x & 31) == 0) most_s[threadIdx.x >> 5] = most;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        for (int w = 1; w < kWarps; ++w) most = fmaxf(most, most_s[w]);
+        if (most > 0.f) atomicMax(word, __float_as_int(most));
+    }
+}
 // Blocks below row_blocks take `per_block` rows each. Such a block counts the rows before its own itself: labels are few bytes, and no block waits for
 // another. The others take the weight: a copy in 16 bits where the products cannot read it as it is, and its rows' lengths.
 template <typename E>
 __global__ void __launch_bounds__(kThreads) prepare_kernel(const __grid_constant__ PrepareArgs a) {
     __shared__ int sums[kWarps], places[kThreads], base_s;
+    __shared__ float most_s[kWarps];
     extern __shared__ int classes_s[];
     wait_for_predecessor();
     if (blockIdx.x == 0 && threadIdx.x == 0) a.words->ticket = 0;
@@ -176,7 +186,7 @@ __global__ void __launch_bounds__(kThreads) prepare_kernel(const __grid_constant
             if (a.norm && lane == 0) a.iw[v] = iw;
             most = fmaxf(most, iw);
         }
-        if (a.relative && lane == 0 && most > 0.f) atomicMax(&a.words->most_iw, __float_as_int(most));   // (the largest, in whatever order)
+        if (a.relative) block_most(most, &a.words->most_iw, most_s);
         return;
     }
     const int r0 = min(a.N, (int)blockIdx.x * a.per_block), r1 = min(a.N, r0 + a.per_block);
@@ -236,7 +246,7 @@ __global__ void __launch_bounds__(kThreads) prepare_kernel(const __grid_constant
     const long long pad = (long long)(a.Np - a.N) * (a.Dp / 8);   // 16-byte pieces behind the last row
     for (long long e = (long long)blockIdx.x * kThreads + threadIdx.x; e < pad; e += (long long)a.row_blocks * kThreads)
         reinterpret_cast<uint4*>(out + (size_t)a.N * a.Dp)[e] = make_uint4(0, 0, 0, 0);
-    if (a.relative && lane == 0 && most > 0.f) atomicMax(&a.words->most_ix, __float_as_int(most));
+    if (a.relative) block_most(most, &a.words->most_ix, most_s);
     if (r0 < a.N && r1 == a.N && threadIdx.x == 0) a.words->counted = base;
 }
 
@@ -434,12 +444,14 @@ __device__ __forceinline__ void finish_row(void* out, int type, long long at, co
             for (int e = 0; e < 8; ++e) s[e] = fmaf(rest[i], x[e], s[e]);
         }
     };
-    float along = 0.f;
+    float along = 0.f, kept[8];   // (rows of up to 256: a lane has eight columns, which are added up once)
     if (norm) {
         for (int j = lane; j < Dp / 8; j += 32) {
             float x[8], s[8];
             unpack_row(own, j, x);
             sum(j, s);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) kept[e] = s[e];
 #pragma unroll
             for (int e = 0; e < 8; ++e) along = fmaf(x[e], 8 * j + e < D ? s[e] : 0.f, along);
         }
@@ -448,7 +460,12 @@ __device__ __forceinline__ void finish_row(void* out, int type, long long at, co
     const bool wide = D % 8 == 0 && type != NA1D_FP32;
     for (int j = lane; j < Dp / 8; j += 32) {
         float s[8];
-        sum(j, s);
+        if (norm && Dp <= 256) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) s[e] = kept[e];
+        } else {
+            sum(j, s);
+        }
         if (norm) {
             float x[8];
             unpack_row(own, j, x);
