@@ -86,8 +86,8 @@ Pieces pieces_of(const Shape& s, bool want_x, bool want_w) {
     // than its share; then their gradients leave at once, unless the way back through the normalisation needs more than one tile of a row.
     const int64_t steps_x = p.pitch / 64, steps_w = s.Np / 64;
     const int64_t items_x = want_x ? s.Np / kTile * p.d_tiles : 0, tiles_w = want_w ? p.piece_tiles * p.d_tiles : 0;
-    const int64_t share = (items_x * steps_x + tiles_w * steps_w + pairs - 1) / pairs, most = share + share / 4 < 16 ? 16 : share + share / 4;
-    p.splits_w = (int)(most >= steps_w ? 1 : (steps_w + most - 1) / most < 16 ? (steps_w + most - 1) / most : 16);
+    const int64_t share = (items_x * steps_x + tiles_w * steps_w + pairs - 1) / pairs, whole = share + share / 4 < 16 ? 16 : share + share / 4;
+    p.splits_w = (int)(whole >= steps_w ? 1 : (steps_w + whole - 1) / whole < 16 ? (steps_w + whole - 1) / whole : 16);
     p.direct_w = want_w && p.splits_w == 1 && (!s.norm || p.d_tiles == 1);
     // Splits of the rows' contraction, which fill up what the weight's items leave of the pairs' time: the end of the last pair (a step takes about
     // half a microsecond) against the partial sums' way to memory and back (4 TB/s; the normalised ones of wide rows are read twice).
