@@ -14,7 +14,7 @@ namespace {
 __device__ int g_head_status = 0;
 
 constexpr int kEpilogue = 16;                       // warps; each reaches 32 lanes of tensor memory, and takes a quarter of a tile's columns
-constexpr int kThreads = 128 + 32 * kEpilogue;      // warp 0: loads, 1: MMA issue, 2: tensor memory, from 4 on: epilogue
+constexpr int kThreads = 64 + 32 * kEpilogue;       // warp 0: tensor memory and loads, 1: MMA issue, from 2 on: epilogue
 constexpr int kWidth = kTile * 4 / kEpilogue;       // columns of a warp
 constexpr int kStep = 64, kHalf = 128;
 constexpr int kOperand = kHalf * kStep * 2;         // 16 KB: 128 rows of 64 channels
@@ -120,7 +120,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) logits_
         ptx::prefetch_tensormap(lane ? &maps.w : &maps.x);
         if (GRAD && lane == 0) ptx::prefetch_tensormap(&maps.out);
     }
-    if (warp == 2) { pair::tmem_alloc(&bar.tmem, kCols); pair::tmem_relinquish(); }
+    if (warp == 0) { __syncwarp(); pair::tmem_alloc(&bar.tmem, kCols); pair::tmem_relinquish(); }
     ptx::tc_fence_before_sync();
     __syncthreads();
     pair::cluster_sync();
@@ -175,11 +175,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) logits_
                 if (ok) pair::commit(&bar.acc_full[it & 1]);
             }
         }
-    } else if (warp >= 4) {
-        const int q = warp & 3, h = (warp - 4) >> 2;   // tensor-memory lanes 32 q .. + 31 (those a warp reaches), quarter h of the columns
+    } else {
+        const int q = warp & 3, h = (warp - 2) >> 2;   // tensor-memory lanes 32 q .. + 31 (those a warp reaches), quarter h of the columns
         const uint32_t lanes = (uint32_t)(q * 32) << 16;
         const float up = GRAD ? gradient_scale(g.words, g.fp16, NORM) : 1.f;
-        uint8_t* out_rows = smem + kStages * kStageBytes + (warp - 4) * kOut;
+        uint8_t* out_rows = smem + kStages * kStageBytes + (warp - 2) * kOut;
         // what belongs to a tile's row: asked for while the tile before is worked on
         struct Row {
             int target, place;
@@ -245,7 +245,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) logits_
             ptx::tc_fence_after_sync();
             const uint32_t acc = tmem + lanes + (it & 1) * kTile + h * kWidth;
             float most = FIXED ? g.cs : -INFINITY, sum = 0.f;
-#pragma unroll 1
+#pragma unroll(GRAD ? 1 : 2)
             for (int n = 0; n < kWidth; n += 32) {
                 float d[32];
                 float2 iw[NORM ? 16 : 1];
@@ -379,7 +379,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) logits_
     ptx::tc_fence_before_sync();
     __syncthreads();
     pair::cluster_sync();   // neither CTA leaves while the other may still signal it or read its operands
-    if (warp == 2) pair::tmem_dealloc(tmem, kCols);
+    if (warp == 0) pair::tmem_dealloc(tmem, kCols);
 }
 
 template <typename E, bool GRAD, bool NORM, bool TOP, bool FIXED = false>
