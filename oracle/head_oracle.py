@@ -42,7 +42,9 @@ def losses(x, w, labels=None, teacher_logits=None, teacher_index=None, scale=1.0
     z = logits(x, w, scale, normalize, labels, margin)[0]
     if labels is not None:
         counted = labels != ignore
-        each = torch.logsumexp(z, 1) - z.gather(1, labels.clamp(0, w.shape[0] - 1)[:, None]).squeeze(1)
+        at = labels.clamp(0, w.shape[0] - 1)[:, None]
+        others = torch.logsumexp(z.scatter(1, at, -math.inf), 1) - z.gather(1, at).squeeze(1)   # (small losses keep their digits)
+        each = torch.logaddexp(others, torch.zeros_like(others))
     else:
         q, counted = teacher_probabilities(teacher_logits, teacher_index, temperature)
         log_p = torch.log_softmax(z / temperature, 1).gather(1, teacher_index.clamp_min(0))

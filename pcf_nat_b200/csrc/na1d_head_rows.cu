@@ -329,19 +329,25 @@ __global__ void __launch_bounds__(kThreads) combine_kernel(const __grid_constant
                     z = z * a.cos_m - sine * a.sin_m;
                 }
                 z *= a.p.cs;
-                // the other classes' sum against the target: others = sum 2^(z_v - top), top the largest of all
-                const float top = fmaxf(m, z), others = s * exp2_fast((m > -INFINITY ? m : top) - top), own = exp2_fast(z - top);
-                const float all = others + own;
-                loss = z == top ? log1pf(others) : fmaf(top - z, kLn2, logf(all));
+                // the other classes' sum against the target's term: a small loss is this ratio, with its relative accuracy
+                const float above = m - z, ratio = s * exp2f(above);
+                const bool small = ratio < 1e30f || ratio != ratio;
+                loss = small ? log1pf(ratio) : fmaf(above, kLn2, logf(s));
                 if (lane == 0) {
-                    a.lse2[c] = top + log2f(all);
-                    a.slope[c] = -(others / all) * slope;
+                    a.lse2[c] = small ? z + log2f(1.f + ratio) : m + log2f(s);
+                    a.slope[c] = -(small ? ratio / (1.f + ratio) : 1.f) * slope;
                     own_row(target, c);
                 }
             }
         } else {
-            const float lse2 = m + log2f(s);
             const size_t at = (size_t)a.row[c] * a.k;
+            // everything against the largest entry, near which the sum's logarithm is small: log p = z - top - log(sum / 2^top)
+            float top = -INFINITY;
+            for (int e = lane; e < a.k; e += 32)
+                if (a.index[at + e] != kNoClass) top = fmaxf(top, a.entry[at + e]);
+            top = warp_max(top);
+            if (!(top > -INFINITY)) top = m;
+            const float over = exp2f(m - top) * s < 1e30f ? log2f(exp2f(m - top) * s) : (m - top) + log2f(s), lse2 = top + over;
             // (a class that comes twice has its entries side by side: all of them take the gradient of the class)
             float best = -1.f, own = 0.f;
             int own_class = kBad;
@@ -350,7 +356,7 @@ __global__ void __launch_bounds__(kThreads) combine_kernel(const __grid_constant
                 const float q = a.q[at + e];
                 if (q != q) loss = q;
                 if (v == kNoClass) continue;
-                const float z2 = a.entry[at + e] - lse2;
+                const float z2 = (a.entry[at + e] - top) - over;
                 if (q > 0.f) loss += q * (logf(q) - z2 * kLn2);
                 float all = q;
                 for (int o = e - 1; o >= 0 && a.index[at + o] == v; --o) all += a.q[at + o];

@@ -188,6 +188,23 @@ def test_large_logits(dtype):
 
 
 @pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("cosine", [False, True])
+def test_small_losses_keep_their_relative_accuracy(cosine, dtype):
+    """Rows that are sure of their class: the loss is the others' share, log1p(r), and off by no more than r is, relative to itself."""
+    N, D, V = 300, 256, 200
+    x, w, y = make(N, D, V, dtype, cosine=cosine)
+    x = (x.float() + torch.linspace(0, 12, N, device=DEV)[:, None] * torch.nn.functional.normalize(w[y].float(), dim=1)).to(dtype)
+    if cosine:
+        loss = b200.angular_cross_entropy(x, w, y, margin=0.0, scale=30.0, reduction="none")
+        r = orc.evaluate(x, w, labels=y, scale=30.0, normalize=True, reduction="none")
+    else:
+        loss = b200.linear_cross_entropy(x, w, y, reduction="none")
+        r = orc.evaluate(x, w, labels=y, reduction="none")
+    assert float(r["loss"].min()) < 1e-3
+    near(loss, r["loss"], r["loss"] * (r["loss_off"] + 2.0 ** -22), "loss")
+
+
+@pytest.mark.parametrize("dtype", TYPES)
 def test_rows_and_classes_of_zeros(dtype):
     x, w, y = make(60, 64, 100, dtype, cosine=True)
     x[5] = 0
