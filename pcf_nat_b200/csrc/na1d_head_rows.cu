@@ -307,7 +307,18 @@ __global__ void __launch_bounds__(kThreads) combine_kernel(const __grid_constant
     if (c < counted) {
         float m = -INFINITY, s = 0.f;
         const float2* part = a.part + (size_t)c * a.parts;
-        for (int p = lane; p < a.parts; p += 32) {
+        int p = lane;
+        for (; p + 96 < a.parts; p += 128) {   // four loads at a time
+            float2 v[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) v[i] = part[p + 32 * i];
+            const float to = fmaxf(fmaxf(fmaxf(v[0].x, v[1].x), fmaxf(v[2].x, v[3].x)), m), by = to > -INFINITY ? to : 0.f;
+            s *= exp2_fast(m - by);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) s = fmaf(v[i].y, exp2_fast(v[i].x - by), s);
+            m = to;
+        }
+        for (; p < a.parts; p += 32) {
             const float2 v = part[p];
             const float to = fmaxf(m, v.x), by = to > -INFINITY ? to : 0.f;
             s = s * exp2_fast(m - by) + v.y * exp2_fast(v.x - by);
@@ -490,7 +501,7 @@ __device__ __forceinline__ void finish_row(void* out, int type, long long at, co
 template <typename E>
 __global__ void __launch_bounds__(kThreads, 3) finish_kernel(const __grid_constant__ FinishArgs a) {
     wait_for_predecessor();
-    const int lane = threadIdx.x & 31, counted = a.words->counted, n = (a.dx || a.own_classes ? a.N : 0) + a.cols;
+    const int lane = threadIdx.x & 31, counted = a.words->counted, first = a.cols + (a.dx ? a.N : 0), n = first + (a.own_classes ? a.N : 0);
     const float up = gradient_scale(a.words, a.fp16, a.norm), f = common_factor(a, counted, up);
     const E *x = static_cast<const E*>(a.x), *w = static_cast<const E*>(a.w);
     auto class_row = [&](int v, const float* part, long long split, int splits) {
@@ -517,19 +528,20 @@ __global__ void __launch_bounds__(kThreads, 3) finish_kernel(const __grid_consta
             class_row(a.v0 + i, a.part_w + (size_t)i * a.Dp, a.piece_rows * a.Dp, a.splits_w);
             continue;
         }
+        if (i >= first) {   // the class of a row, if it is the one that has the class's sums
+            const int c = a.place[i - first], v = c < 0 ? c : a.target[c];
+            if (v >= 0 && a.own_count[v] <= kOwn && a.own[(size_t)v * kOwn] == c) class_row(v, a.part_w + (size_t)c * a.Dp, 0, 1);
+            continue;
+        }
         const int r = i - a.cols, c = a.place[r];
         if (c < 0) {
-            if (a.dx)
-                for (int j = lane; j < a.D; j += 32) store_any(a.dx, a.x_type, (long long)r * a.D + j, 0.f);
+            for (int j = lane; j < a.D; j += 32) store_any(a.dx, a.x_type, (long long)r * a.D + j, 0.f);
             continue;
         }
         const int v = a.target[c];
-        if (a.dx) {
-            const float rest[kOwn] = {v >= 0 ? own_rest<E>(a, c, up) : 0.f};
-            finish_row<E>(a.dx, a.x_type, (long long)r * a.D, a.part_x + (size_t)c * a.Dp, a.Np * a.Dp, a.splits_x, x + (size_t)c * a.Dp, a.norm ? a.ix[c] : 1.f, f,
-                          v >= 0 ? 1 : 0, rest, [&](int) { return w + (size_t)v * a.ldw; }, a.norm, a.D, a.Dp, lane);
-        }
-        if (a.own_classes && v >= 0 && a.own_count[v] <= kOwn && a.own[(size_t)v * kOwn] == c) class_row(v, a.part_w + (size_t)c * a.Dp, 0, 1);
+        const float rest[kOwn] = {v >= 0 ? own_rest<E>(a, c, up) : 0.f};
+        finish_row<E>(a.dx, a.x_type, (long long)r * a.D, a.part_x + (size_t)c * a.Dp, a.Np * a.Dp, a.splits_x, x + (size_t)c * a.Dp, a.norm ? a.ix[c] : 1.f, f,
+                      v >= 0 ? 1 : 0, rest, [&](int) { return w + (size_t)v * a.ldw; }, a.norm, a.D, a.Dp, lane);
     }
 }
 
@@ -605,7 +617,7 @@ FinishArgs finish_args(const na1d_head& h, const Shape& s, const Saved& sv, void
     return a;
 }
 cudaError_t finish(const na1d_head& h, const FinishArgs& a, cudaStream_t st) {
-    const int blocks = blocks_for((a.dx || a.own_classes ? a.N : 0) + a.cols);
+    const int blocks = blocks_for((int64_t)(a.dx ? a.N : 0) + (a.own_classes ? a.N : 0) + a.cols);
     return launch(h.dtype == NA1D_BF16 ? finish_kernel<__nv_bfloat16> : finish_kernel<__half>, blocks, kThreads, 0, st, true, a);
 }
 
