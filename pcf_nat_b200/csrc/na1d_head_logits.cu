@@ -245,8 +245,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) logits_
             ptx::tc_fence_after_sync();
             const uint32_t acc = tmem + lanes + (it & 1) * kTile + h * kWidth;
             float most = FIXED ? g.cs : -INFINITY, sum = 0.f;
+            // (rows behind the last that counts are nobody's: the products contract over whole steps of 64)
+            const bool any_row = c - lane < (GRAD ? (counted + 63) / 64 * 64 : counted);
 #pragma unroll(GRAD ? 1 : 2)
             for (int n = 0; n < kWidth; n += 32) {
+                if (!any_row) break;
                 float d[32];
                 float2 iw[NORM ? 16 : 1];
                 const int col = v + n;
@@ -362,7 +365,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) logits_
             ptx::tc_fence_before_sync();
             __syncwarp();
             if (lane == 0) pair::arrive_cluster(pair::in_leader(&bar.acc_empty[it & 1]));
-            if (GRAD) {
+            if (GRAD && any_row) {
                 ptx::fence_proxy_async_smem();
                 __syncwarp();
                 if (lane == 0) {
