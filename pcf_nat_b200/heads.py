@@ -137,8 +137,8 @@ def _run(dt, x, weight, labels, teacher_logits, teacher_index, cfg, reduction):
     shape = x.shape[:-1]
     x2 = x.reshape(-1, x.shape[-1])
     if x2.shape[0] == 0:
-        # no rows: a loss of zero that still belongs to the graph
-        zero = (x.sum(dtype=torch.float32) + weight.sum(dtype=torch.float32) * 0) * 0
+        # no rows: a loss of zero that still belongs to the graph (of no row of the weight either: it may hold infinities)
+        zero = x.sum(dtype=torch.float32) + weight[:0].sum(dtype=torch.float32)
         return zero if reduction != "none" else zero.expand(shape) + torch.zeros(shape, device=x.device)
     if x2.stride(1) != 1:
         x2 = x2.contiguous()

@@ -139,6 +139,15 @@ def test_no_rows():
     assert b200.linear_cross_entropy(x, w, y, reduction="none").shape == (0,)
 
 
+@pytest.mark.parametrize("reduction", ["mean", "sum", "none"])
+def test_no_rows_of_a_weight_with_infinities(reduction):
+    x, w = torch.zeros(0, 64, device=DEV, dtype=torch.bfloat16, requires_grad=True), torch.full((30, 64), float("inf"), device=DEV).bfloat16().requires_grad_()
+    loss = b200.linear_cross_entropy(x, w, torch.zeros(0, dtype=torch.int64, device=DEV), reduction=reduction)
+    assert not loss.any() and loss.shape == ((0,) if reduction == "none" else ())
+    loss.sum().backward()
+    assert w.grad.shape == w.shape and not w.grad.any()
+
+
 @pytest.mark.parametrize("op", ["ce", "angular"])
 def test_a_label_that_is_no_class_shows(op):
     x, w, y = make(40, 64, 100, torch.bfloat16)
