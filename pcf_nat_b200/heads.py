@@ -159,6 +159,12 @@ def _labels_loss(x, weight, labels, cfg, reduction):
     return _run(dt, x, weight, labels.reshape(-1).to(torch.int64).contiguous(), None, None, cfg, reduction)
 
 
+def _numbers(**named):
+    for name, v in named.items():
+        if isinstance(v, torch.Tensor):   # (it would be read back from the device, and get no gradient)
+            raise TypeError("%s is a number, got a tensor" % name)
+
+
 def _tensors(*ts):
     return all(isinstance(t, torch.Tensor) for t in ts) and not torch.compiler.is_compiling()
 
@@ -171,6 +177,7 @@ def linear_cross_entropy(x, weight, labels, *, scale=1.0, ignore_index=-100, red
     them reaches the loss or a gradient, and no time goes into them; where no row counts the mean is 0. A label outside the classes makes
     its row's loss, and the gradients that depend on it, NaN (there is no synchronisation to raise an error from). ``reduction``: "mean" over
     the rows that count, "sum", or "none" (0 for the others). Differentiable once in ``x`` and ``weight``; same bits from run to run."""
+    _numbers(scale=scale, ignore_index=ignore_index)
     loss = None
     if _tensors(x, weight, labels):
         loss = ops.native.head(x, weight, labels, None, None, scale, 0.0, 1.0, False, ignore_index, _REDUCTION.get(reduction, -1))
@@ -181,6 +188,7 @@ def angular_cross_entropy(x, weight, labels, *, margin=0.2, scale=30.0, ignore_i
     """AAM-softmax: cross entropy of ``scale`` times the cosines of rows and classes, the label's angle widened by ``margin`` radians
     (``model.AAMSoftmax``; cos(a + m) as cos a cos m - sin a sin m, the squared sine at least 2e-7). A row or class of zeros has cosine 0 with
     all others and no gradient. Otherwise as ``linear_cross_entropy``."""
+    _numbers(margin=margin, scale=scale, ignore_index=ignore_index)
     loss = None
     if _tensors(x, weight, labels):
         loss = ops.native.head(x, weight, labels, None, None, scale, margin, 1.0, True, ignore_index, _REDUCTION.get(reduction, -1))
@@ -194,6 +202,7 @@ def linear_distillation(x, weight, teacher_logits, teacher_index, *, temperature
     ``teacher_logits`` (..., k) of any floating type, ``teacher_index`` (..., k) int64 or int32: the entries' classes, negative where there is
     no entry (its logit is not read). Rows without an entry do not count; a class may come twice. k is at most 1024. No gradient
     goes to the teacher. Otherwise as ``linear_cross_entropy``."""
+    _numbers(temperature=temperature, scale=scale)
     if _tensors(x, weight, teacher_logits, teacher_index):
         loss = ops.native.head(x, weight, None, teacher_logits, teacher_index, scale, 0.0, temperature, normalize, 0, _REDUCTION.get(reduction, -1))
         if loss is not None:

@@ -39,6 +39,22 @@ def test_label_losses_refuse(f):
         f(x, w, y[:3])
 
 
+def test_numbers_that_are_tensors_are_refused():
+    x, w, y = _args()
+    one = torch.ones((), requires_grad=True)
+    for f in (b200.linear_cross_entropy, b200.angular_cross_entropy):
+        with pytest.raises(TypeError, match="scale is a number"):
+            f(x, w, y, scale=one)
+        with pytest.raises(TypeError, match="ignore_index is a number"):
+            f(x, w, y, ignore_index=torch.tensor(3))
+    with pytest.raises(TypeError, match="margin is a number"):
+        b200.angular_cross_entropy(x, w, y, margin=one)
+    t, i = torch.zeros(4, 3), torch.zeros(4, 3, dtype=torch.int64)
+    for name in ("scale", "temperature"):
+        with pytest.raises(TypeError, match=name + " is a number"):
+            b200.linear_distillation(x, w, t, i, **{name: one})
+
+
 def test_distillation_refuses():
     x, w, _ = _args()
     t, i = torch.zeros(4, 3), torch.zeros(4, 3, dtype=torch.int64)
