@@ -578,7 +578,8 @@ cudaError_t prepare(const na1d_head& h, const Shape& s, const Saved& sv, int* fl
     a.row_blocks = (int)((s.N + a.per_block - 1) / a.per_block);
     a.row_blocks = a.row_blocks < 16 ? 16 : a.row_blocks;   // (a few rows: the others fill up the tile with zeros)
     // Few rows find out by themselves which of them have a teacher (a row's first entry tells, mostly): a launch less. Many would look at all rows
-    // before theirs once for each block (1003 rows of up to 20 entries: 12 us more).
+    // before theirs once for each block (a pass in a graph: 85 us against 75 with the launch at 1003 rows of up to 20 entries,
+    // 49.8 against 49.2 at 256 of 32, 45.1 either way at 16 of 8).
     const bool early = s.N * s.k > 8192;
     size_t smem = 0;
     if (s.k) {
