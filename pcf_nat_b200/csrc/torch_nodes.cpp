@@ -1157,11 +1157,16 @@ struct NA1dHead : public torch::autograd::Function<NA1dHead> {
             const Tensor saved = aligned(s[0], 256);
             const c10::cuda::CUDAGuard guard(saved.device());
             Tensor w = s[1];
-            if (d["in_place"].toBool()) {   // wherever a hook has put it
-                if (w.stride(1) != 1 || w.stride(0) % 8 != 0 || w.stride(0) < w.size(1)) w = w.contiguous();
-                w = w.storage_offset() % 8 == 0 && (reinterpret_cast<uintptr_t>(w.data_ptr()) & 15) == 0 ? w : w.clone(at::MemoryFormat::Contiguous);
-                h.weight = ptr(w);
-                h.weight_stride = w.stride(0);
+            if (d["in_place"].toBool()) {   // wherever a hook has put it; `saved` has no room for a copy, so the kernels have to read it there
+                auto take = [&] {
+                    h.weight = ptr(w);
+                    h.weight_stride = w.stride(0);
+                    return w.stride(1) == 1 && head_in_place(h);
+                };
+                if (!take()) {              // (contiguous() would leave a single row with any stride)
+                    w = w.clone(at::MemoryFormat::Contiguous);
+                    TORCH_CHECK(take(), "a head's weight came back from a saved-tensor hook in a form that it did not have");
+                }
             }
             const bool want_x = ctx->needs_input_grad(0), want_w = ctx->needs_input_grad(1);
             const Tensor d_loss = grads[0].scalar_type() == at::kFloat && grads[0].is_contiguous() ? grads[0] : grads[0].to(at::kFloat).contiguous();
