@@ -78,7 +78,8 @@ class _HeadFunction(torch.autograd.Function):
         head, want_x, want_w = _lib.Head.from_buffer_copy(ctx.head), ctx.needs_input_grad[0], ctx.needs_input_grad[1]
         dev = saved.device
         with ops._on_device(dev):
-            if saved.data_ptr() % 256:                  # (saved tensors come back from wherever a hook has put them)
+            saved = saved.contiguous()                  # (saved tensors come back from wherever a hook has put them, in any stride)
+            if saved.data_ptr() % 256:
                 saved = saved.clone()
             head.x = head.labels = head.teacher_logits = head.teacher_index = saved.data_ptr()   # not read any more
             if ctx.in_place:

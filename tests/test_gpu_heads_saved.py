@@ -39,3 +39,25 @@ def test_weight_in_padded_rows_with_an_aligned_start(classes, python, monkeypatc
         assert padded.stride(0) == 67 and padded.data_ptr() % 16 == 0
         return padded
     _same(step, unpack, python, monkeypatch)
+
+
+@pytest.mark.parametrize("python", [False, True])
+def test_kept_buffer_with_a_stride(python, monkeypatch):
+    """Every second byte of a larger tensor: rows, entries and places in it would be read as anything."""
+    g = torch.Generator(device=DEV).manual_seed(3)
+    x = torch.randn(200, 64, device=DEV, generator=g).bfloat16()
+    w = (0.2 * torch.randn(500, 64, device=DEV, generator=g)).bfloat16()
+    t, i = torch.randn(200, 5, device=DEV, generator=g), torch.randint(0, 500, (200, 5), device=DEV, generator=g)
+
+    def step():
+        x1, w1 = x.clone().requires_grad_(), w.clone().requires_grad_()
+        return torch.autograd.grad(b200.linear_distillation(x1, w1, t, i), (x1, w1))
+
+    def unpack(t):
+        if t.dim() != 1:
+            return t
+        wide = t.new_zeros(2 * t.numel())
+        wide[::2] = t
+        assert wide[::2].stride(0) == 2 and wide.data_ptr() % 256 == 0
+        return wide[::2]
+    _same(step, unpack, python, monkeypatch)
