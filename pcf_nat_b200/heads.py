@@ -120,7 +120,15 @@ def _rows(x, weight, reduction):
         raise ValueError("reduction is 'mean', 'sum' or 'none', got %r" % (reduction,))
     if torch.compiler.is_compiling():
         raise NotImplementedError("the losses of a head are eager operators")
+    _no_tangents(x, weight)
     return _compute_type(x, weight)
+
+
+def _no_tangents(*ts):
+    """Forward-mode differentiation is refused: a tangent on an input that needs no gradient would be dropped without a word. (The C++ node does not
+    take such inputs.)"""
+    if any(isinstance(t, torch.Tensor) and torch.autograd.forward_ad.unpack_dual(t).tangent is not None for t in ts):
+        raise NotImplementedError("the losses of a head have no forward-mode derivative")
 
 
 def _index(t, shape, name):
@@ -210,6 +218,7 @@ def linear_distillation(x, weight, teacher_logits, teacher_index, *, temperature
             return loss
     cfg = (0, float(scale), 0.0, float(temperature), bool(normalize))
     dt = _rows(x, weight, reduction)
+    _no_tangents(teacher_logits)
     if not isinstance(teacher_index, torch.Tensor) or teacher_index.dim() != x.dim() or teacher_index.shape[-1] == 0:
         raise ValueError("teacher_index is (..., k) for x (..., dim), k at least 1")
     _index(teacher_index, x.shape[:-1] + teacher_index.shape[-1:], "a teacher's classes")

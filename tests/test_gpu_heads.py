@@ -440,3 +440,25 @@ def test_weight_changed_between_the_passes():
         w.mul_(2)
     with pytest.raises(RuntimeError, match="modified by an inplace operation"):
         loss.backward()
+
+
+@pytest.mark.parametrize("python", [False, True])
+@pytest.mark.parametrize("op", ["ce", "angular", "distill"])
+def test_transforms_are_refused(op, python, monkeypatch):
+    """A tangent is not dropped, and the function transforms raise."""
+    if python:
+        monkeypatch.setattr(ops, "native", ops._PythonRoutes)
+    x, w, y, t, i = make(20, 64, 100, torch.bfloat16, k=4)
+    f = {"ce": lambda x, w, t: b200.linear_cross_entropy(x, w, y), "angular": lambda x, w, t: b200.angular_cross_entropy(x, w, y),
+         "distill": lambda x, w, t: b200.linear_distillation(x, w, t, i)}[op]
+    fwd = torch.autograd.forward_ad
+    for n in range(3 if op == "distill" else 2):
+        args = [x, w, t]
+        with fwd.dual_level():
+            args[n] = fwd.make_dual(args[n], torch.ones_like(args[n]))
+            with pytest.raises(NotImplementedError, match="forward-mode"):
+                f(*args)
+    with pytest.raises(RuntimeError):
+        torch.func.vmap(lambda a: f(a, w, t))(torch.stack([x, x]))
+    with pytest.raises(RuntimeError):
+        torch.func.grad(lambda a: f(a, w, t))(x)

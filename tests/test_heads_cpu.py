@@ -122,3 +122,22 @@ def test_buffers_stay_far_below_the_logits(rows, dim, classes):
     assert saved <= padded * (2 * (dim + 8) + 64) + 64 * (classes + 256) + 4096   # (a copy of the rows, a few words for each row and class)
     # a piece's gradients (at most 256 MB, or 1024 classes of them), and both products' partial sums
     assert back <= max(256 << 20, padded * 1024 * 2) + 33 * 4 * (dim + 8) * padded + 17 * 4 * (dim + 8) * (classes + 256) + 4096
+
+
+@pytest.mark.parametrize("requires_grad", [False, True])
+@pytest.mark.parametrize("op,dual", [(op, dual) for op in ("ce", "angular", "distill") for dual in ("x", "weight", "teacher") if dual != "teacher" or op == "distill"])
+def test_forward_mode_is_refused(op, dual, requires_grad):
+    """A tangent on any input, whether or not that input needs a gradient too."""
+    x, w, y = _args()
+    t, i = torch.zeros(4, 3), torch.zeros(4, 3, dtype=torch.int64)
+    f = {"ce": lambda x, w, t: b200.linear_cross_entropy(x, w, y), "angular": lambda x, w, t: b200.angular_cross_entropy(x, w, y),
+         "distill": lambda x, w, t: b200.linear_distillation(x, w, t, i)}[op]
+    args = [x, w, t]
+    n = ["x", "weight", "teacher"].index(dual)
+    with torch.autograd.forward_ad.dual_level():
+        args[n] = torch.autograd.forward_ad.make_dual(args[n].requires_grad_(requires_grad), torch.ones_like(args[n]))
+        with pytest.raises(NotImplementedError, match="forward-mode"):
+            f(*args)
+    args = [x, w, t]
+    with pytest.raises(NotImplementedError, match="forward-mode"):
+        torch.func.jvp(lambda a: f(*(a if j == n else b for j, b in enumerate(args))), (args[n].detach(),), (torch.ones_like(args[n]),))
