@@ -93,6 +93,7 @@ struct Shape {
     int64_t x_stride, w_stride;
     bool norm, train_classes, copy_w;
     float cs;                   // log2(e) scale / temperature: from a product (or cosine) to a power of two
+    int room;                   // 2^room times the largest gradient of a cosine's logit fits fp16
 };
 
 Shape shape_of(const na1d_head& h);
@@ -124,6 +125,7 @@ struct FinishArgs {
     long long Np, piece_rows, ldw;
     int N, D, Dp, cols, v0, splits_x, splits_w, x_type, w_type, reduction;
     float factor;
+    int room;
     bool fp16, norm;
     bool own_classes;           // part_w has the sums of classes that are rows' own, at such a row
 };
@@ -142,15 +144,15 @@ int logits_read_status();
 int grad_read_status();
 
 // power of two that a 16-bit gradient of logits is multiplied with. bf16: none. fp16 holds 6e-5 to 65504 in full: probabilities times 2^14;
-// normalised ones also carry the inverse norms, at most `most`, and the margin's slope (at most 450).
-__device__ __forceinline__ float gradient_scale(const Words* w, bool fp16, bool norm) {
+// normalised ones also carry the inverse norms, at most `most`, and the margin's slope, which `room` leaves space for.
+__device__ __forceinline__ float gradient_scale(const Words* w, bool fp16, bool norm, int room) {
     if (!fp16) return 1.f;
     if (!norm) return 16384.f;
     const float most = __int_as_float(w->most_ix) * __int_as_float(w->most_iw);
     if (!(most > 0.f) || most > 1e30f) return 1.f;
     int e;
     frexpf(most, &e);
-    e = 6 - e;
+    e = room - e;
     return ldexpf(1.f, e < -100 ? -100 : e > 100 ? 100 : e);
 }
 

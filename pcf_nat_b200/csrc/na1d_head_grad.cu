@@ -250,7 +250,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) grad_ke
         const int q = warp & 3, h = (warp - 4) >> 2;   // tensor-memory lanes 32 q .. + 31 (those a warp reaches); columns 16 h, 16 h + 64, ..
         const uint32_t lanes = (uint32_t)(q * 32) << 16;
         const int counted = g.words->counted, row = q * 32 + lane;
-        const float factor = g.direct ? common_factor(g.f, counted, gradient_scale(g.words, g.f.fp16, g.f.norm)) : 1.f;
+        const float factor = g.direct ? common_factor(g.f, counted, gradient_scale(g.words, g.f.fp16, g.f.norm, g.f.room)) : 1.f;
         const uint8_t* own_row = own_rows + row * 128;
         int it = 0, projected = 0;
         while (next_item(g, p, walk, pairs, t)) {

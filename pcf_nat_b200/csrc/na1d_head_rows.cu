@@ -504,7 +504,7 @@ template <typename E>
 __global__ void __launch_bounds__(kThreads, 3) finish_kernel(const __grid_constant__ FinishArgs a) {
     wait_for_predecessor();
     const int lane = threadIdx.x & 31, counted = a.words->counted, first = a.cols + (a.dx ? a.N : 0), n = first + (a.own_classes ? a.N : 0);
-    const float up = gradient_scale(a.words, a.fp16, a.norm), f = common_factor(a, counted, up);
+    const float up = gradient_scale(a.words, a.fp16, a.norm, a.room), f = common_factor(a, counted, up);
     const E *x = static_cast<const E*>(a.x), *w = static_cast<const E*>(a.w);
     auto class_row = [&](int v, const float* part, long long split, int splits) {
         float rest[kOwn];
@@ -615,7 +615,7 @@ FinishArgs finish_args(const na1d_head& h, const Shape& s, const Saved& sv, void
     a.slope = sv.slope; a.target = sv.target; a.own_count = sv.own_count; a.own = sv.own;
     a.Np = s.Np; a.piece_rows = p.pitch; a.ldw = ldw;
     a.N = (int)s.N; a.D = (int)s.D; a.Dp = (int)s.Dp; a.cols = (int)cols; a.v0 = (int)v0; a.splits_x = p.splits_x; a.splits_w = p.splits_w;
-    a.x_type = h.x_type; a.w_type = h.weight_type; a.reduction = h.reduction; a.norm = s.norm; a.fp16 = h.dtype == NA1D_FP16;
+    a.x_type = h.x_type; a.w_type = h.weight_type; a.reduction = h.reduction; a.norm = s.norm; a.fp16 = h.dtype == NA1D_FP16; a.room = s.room;
     a.factor = s.k ? h.scale * h.temperature : h.scale;
     return a;
 }
