@@ -343,11 +343,14 @@ typedef struct {
 int64_t na1d_head_saved_bytes(const na1d_head* head);
 int64_t na1d_head_forward_scratch(const na1d_head* head);
 int64_t na1d_head_backward_scratch(const na1d_head* head, int want_x, int want_weight);
+/* 1 where the kernels read the weight in its place, 0 where the forward pass keeps a copy in `saved` (negative: status code); host-only. The backward
+ * pass needs the answer of its forward: the same, with another weight pointer or stride. */
+int na1d_head_weight_in_place(const na1d_head* head);
 /* loss: (rows) with NA1D_HEAD_NONE, else one number. saved (256-byte aligned): kept for the backward pass; scratch (256-byte aligned): free
  * when the call's work is done. */
 int na1d_head_forward(const na1d_head* head, float* loss, void* saved, void* scratch, void* stream);
 /* d_x (rows, dim) and d_weight (classes, dim), dense, of x_type and weight_type, 32-byte aligned; either may be NULL. d_loss as loss. The
- * weight (and nothing else of the forward's inputs) is read again; saved is only read, so passes over it may overlap. */
+ * weight (and nothing else of the forward's inputs) is read again, where there is no copy of it; saved is only read, so passes over it may overlap. */
 int na1d_head_backward(const na1d_head* head, void* d_x, void* d_weight, const float* d_loss, void* saved, void* scratch, void* stream);
 
 /* ------------------------------------------------------------------------------------------

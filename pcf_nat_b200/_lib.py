@@ -136,6 +136,8 @@ _lib.na1d_head_forward_scratch.restype = _i64
 _lib.na1d_head_forward_scratch.argtypes = [_ptr]
 _lib.na1d_head_backward_scratch.restype = _i64
 _lib.na1d_head_backward_scratch.argtypes = [_ptr, _i32, _i32]
+_lib.na1d_head_weight_in_place.restype = _i32
+_lib.na1d_head_weight_in_place.argtypes = [_ptr]
 _lib.na1d_head_forward.restype = _i32
 _lib.na1d_head_forward.argtypes = [_ptr] * 5
 _lib.na1d_head_backward.restype = _i32

@@ -15,12 +15,15 @@ Shape shape_of(const na1d_head& h) {
     s.parts = (s.V + kTile - 1) / kTile * (kTile / kPart);
     s.x_stride = h.x_stride; s.w_stride = h.weight_stride;
     s.norm = h.normalize != 0;
-    // the weight is read where it is if its rows are whole 16-byte pieces
-    s.copy_w = h.weight_type != h.dtype || s.D % 8 != 0 || h.weight_stride % 8 != 0 || h.weight_stride < s.D || (reinterpret_cast<uintptr_t>(h.weight) & 15) != 0;
+    const bool fp16 = h.dtype == NA1D_FP16;
+    // the weight is read where it is if its rows are whole 16-byte pieces, and need no powers of two of their own
+    s.copy_w = (fp16 && s.norm) || h.weight_type != h.dtype || s.D % 8 != 0 || h.weight_stride % 8 != 0 || h.weight_stride < s.D || (reinterpret_cast<uintptr_t>(h.weight) & 15) != 0;
     s.cs = kLog2e * h.scale / (s.k ? h.temperature : 1.f);
-    // |p - 1| or |p - q| up to 1, times the margin's slope cos m + c / sin a sin m: 445 at a margin of 0.2, 2236 at a right angle
+    // fp16 holds 6e-5 to 65504 in full: probabilities times 2^14. Those of cosines carry the inverse lengths, up to 2^-lift each, and
+    // |p - 1| or |p - q| of up to 1 times the margin's slope cos m + c / sin a sin m: 445 at a margin of 0.2, 2236 at a right angle.
     const double slope = s.k || h.margin == 0.f ? 1.0 : std::fabs(std::cos((double)h.margin)) + std::fabs(std::sin((double)h.margin)) / std::sqrt((double)kSineFloor);
-    s.room = (int)std::floor(std::log2(65504.0 / (1.01 * slope)));   // (1 %: rounded cosines and lengths)
+    const int room = s.norm ? 2 * lift(true) + (int)std::floor(std::log2(65504.0 / (1.01 * slope))) : 14;   // (1 %: rounded cosines and lengths)
+    s.up = fp16 ? std::ldexp(1.f, room) : 1.f;
     return s;
 }
 
@@ -43,6 +46,8 @@ Saved saved_at(const na1d_head& h, const Shape& s, void* base) {
     if (s.norm) {
         v.ix = static_cast<float*>(take(s.Np * 4));
         v.iw = static_cast<float*>(take(round_up(s.V, kTile) * 4));
+        v.x_up = static_cast<float*>(take(s.Np * 4));
+        if (s.copy_w) v.w_up = static_cast<float*>(take(s.V * 4));
     }
     if (s.k) {
         v.q = static_cast<float*>(take(s.N * s.k * 4));
@@ -184,7 +189,6 @@ int forward(const na1d_head& h, float* loss, void* saved, void* scratch, cudaStr
     const Forward f = forward_at(s, scratch);
     const void* w = s.copy_w ? sv.w : h.weight;
     const int64_t ldw = s.copy_w ? s.Dp : h.weight_stride;
-    if (s.norm && h.dtype == NA1D_FP16) NA1D_HEAD_TRY(cudaMemsetAsync(sv.words, 0, sizeof(Words), st));   // (the largest inverse lengths; the rest the kernels set)
     NA1D_HEAD_TRY(prepare(h, s, sv, f.flags, loss, st));
     NA1D_HEAD_TRY(stats(h, s, sv, f.part, w, ldw, st));
     NA1D_HEAD_TRY(combine(h, s, sv, f.part, f.block_sums, loss, w, ldw, st));
@@ -232,6 +236,10 @@ int64_t na1d_head_backward_scratch(const na1d_head* head, int want_x, int want_w
     if (int s = na1d::head::check(head)) return s;
     const na1d::head::Shape s = na1d::head::shape_of(*head);
     return na1d::head::backward_at(*head, s, na1d::head::pieces_of(s, want_x != 0, want_weight != 0), want_x != 0, want_weight != 0, nullptr).bytes;
+}
+int na1d_head_weight_in_place(const na1d_head* head) {
+    if (int s = na1d::head::check(head)) return s;
+    return !na1d::head::shape_of(*head).copy_w;
 }
 int na1d_head_forward(const na1d_head* head, float* loss, void* saved, void* scratch, void* stream) {
     if (int s = na1d::head::check(head)) return s;

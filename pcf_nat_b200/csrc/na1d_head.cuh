@@ -58,6 +58,10 @@ constexpr float kSineFloor = 2e-7f;   // of the squared sine in the margin's for
 constexpr int kIgnored = -1, kBad = -2;
 constexpr int kNoClass = 0x7fffffff;  // behind a row's entries, which are sorted by class
 constexpr int kOwn = 4;               // rows of a class whose own gradients' roundings are made good
+// Normalised rows (and classes, where the weight is copied) are kept times a power of two that leaves them a length of 2^lift(..) to twice that. A cosine's
+// gradient carries both inverse lengths: so its range in fp16 is the same for every row and class, whatever the others' lengths are. 2^7 keeps elements of
+// 2^-21 of a row's length out of fp16's subnormals, and the longest elements far from its end.
+__host__ __device__ constexpr int lift(bool fp16) { return fp16 ? 7 : 0; }
 
 inline int64_t round_up(int64_t x, int64_t m) { return (x + m - 1) / m * m; }
 
@@ -65,7 +69,6 @@ inline int64_t round_up(int64_t x, int64_t m) { return (x + m - 1) / m * m; }
 struct Words {
     int counted;                // rows that count
     int ticket;                 // blocks of the combining kernel that are done
-    int most_ix, most_iw;       // largest inverse norms (their bits), for the range of fp16
 };
 
 // Pointers into `saved`. Rows that count are numbered c = 0 .. counted - 1 in their order.
@@ -78,8 +81,10 @@ struct Saved {
     float* slope;      // (Np) gradient of that class's logit: (p - 1) psi', or p - q
     int* own_count;    // (V rounded up) rows whose own class it is
     int* own;          // (V, kOwn) and the first of them to come
-    float* ix;         // (Np) 1 / |x| (normalised)
-    float* iw;         // (V rounded up) 1 / |w|
+    float* ix;         // (Np) 1 / |x| of the kept row (normalised)
+    float* iw;         // (V rounded up) 1 / |w|, of the kept class where there is a copy
+    float* x_up;       // (Np) the power of two that the kept row is x times
+    float* w_up;       // (V) of the kept class; null where the weight stays where it is
     float* q;          // (N, k) teacher's probabilities, sorted by class
     int* index;        // (N, k) classes in their order, kNoClass behind them
     float* entry;      // (N, k) the entry's logit as a power of two, then its gradient p - q
@@ -91,9 +96,9 @@ struct Saved {
 struct Shape {
     int64_t N, D, V, k, Np, Dp, parts;
     int64_t x_stride, w_stride;
-    bool norm, train_classes, copy_w;
+    bool norm, copy_w;
     float cs;                   // log2(e) scale / temperature: from a product (or cosine) to a power of two
-    int room;                   // 2^room times the largest gradient of a cosine's logit fits fp16
+    float up;                   // power of two that a 16-bit gradient of logits is multiplied with
 };
 
 Shape shape_of(const na1d_head& h);
@@ -119,14 +124,13 @@ struct FinishArgs {
     void *dx, *dw;
     const float *part_x, *part_w, *d_loss, *coef;
     const void *x, *w;
-    const float *ix, *iw, *slope;
+    const float *ix, *iw, *x_up, *w_up, *slope;
     const int *place, *target, *own_count, *own;
     const Words* words;
     long long Np, piece_rows, ldw;
     int N, D, Dp, cols, v0, splits_x, splits_w, x_type, w_type, reduction;
-    float factor;
-    int room;
-    bool fp16, norm;
+    float factor, up;
+    bool norm;
     bool own_classes;           // part_w has the sums of classes that are rows' own, at such a row
 };
 FinishArgs finish_args(const na1d_head& h, const Shape& s, const Saved& sv, void* dx, void* dw, const float* part_x, const float* part_w, const float* d_loss,
@@ -142,19 +146,6 @@ cudaError_t products(const na1d_head& h, const Shape& s, const Saved& sv, const 
                      float* part_w, const FinishArgs& f, const void* w, int64_t ldw, cudaStream_t st);
 int logits_read_status();
 int grad_read_status();
-
-// power of two that a 16-bit gradient of logits is multiplied with. bf16: none. fp16 holds 6e-5 to 65504 in full: probabilities times 2^14;
-// normalised ones also carry the inverse norms, at most `most`, and the margin's slope, which `room` leaves space for.
-__device__ __forceinline__ float gradient_scale(const Words* w, bool fp16, bool norm, int room) {
-    if (!fp16) return 1.f;
-    if (!norm) return 16384.f;
-    const float most = __int_as_float(w->most_ix) * __int_as_float(w->most_iw);
-    if (!(most > 0.f) || most > 1e30f) return 1.f;
-    int e;
-    frexpf(most, &e);
-    e = room - e;
-    return ldexpf(1.f, e < -100 ? -100 : e > 100 ? 100 : e);
-}
 
 // The gradient of a row's own class as it is rounded to 16 bits, in one order of operations: `out` = row_factor(..)
 __device__ __forceinline__ float row_factor(float up, float ix, float coef, bool norm) { return norm ? up * ix * coef : up * coef; }
@@ -173,15 +164,15 @@ __device__ __forceinline__ void store_any(void* p, int type, long long i, float 
 }
 // What rounding took from the gradient of row c's own class (the largest of the row, mostly): it is made good in fp32
 template <typename E>
-__device__ __forceinline__ float own_rest(const FinishArgs& a, int c, float up) {
+__device__ __forceinline__ float own_rest(const FinishArgs& a, int c) {
     const int v = a.target[c];
-    const float f = own_gradient(a.slope[c], row_factor(up, a.norm ? a.ix[c] : 1.f, a.coef ? a.coef[c] : 1.f, a.norm), a.norm ? a.iw[v] : 1.f, a.norm);
+    const float f = own_gradient(a.slope[c], row_factor(a.up, a.norm ? a.ix[c] : 1.f, a.coef ? a.coef[c] : 1.f, a.norm), a.norm ? a.iw[v] : 1.f, a.norm);
     const float rest = f - (float)E(f);
     return fabsf(rest) < INFINITY ? rest : 0.f;
 }
 // what both gradients are multiplied with
-__device__ __forceinline__ float common_factor(const FinishArgs& a, int counted, float up) {
-    const float f = a.factor / up;
+__device__ __forceinline__ float common_factor(const FinishArgs& a, int counted) {
+    const float f = a.factor / a.up;
     return a.reduction == NA1D_HEAD_NONE ? f * a.coef[a.Np] : f * (a.d_loss[0] / (a.reduction == NA1D_HEAD_MEAN ? (float)max(counted, 1) : 1.f));
 }
 

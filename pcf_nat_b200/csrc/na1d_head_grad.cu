@@ -250,7 +250,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) grad_ke
         const int q = warp & 3, h = (warp - 4) >> 2;   // tensor-memory lanes 32 q .. + 31 (those a warp reaches); columns 16 h, 16 h + 64, ..
         const uint32_t lanes = (uint32_t)(q * 32) << 16;
         const int counted = g.words->counted, row = q * 32 + lane;
-        const float factor = g.direct ? common_factor(g.f, counted, gradient_scale(g.words, g.f.fp16, g.f.norm, g.f.room)) : 1.f;
+        const float factor = g.direct ? common_factor(g.f, counted) : 1.f;
         const uint8_t* own_row = own_rows + row * 128;
         int it = 0, projected = 0;
         while (next_item(g, p, walk, pairs, t)) {
@@ -260,13 +260,16 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) grad_ke
             const bool live = r < (t.rows ? counted : g.cols), direct = g.direct && !t.rows;
             float* dst = t.rows ? g.part_x + (size_t)t.split * g.Np * g.Dq + (size_t)r * g.Dq : g.part_w + (size_t)t.split * g.piece_rows * g.Dq + (size_t)r * g.Dq;
             bool whole = !direct;                      // an fp32 sum at dst
-            float iw = 0.f;
+            float iw = 0.f, back = 1.f;
             if (direct && live) {
                 // a class that is some rows' own (and not that of many, whose roundings average out) gets what rounding took in the last step
                 const int count = g.f.own_count[v];
                 whole = count > 0 && count <= kOwn;
                 if (whole) dst = g.part_w + (size_t)g.f.own[(size_t)v * kOwn] * g.Dq;
-                if (PROJECT) iw = g.f.iw[v];
+                if (PROJECT) {
+                    iw = g.f.iw[v];
+                    if (g.f.w_up) back = g.f.w_up[v];
+                }
             }
             if (!empty) {
                 if (!ptx::mbar_wait_relaxed(&bar.acc_full[it & 1], (it >> 1) & 1) || *abort_flag) { atomicExch(&g_head_status, 4); *abort_flag = 1; break; }
@@ -329,7 +332,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) grad_ke
                         for (int j = 0; j < 16; ++j) d[j] = fmaf(-along, e[j], d[j]);
                     }
 #pragma unroll
-                    for (int j = 0; j < 16; ++j) d[j] *= factor;
+                    for (int j = 0; j < 16; ++j) d[j] = PROJECT ? d[j] * factor * back : d[j] * factor;
                     store_columns<E>(g.f, v, col, d);
                 }
             }

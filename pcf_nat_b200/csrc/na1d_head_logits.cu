@@ -53,9 +53,7 @@ struct Args {
     long long pitch;
     int parts;
     int V, v0, tiles, k, steps, tail;   // first class and tiles of classes of this launch; stages of a tile, products of 16 channels in the last one
-    float cs;
-    int room;
-    bool fp16;
+    float cs, up;
 };
 
 __device__ __forceinline__ float exp2_fast(float x) {
@@ -185,7 +183,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) logits_
     } else {
         const int q = warp & 3, h = (warp - 2) >> 2;   // tensor-memory lanes 32 q .. + 31 (those a warp reaches), quarter h of the columns
         const uint32_t lanes = (uint32_t)(q * 32) << 16;
-        const float up = GRAD ? gradient_scale(g.words, g.fp16, NORM, g.room) : 1.f;
+        const float up = GRAD ? g.up : 1.f;
         uint8_t* out_rows = smem + kStages * kStageBytes + (warp - 2) * kOut;
         // what belongs to a tile's row: asked for while the tile before is worked on
         struct Row {
@@ -413,7 +411,7 @@ template <bool GRAD>
 cudaError_t start(const na1d_head& h, const Shape& s, const Saved& sv, Args a, const void* w, int64_t ldw, bool after, cudaStream_t st) {
     a.words = sv.words; a.row = sv.row; a.target = sv.target; a.index = sv.index; a.entry = sv.entry;
     a.ix = sv.ix; a.iw = sv.iw; a.lse2 = sv.lse2; a.slope = sv.slope;
-    a.parts = (int)s.parts; a.V = (int)s.V; a.k = (int)s.k; a.cs = s.cs; a.room = s.room; a.fp16 = h.dtype == NA1D_FP16;
+    a.parts = (int)s.parts; a.V = (int)s.V; a.k = (int)s.k; a.cs = s.cs; a.up = s.up;
     a.steps = (int)((s.D + kStep - 1) / kStep);
     a.tail = (int)((s.D - (int64_t)(a.steps - 1) * kStep + 15) / 16);
     // scaled cosines of at most +-48 powers of two: the smallest term is 2^-96 of the one that the scale stands for

@@ -25,6 +25,7 @@ __device__ __forceinline__ float exp2_fast(float x) {
     return y;
 }
 
+__device__ __forceinline__ float power_of_two(int e) { return __int_as_float((127 + e) << 23); }   // -126 <= e <= 127
 template <typename E> __device__ __forceinline__ float squares(const uint4& v, float ss) {
     float f[8];
     Cvt<E>::unpack(v, f);
@@ -32,38 +33,65 @@ template <typename E> __device__ __forceinline__ float squares(const uint4& v, f
     for (int k = 0; k < 8; ++k) ss = fmaf(f[k], f[k], ss);
     return ss;
 }
-__device__ __forceinline__ float inverse_of(float ss) {   // of a row whose squares the lanes have
+// Inverse length of a row whose squares the lanes have. `up`: 2^up times the row has a length of 2^lift to twice that, and `kept` is 1 / its length then
+struct Length {
+    float inverse, kept;
+    int up;
+};
+__device__ __forceinline__ Length length_of(float ss, int lift) {
     ss = warp_sum(ss);
-    return ss > 0.f ? rsqrtf(ss) : ss == 0.f ? 0.f : ss;   // (NaN stays)
+    Length l = {ss > 0.f ? rsqrtf(ss) : ss == 0.f ? 0.f : ss, 0.f, 0};   // (NaN stays)
+    l.kept = l.inverse;
+    if (l.inverse > 0.f) {
+        const int e = ((__float_as_int(l.inverse) >> 23) & 255) - 126;   // inverse = m 2^e, m from 1/2 to 1: the length is 2^-e to twice that
+        l.up = e + lift;
+        l.kept = l.inverse * power_of_two(-l.up);
+    }
+    return l;
 }
-// One row of D elements to 16 bits at dst (Dp of them, zeros behind D; null: not stored), returns 1 / its length (0 where that is 0).
+template <typename E> __device__ __forceinline__ uint4 times_power(const uint4& v, float p) {
+    float f[8];
+    Cvt<E>::unpack(v, f);
+#pragma unroll
+    for (int k = 0; k < 8; ++k) f[k] *= p;
+    return Cvt<E>::pack(f);
+}
+// One row of D elements to 16 bits at dst (Dp of them, zeros behind D; null: not stored), times a power of two where it is normalised.
 // wide: rows start on 16 bytes, D is a multiple of 8.
 template <typename E>
-__device__ __forceinline__ float copy_row(E* dst, const void* src, int type, long long at, int D, int Dp, bool wide, bool norm, int lane) {
-    float ss = 0.f;
+__device__ __forceinline__ Length copy_row(E* dst, const void* src, int type, long long at, int D, int Dp, bool wide, bool norm, int lift, int lane) {
     // eight elements to a lane at a time in every form, so that a row's length has the same bits in all of them
-    for (int j = lane; j < Dp / 8; j += 32) {
-        uint4 v;
-        if (wide && type != NA1D_FP32) {
-            v = __ldg(reinterpret_cast<const uint4*>(static_cast<const E*>(src) + at) + j);
+    auto piece = [&](int j) {
+        if (wide && type != NA1D_FP32) return __ldg(reinterpret_cast<const uint4*>(static_cast<const E*>(src) + at) + j);
+        float f[8];
+        if (wide) {
+            const float4* p = reinterpret_cast<const float4*>(static_cast<const float*>(src) + at) + 2 * j;
+            const float4 a = __ldg(p), b = __ldg(p + 1);
+            f[0] = a.x; f[1] = a.y; f[2] = a.z; f[3] = a.w; f[4] = b.x; f[5] = b.y; f[6] = b.z; f[7] = b.w;
         } else {
-            float f[8];
-            if (wide) {
-                const float4* p = reinterpret_cast<const float4*>(static_cast<const float*>(src) + at) + 2 * j;
-                const float4 a = __ldg(p), b = __ldg(p + 1);
-                f[0] = a.x; f[1] = a.y; f[2] = a.z; f[3] = a.w; f[4] = b.x; f[5] = b.y; f[6] = b.z; f[7] = b.w;
-            } else {
 #pragma unroll
-                for (int k = 0; k < 8; ++k) f[k] = 8 * j + k < D ? load_any(src, type, at + 8 * j + k) : 0.f;
-            }
-            v = Cvt<E>::pack(f);
+            for (int k = 0; k < 8; ++k) f[k] = 8 * j + k < D ? load_any(src, type, at + 8 * j + k) : 0.f;
         }
-        if (dst) reinterpret_cast<uint4*>(dst)[j] = v;
-        if (norm) ss = squares<E>(v, ss);
+        return Cvt<E>::pack(f);
+    };
+    const int n = Dp / 8;
+    if (!norm) {
+        for (int j = lane; j < n; j += 32) reinterpret_cast<uint4*>(dst)[j] = piece(j);
+        return Length{1.f, 1.f, 0};
     }
-    return norm ? inverse_of(ss) : 1.f;
+    float ss = 0.f;
+    uint4 last = make_uint4(0, 0, 0, 0);   // (all of a row of up to 256: it is loaded once)
+    for (int j = lane; j < n; j += 32) {
+        last = piece(j);
+        ss = squares<E>(last, ss);
+    }
+    const Length l = length_of(ss, lift);
+    if (dst) {
+        const float p = power_of_two(l.up);
+        for (int j = lane; j < n; j += 32) reinterpret_cast<uint4*>(dst)[j] = times_power<E>(n <= 32 ? last : piece(j), p);
+    }
+    return l;
 }
-template <typename E> __device__ __forceinline__ float inverse_length(const uint4& v, float ss) { return inverse_of(squares<E>(v, ss)); }
 
 // ---------------------------------------------------------------- a teacher's probabilities
 struct TeacherArgs {
@@ -127,11 +155,11 @@ struct PrepareArgs {
     float* loss;               // (N) zeros for rows that do not count; null where the loss is one number
     Words* words;
     int *place, *row, *target, *own_count;
-    float *ix, *iw;
+    float *ix, *iw, *x_up, *w_up;
     void *out, *w_out;         // w_out: null where the weight stays where it is
     long long x_stride, w_stride, ignore;
-    int N, Np, V, D, Dp, x_type, w_type, per_block, row_blocks;
-    bool wide, w_wide, norm, relative;   // relative: the largest inverse lengths are wanted
+    int N, Np, V, D, Dp, x_type, w_type, per_block, row_blocks, lift;
+    bool wide, w_wide, norm;
     TeacherArgs t;
     bool top;
 };
@@ -145,27 +173,16 @@ __device__ __forceinline__ bool row_counts(const PrepareArgs& a, int i) {
     }
     return false;
 }
-// the largest of a block's warps' values (the same in all lanes) into *word, as bits (one atomic a block, in whatever order)
-__device__ __forceinline__ void block_most(float most, int* word, float* most_s) {
-    if ((threadIdx.x & 31) == 0) most_s[threadIdx.x >> 5] = most;
-    __syncthreads();
-    if (threadIdx.x == 0) {
-        for (int w = 1; w < kWarps; ++w) most = fmaxf(most, most_s[w]);
-        if (most > 0.f) atomicMax(word, __float_as_int(most));
-    }
-}
 // Blocks below row_blocks take `per_block` rows each. Such a block counts the rows before its own itself: labels are few bytes, and no block waits for
 // another. The others take the weight: a copy in 16 bits where the products cannot read it as it is, and its rows' lengths.
 template <typename E>
 __global__ void __launch_bounds__(kThreads) prepare_kernel(const __grid_constant__ PrepareArgs a) {
     __shared__ int sums[kWarps], places[kThreads], base_s;
-    __shared__ float most_s[kWarps];
     extern __shared__ int classes_s[];
     wait_for_predecessor();
     if (blockIdx.x == 0 && threadIdx.x == 0) a.words->ticket = 0;
     for (int v = blockIdx.x * kThreads + threadIdx.x; v < a.V; v += gridDim.x * kThreads) a.own_count[v] = 0;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    float most = 0.f;
     if ((int)blockIdx.x >= a.row_blocks) {
         const int step = (gridDim.x - a.row_blocks) * kWarps;
         int v = (blockIdx.x - a.row_blocks) * kWarps + warp;
@@ -177,18 +194,18 @@ __global__ void __launch_bounds__(kThreads) prepare_kernel(const __grid_constant
                     r[i] = lane < a.D / 8 ? __ldg(reinterpret_cast<const uint4*>(static_cast<const E*>(a.w) + (v + i * step) * a.w_stride) + lane) : make_uint4(0, 0, 0, 0);
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    const float iw = inverse_length<E>(r[i], 0.f);
-                    if (lane == 0) a.iw[v + i * step] = iw;
-                    most = fmaxf(most, iw);
+                    const Length l = length_of(squares<E>(r[i], 0.f), 0);
+                    if (lane == 0) a.iw[v + i * step] = l.inverse;
                 }
             }
         }
         for (; v < a.V; v += step) {
-            const float iw = copy_row<E>(a.w_out ? static_cast<E*>(a.w_out) + (size_t)v * a.Dp : nullptr, a.w, a.w_type, v * a.w_stride, a.D, a.Dp, a.w_wide, a.norm, lane);
-            if (a.norm && lane == 0) a.iw[v] = iw;
-            most = fmaxf(most, iw);
+            const Length l = copy_row<E>(a.w_out ? static_cast<E*>(a.w_out) + (size_t)v * a.Dp : nullptr, a.w, a.w_type, v * a.w_stride, a.D, a.Dp, a.w_wide, a.norm, a.lift, lane);
+            if (a.norm && lane == 0) {
+                a.iw[v] = a.w_up ? l.kept : l.inverse;
+                if (a.w_up) a.w_up[v] = power_of_two(l.up);
+            }
         }
-        if (a.relative) block_most(most, &a.words->most_iw, most_s);
         return;
     }
     const int r0 = min(a.N, (int)blockIdx.x * a.per_block), r1 = min(a.N, r0 + a.per_block);
@@ -234,9 +251,11 @@ __global__ void __launch_bounds__(kThreads) prepare_kernel(const __grid_constant
         for (int j = warp; j < n; j += kWarps) {
             const int p = places[j];
             if (p >= 0) {
-                const float ix = copy_row<E>(out + (size_t)p * a.Dp, a.x, a.x_type, (c0 + j) * a.x_stride, a.D, a.Dp, a.wide, a.norm, lane);
-                if (a.norm && lane == 0) a.ix[p] = ix;
-                most = fmaxf(most, ix);
+                const Length l = copy_row<E>(out + (size_t)p * a.Dp, a.x, a.x_type, (c0 + j) * a.x_stride, a.D, a.Dp, a.wide, a.norm, a.lift, lane);
+                if (a.norm && lane == 0) {
+                    a.ix[p] = l.kept;
+                    a.x_up[p] = power_of_two(l.up);
+                }
                 if (a.top && !a.t.flags) teacher_row(a.t, c0 + j, classes_s + warp * a.t.k, lane);
             } else {
                 for (int e = lane; e < a.Dp / 8; e += 32) reinterpret_cast<uint4*>(out + (size_t)(-1 - p) * a.Dp)[e] = make_uint4(0, 0, 0, 0);
@@ -248,7 +267,6 @@ __global__ void __launch_bounds__(kThreads) prepare_kernel(const __grid_constant
     const long long pad = (long long)(a.Np - a.N) * (a.Dp / 8);   // 16-byte pieces behind the last row
     for (long long e = (long long)blockIdx.x * kThreads + threadIdx.x; e < pad; e += (long long)a.row_blocks * kThreads)
         reinterpret_cast<uint4*>(out + (size_t)a.N * a.Dp)[e] = make_uint4(0, 0, 0, 0);
-    if (a.relative) block_most(most, &a.words->most_ix, most_s);
     if (r0 < a.N && r1 == a.N && threadIdx.x == 0) a.words->counted = base;
 }
 
@@ -442,9 +460,9 @@ __global__ void __launch_bounds__(1024) coefficients_kernel(const float* __restr
 template <typename E>
 __device__ __forceinline__ void unpack_row(const E* row, int j, float* f) { Cvt<E>::unpack(__ldg(reinterpret_cast<const uint4*>(row) + j), f); }
 // One row of a gradient: the splits' sum and what rounding took (`n` rows of the other operand times `rest`: `other(i)`), without its part along the row it
-// belongs to where that is normalised, times the common factor.
+// belongs to where that is normalised, times the common factor and the power of two that the row is kept with.
 template <typename E, typename Other>
-__device__ __forceinline__ void finish_row(void* out, int type, long long at, const float* part, long long split, int splits, const E* own, float inverse, float f,
+__device__ __forceinline__ void finish_row(void* out, int type, long long at, const float* part, long long split, int splits, const E* own, float inverse, float f, float back,
                                            int n, const float* rest, Other other, bool norm, int D, int Dp, int lane) {
     auto sum = [&](int j, float* s) {
 #pragma unroll
@@ -492,7 +510,7 @@ __device__ __forceinline__ void finish_row(void* out, int type, long long at, co
             for (int e = 0; e < 8; ++e) s[e] = fmaf(-along, x[e], s[e]);
         }
 #pragma unroll
-        for (int e = 0; e < 8; ++e) s[e] *= f;
+        for (int e = 0; e < 8; ++e) s[e] = s[e] * f * back;
         if (wide) reinterpret_cast<uint4*>(static_cast<E*>(out) + at)[j] = Cvt<E>::pack(s);
         else
 #pragma unroll
@@ -504,7 +522,7 @@ template <typename E>
 __global__ void __launch_bounds__(kThreads, 3) finish_kernel(const __grid_constant__ FinishArgs a) {
     wait_for_predecessor();
     const int lane = threadIdx.x & 31, counted = a.words->counted, first = a.cols + (a.dx ? a.N : 0), n = first + (a.own_classes ? a.N : 0);
-    const float up = gradient_scale(a.words, a.fp16, a.norm, a.room), f = common_factor(a, counted, up);
+    const float f = common_factor(a, counted);
     const E *x = static_cast<const E*>(a.x), *w = static_cast<const E*>(a.w);
     auto class_row = [&](int v, const float* part, long long split, int splits) {
         float rest[kOwn];
@@ -519,10 +537,10 @@ __global__ void __launch_bounds__(kThreads, 3) finish_kernel(const __grid_consta
             for (int o = 0; o < kOwn; ++o) {
                 const unsigned who = __ballot_sync(0xffffffffu, lane < rows && rank == o);
                 rows_in_order[o] = __shfl_sync(0xffffffffu, mine, who ? __ffs(who) - 1 : 0);
-                rest[o] = o < rows ? own_rest<E>(a, rows_in_order[o], up) : 0.f;
+                rest[o] = o < rows ? own_rest<E>(a, rows_in_order[o]) : 0.f;
             }
         }
-        finish_row<E>(a.dw, a.w_type, (long long)v * a.D, part, split, splits, w + (size_t)v * a.ldw, a.norm ? a.iw[v] : 1.f, f, rows, rest,
+        finish_row<E>(a.dw, a.w_type, (long long)v * a.D, part, split, splits, w + (size_t)v * a.ldw, a.norm ? a.iw[v] : 1.f, f, a.w_up ? a.w_up[v] : 1.f, rows, rest,
                       [&](int o) { return x + (size_t)rows_in_order[o] * a.Dp; }, a.norm, a.D, a.Dp, lane);
     };
     for (int i = blockIdx.x * kWarps + (threadIdx.x >> 5); i < n; i += gridDim.x * kWarps) {
@@ -541,9 +559,9 @@ __global__ void __launch_bounds__(kThreads, 3) finish_kernel(const __grid_consta
             continue;
         }
         const int v = a.target[c];
-        const float rest[kOwn] = {v >= 0 ? own_rest<E>(a, c, up) : 0.f};
+        const float rest[kOwn] = {v >= 0 ? own_rest<E>(a, c) : 0.f};
         finish_row<E>(a.dx, a.x_type, (long long)r * a.D, a.part_x + (size_t)c * a.Dp, a.Np * a.Dp, a.splits_x, x + (size_t)c * a.Dp, a.norm ? a.ix[c] : 1.f, f,
-                      v >= 0 ? 1 : 0, rest, [&](int) { return w + (size_t)v * a.ldw; }, a.norm, a.D, a.Dp, lane);
+                      a.norm ? a.x_up[c] : 1.f, v >= 0 ? 1 : 0, rest, [&](int) { return w + (size_t)v * a.ldw; }, a.norm, a.D, a.Dp, lane);
     }
 }
 
@@ -567,11 +585,11 @@ cudaError_t prepare(const na1d_head& h, const Shape& s, const Saved& sv, int* fl
     PrepareArgs a = {};
     a.x = h.x; a.w = h.weight; a.labels = h.labels; a.top = s.k > 0;
     a.loss = h.reduction == NA1D_HEAD_NONE ? loss : nullptr;
-    a.words = sv.words; a.place = sv.place; a.row = sv.row; a.target = sv.target; a.own_count = sv.own_count; a.ix = sv.ix; a.iw = sv.iw;
+    a.words = sv.words; a.place = sv.place; a.row = sv.row; a.target = sv.target; a.own_count = sv.own_count; a.ix = sv.ix; a.iw = sv.iw; a.x_up = sv.x_up; a.w_up = sv.w_up;
     a.out = sv.x; a.w_out = s.copy_w ? sv.w : nullptr;
     a.x_stride = h.x_stride; a.w_stride = h.weight_stride; a.ignore = h.ignore_index;
     a.N = (int)s.N; a.Np = (int)s.Np; a.V = (int)s.V; a.D = (int)s.D; a.Dp = (int)s.Dp; a.x_type = h.x_type; a.w_type = h.weight_type;
-    a.norm = s.norm; a.relative = s.norm && h.dtype == NA1D_FP16;
+    a.norm = s.norm; a.lift = lift(h.dtype == NA1D_FP16);
     a.wide = whole_pieces(h.x, h.x_stride, s.D);
     a.w_wide = whole_pieces(h.weight, h.weight_stride, s.D);
     a.per_block = (int)round_up((s.N + 295) / 296, kWarps);
@@ -611,11 +629,11 @@ FinishArgs finish_args(const na1d_head& h, const Shape& s, const Saved& sv, void
                        const float* coef, const Pieces& p, int64_t v0, int64_t cols, const void* w, int64_t ldw) {
     FinishArgs a = {};
     a.dx = dx; a.dw = dw; a.part_x = part_x; a.part_w = part_w; a.d_loss = d_loss; a.coef = coef;
-    a.x = sv.x; a.w = w; a.ix = sv.ix; a.iw = sv.iw; a.place = sv.place; a.words = sv.words;
+    a.x = sv.x; a.w = w; a.ix = sv.ix; a.iw = sv.iw; a.x_up = sv.x_up; a.w_up = sv.w_up; a.place = sv.place; a.words = sv.words;
     a.slope = sv.slope; a.target = sv.target; a.own_count = sv.own_count; a.own = sv.own;
     a.Np = s.Np; a.piece_rows = p.pitch; a.ldw = ldw;
     a.N = (int)s.N; a.D = (int)s.D; a.Dp = (int)s.Dp; a.cols = (int)cols; a.v0 = (int)v0; a.splits_x = p.splits_x; a.splits_w = p.splits_w;
-    a.x_type = h.x_type; a.w_type = h.weight_type; a.reduction = h.reduction; a.norm = s.norm; a.fp16 = h.dtype == NA1D_FP16; a.room = s.room;
+    a.x_type = h.x_type; a.w_type = h.weight_type; a.reduction = h.reduction; a.norm = s.norm; a.up = s.up;
     a.factor = s.k ? h.scale * h.temperature : h.scale;
     return a;
 }

@@ -1120,9 +1120,7 @@ struct HeadForward {
     }
 };
 // whether the forward pass reads the weight where it is: then the backward pass does so too, else it has a copy of its own
-bool head_in_place(const na1d_head& h) {
-    return h.weight_type == h.dtype && h.dim % 8 == 0 && h.weight_stride % 8 == 0 && h.weight_stride >= h.dim && (reinterpret_cast<uintptr_t>(h.weight) & 15) == 0;
-}
+bool head_in_place(const na1d_head& h) { return head_bytes(na1d_head_weight_in_place(&h), "na1d_head_weight_in_place") != 0; }
 
 struct NA1dHead : public torch::autograd::Function<NA1dHead> {
     static Tensor forward(AutogradContext* ctx, const Tensor& x, const Tensor& w, const OptTensor& labels, const OptTensor& logits, const OptTensor& index, int64_t x_stride,

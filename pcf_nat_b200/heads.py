@@ -56,6 +56,12 @@ def _forward(cfg, x, weight, labels, teacher_logits, teacher_index):
     return loss, saved, head
 
 
+def _in_place(head, weight):
+    """Makes `weight` the head's: whether the kernels read it there (`saved` has no copy of it)."""
+    head.weight, head.weight_stride = weight.data_ptr(), weight.stride(0)
+    return bool(_bytes(_L.na1d_head_weight_in_place(ctypes.byref(head)), "na1d_head_weight_in_place"))
+
+
 class _HeadFunction(torch.autograd.Function):
     """The route of calls that the C++ node (csrc/torch_nodes.cpp) leaves to Python."""
 
@@ -63,7 +69,7 @@ class _HeadFunction(torch.autograd.Function):
     def forward(ctx, x, weight, labels, teacher_logits, teacher_index, cfg):
         loss, saved, head = _forward(cfg, x, weight, labels, teacher_logits, teacher_index)
         # the weight is read again where it is, unless the forward pass made a copy of its own (then the copy is in `saved`)
-        ctx.in_place = weight.dtype != torch.float32 and weight.shape[1] % 8 == 0 and weight.stride(0) % 8 == 0 and weight.stride(0) >= weight.shape[1] and weight.data_ptr() % 16 == 0
+        ctx.in_place = _in_place(head, weight)
         ctx.save_for_backward(saved, weight if ctx.in_place else None)
         ctx.head, ctx.x_dtype, ctx.w_dtype = head, x.dtype, weight.dtype
         ctx.set_materialize_grads(False)
@@ -83,9 +89,10 @@ class _HeadFunction(torch.autograd.Function):
                 saved = saved.clone()
             head.x = head.labels = head.teacher_logits = head.teacher_index = saved.data_ptr()   # not read any more
             if ctx.in_place:
-                if weight.stride(1) != 1 or weight.stride(0) % 8 or weight.stride(0) < weight.shape[1] or weight.data_ptr() % 16:
+                if weight.stride(1) != 1 or not _in_place(head, weight):
                     weight = weight.clone(memory_format=torch.contiguous_format)
-                head.weight, head.weight_stride = weight.data_ptr(), weight.stride(0)
+                    if not _in_place(head, weight):
+                        raise RuntimeError("a head's weight came back from a saved-tensor hook in a form that it did not have")
             ref = ctypes.byref(head)
             d_loss = d_loss.to(torch.float32).contiguous()
             dx = torch.empty((head.rows, head.dim), dtype=ctx.x_dtype, device=dev) if want_x else None

@@ -45,3 +45,73 @@ def test_wide_margins_at_a_sine_of_zero(dtype, sign, margin):
         # (each gradient of a logit rounded once, up to 20 times the row's length; the result once more)
         parts = 20.0 / own.detach().double().norm(dim=1) * u * (1 if own is x else 16)
         assert bool((err <= size + parts + u * scale).all())
+
+
+def _cosine_problem(op, N, D, V, seed):
+    """Values that stay exact in both types when they are multiplied with powers of two down to 2^-8."""
+    g = torch.Generator(device=DEV).manual_seed(seed)
+    w = torch.randint(-31, 32, (V, D), device=DEV, generator=g) / 16.0
+    y = torch.randint(0, V // 2, (N,), device=DEV, generator=g)     # (the second half of the classes is no row's own)
+    x = torch.randint(-15, 16, (N, D), device=DEV, generator=g) / 16.0 + w[y]
+    t, i = torch.randn(N, 4, device=DEV, generator=g), (y[:, None] + torch.arange(4, device=DEV) * 7) % (V // 2)
+    return x, w, y, t, i
+
+
+def _cosine_loss(op, x, w, y, t, i, reduction="sum"):
+    if op == "angular":
+        return b200.angular_cross_entropy(x, w, y, margin=0.2, scale=30.0, reduction=reduction)
+    return b200.linear_distillation(x, w, t, i, scale=30.0, normalize=True, reduction=reduction)
+
+
+@pytest.mark.parametrize("op", ["angular", "distill"])
+@pytest.mark.parametrize("row,cls", [(1e-5, 1.0), (1.0, 1e-5), (1e-3, 1e-3), (1e-4, 1e-4), (30.0, 1e-4)])
+def test_one_length_far_from_the_others_in_fp16(op, row, cls):
+    """A short row or class costs the others' gradients nothing. Each row's and each class's own error, against what rounding allows whatever the others' lengths are: half a
+    step of fp16 (and the logits' fp32 errors) of each gradient of a logit, or half a subnormal step: 2^-25 / 2^5 of a probability."""
+    N, D, V = 40, 32, 6000
+    x, w, y, t, i = _cosine_problem(op, N, D, V, 1)
+    x[3] *= row
+    w[17] *= cls
+    w[V - 5] *= cls
+    x, w = x.half().float().requires_grad_(), w.half().float().requires_grad_()
+    with torch.autocast("cuda", dtype=torch.float16):
+        _cosine_loss(op, x, w, y, t, i).backward()
+    ops.device_status()
+    kw = dict(labels=y, margin=0.2) if op == "angular" else dict(teacher_logits=t, teacher_index=i)
+    r = orc.evaluate(x.detach().half(), w.detach().half(), scale=30.0, normalize=True, reduction="sum", **kw)
+    z, _, ix, iw, slope = orc.logits(x.detach(), w.detach(), 30.0, True, kw.get("labels"), kw.get("margin", 0.0))
+    h = torch.softmax(z, 1)
+    if op == "angular":
+        h.scatter_(1, y[:, None], (h.gather(1, y[:, None]) - 1) * slope[:, None])
+    else:
+        h.scatter_add_(1, i, -orc.teacher_probabilities(t, i, 1.0)[0])
+    relative = 2.0 ** -11 + 4 * 30 * (D + 8) * 2.0 ** -23
+    for got, ref, inverse, sums, terms in ((x.grad, r["dx"], ix, h.abs().sum(1), V), (w.grad, r["dw"], iw, h.abs().sum(0), N)):
+        off = 30 * inverse * (sums * (relative + (terms + D + 16) * 2.0 ** -23) + terms * 2.0 ** -30)
+        err = (got.double() - ref).norm(dim=1)
+        assert bool((err <= off).all()), float((err / off).max())
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("copy", [False, True])
+@pytest.mark.parametrize("op", ["angular", "distill"])
+def test_powers_of_two_of_single_rows_change_no_bits(op, copy, dtype):
+    """Cosines do not know a row's length, nor do the other rows' gradients: the same bits, its own gradient times the inverse power."""
+    N, D, V = 60, 64, 3000
+    x, w, y, t, i = _cosine_problem(op, N, D, V, 2)
+    a, b = torch.ones(N, 1, device=DEV), torch.ones(V, 1, device=DEV)
+    a[5], a[6], b[9], b[V - 2] = 2.0 ** -8, 2.0 ** 4, 2.0 ** -7, 2.0 ** 5
+    got = []
+    for p, q in ((torch.ones_like(a), torch.ones_like(b)), (a, b)):
+        u, v = (x * p).to(dtype), (w * q).to(dtype if not copy else torch.float32)
+        assert torch.equal(u.float(), x * p) and torch.equal(v.float(), w * q)
+        u, v = u.requires_grad_(), v.requires_grad_()
+        loss = _cosine_loss(op, u, v, y, t, i, "none")
+        gu, gv = torch.autograd.grad((loss * 2.0 ** -9).sum(), (u, v))    # (no gradient leaves fp16's range)
+        got.append((loss.detach(), gu.float() * p, gv.float() * q))
+    same = [torch.equal(s, r) for s, r in zip(*got)]
+    if dtype == torch.float16:            # (results below 2^-14 have fewer bits)
+        off = 2.0 ** -24 * torch.maximum(p, torch.ones_like(p)), 2.0 ** -24 * torch.maximum(q, torch.ones_like(q))
+        near = [bool(((s - r).abs() <= o).all()) for s, r, o in zip(got[0][1:], got[1][1:], off)]
+        same[1:] = [s or n for s, n in zip(same[1:], near)]
+    assert same == [True] * 3

@@ -141,3 +141,18 @@ def test_forward_mode_is_refused(op, dual, requires_grad):
     args = [x, w, t]
     with pytest.raises(NotImplementedError, match="forward-mode"):
         torch.func.jvp(lambda a: f(*(a if j == n else b for j, b in enumerate(args))), (args[n].detach(),), (torch.ones_like(args[n]),))
+
+
+@pytest.mark.parametrize("more,in_place", [
+    (dict(), 1), (dict(weight_stride=24), 1), (dict(dtype=1, x_type=1, weight_type=1), 1), (dict(normalize=1), 1),
+    (dict(dtype=1, x_type=1, weight_type=1, normalize=1), 0),         # (fp16 cosines: classes times powers of two)
+    (dict(weight_type=2), 0), (dict(dim=15), 0), (dict(weight_stride=20), 0), (dict(weight_stride=8), 0), (dict(weight=P + 2), 0),
+    (dict(classes=1, weight_stride=19), 0), (dict(scale=0.0), -13),
+])
+def test_where_the_weight_is_read(more, in_place):
+    """The nodes keep the weight itself or rely on the copy in `saved` by this answer; the copy is what makes `saved` larger."""
+    h = _head(**more)
+    assert L.na1d_head_weight_in_place(ctypes.byref(h)) == in_place
+    if in_place >= 0:
+        dense = _head(**{**more, "weight": P, "weight_stride": 16, "weight_type": more.get("dtype", 0), "dim": 16, "dtype": 0, "x_type": 0, "weight_type": 0})
+        assert (L.na1d_head_saved_bytes(ctypes.byref(h)) > L.na1d_head_saved_bytes(ctypes.byref(dense))) == (in_place == 0)
