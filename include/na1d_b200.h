@@ -311,7 +311,7 @@ int na1d_stats_pool_backward(void* d_logits, void* dx, const float* d_out, const
  *              z / temperature; loss_i = temperature^2 sum_j q_j (log q_j - log p_(index j)). Rows without an entry (or with nothing but
  *              logits of -infinity) do not count. A class may come twice.
  * A label or entry that is no class makes its row's loss, and what depends on it, NaN; nothing is read outside the tensors. A row or class
- * of zeros has no direction: its cosines are 0 and its gradient is. The mean is over rows that count, and 0 where none does.
+ * of zeros (or shorter than 2^-126) has no direction: its cosines are 0 and its gradient is. One with an infinity is NaN. The mean is over rows that count, and 0 where none does.
  *
  * Products are of 16-bit values (dtype) with sums in fp32; fp32 rows or weights are rounded to dtype first, and their gradients are fp32. The
  * gradient of the logits is rounded to dtype once, before its products with weight and rows; everything else is held in fp32. No atomics

@@ -306,7 +306,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) grad_ke
                 if (lane == 0) ptx::mbar_arrive(&bar.along);
                 if (!ptx::mbar_wait(&bar.along, projected & 1) || *abort_flag) { atomicExch(&g_head_status, 7); *abort_flag = 1; break; }
                 const float(*sums)[kHalf] = along_s[projected & 1];
-                along = ((sums[0][row] + sums[1][row]) + (sums[2][row] + sums[3][row])) * iw * iw;
+                along = ((sums[0][row] + sums[1][row]) + (sums[2][row] + sums[3][row])) * iw;
             }
 #pragma unroll 1
             for (int n = 16 * h; n < g.d_width; n += 64) {
@@ -329,7 +329,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) grad_ke
                         float e[16];
                         own_columns(n, e);
 #pragma unroll
-                        for (int j = 0; j < 16; ++j) d[j] = fmaf(-along, e[j], d[j]);
+                        for (int j = 0; j < 16; ++j) d[j] = fmaf(-along, e[j] * iw, d[j]);
                     }
 #pragma unroll
                     for (int j = 0; j < 16; ++j) d[j] = PROJECT ? d[j] * factor * back : d[j] * factor;

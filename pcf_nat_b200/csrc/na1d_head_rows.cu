@@ -38,22 +38,47 @@ struct Length {
     float inverse, kept;
     int up;
 };
-__device__ __forceinline__ Length length_of(float ss, int lift) {
+// Squares outside fp32's range, or nearly: taken again of the row (`n` pieces) against its largest element. Rows of zeros, and ones shorter than 2^-126: all 0;
+// a row with an infinity or NaN has no length: NaN.
+template <typename E, typename Piece>
+__device__ __forceinline__ Length length_of(float ss, int lift, int n, Piece piece, int lane) {
     ss = warp_sum(ss);
-    Length l = {ss > 0.f ? rsqrtf(ss) : ss == 0.f ? 0.f : ss, 0.f, 0};   // (NaN stays)
-    l.kept = l.inverse;
-    if (l.inverse > 0.f) {
-        const int e = ((__float_as_int(l.inverse) >> 23) & 255) - 126;   // inverse = m 2^e, m from 1/2 to 1: the length is 2^-e to twice that
-        l.up = e + lift;
-        l.kept = l.inverse * power_of_two(-l.up);
+    float inverse;
+    int less = 0;   // `inverse` is of the row times 2^-less
+    if (ss >= 0x1p-100f && ss <= 0x1p100f) {
+        inverse = rsqrtf(ss);
+    } else {
+        float f[8], most = 0.f, again = 0.f;
+        for (int j = lane; j < n; j += 32) {
+            Cvt<E>::unpack(piece(j), f);
+#pragma unroll
+            for (int k = 0; k < 8; ++k) most = fmaxf(most, fabsf(f[k]));
+        }
+        most = warp_max(most);
+        if (ss != ss || most == INFINITY) return Length{NAN, NAN, 0};
+        if (most == 0.f) return Length{0.f, 0.f, 0};
+        frexpf(most, &less);
+        for (int j = lane; j < n; j += 32) {
+            Cvt<E>::unpack(piece(j), f);
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+                const float g = ldexpf(f[k], -less);
+                again = fmaf(g, g, again);
+            }
+        }
+        inverse = rsqrtf(warp_sum(again));
     }
-    return l;
+    const int e = ((__float_as_int(inverse) >> 23) & 255) - 126;   // inverse = m 2^e, m from 1/2 to 1: the length is 2^-e to twice that
+    if (e - less > 126) return Length{0.f, 0.f, 0};
+    return Length{less ? ldexpf(inverse, -less) : inverse, inverse * power_of_two(-e - lift), e - less + lift};
 }
-template <typename E> __device__ __forceinline__ uint4 times_power(const uint4& v, float p) {
+// eight elements times 2^l.up (in two steps: it may be beyond fp32); zeros, or NaN, where the row has no direction
+template <typename E> __device__ __forceinline__ uint4 kept_piece(const uint4& v, const Length& l) {
+    const float p = power_of_two(l.up / 2), q = l.kept > 0.f ? power_of_two(l.up - l.up / 2) : l.kept;
     float f[8];
     Cvt<E>::unpack(v, f);
 #pragma unroll
-    for (int k = 0; k < 8; ++k) f[k] *= p;
+    for (int k = 0; k < 8; ++k) f[k] = f[k] * p * q;
     return Cvt<E>::pack(f);
 }
 // One row of D elements to 16 bits at dst (Dp of them, zeros behind D; null: not stored), times a power of two where it is normalised.
@@ -85,11 +110,9 @@ __device__ __forceinline__ Length copy_row(E* dst, const void* src, int type, lo
         last = piece(j);
         ss = squares<E>(last, ss);
     }
-    const Length l = length_of(ss, lift);
-    if (dst) {
-        const float p = power_of_two(l.up);
-        for (int j = lane; j < n; j += 32) reinterpret_cast<uint4*>(dst)[j] = times_power<E>(n <= 32 ? last : piece(j), p);
-    }
+    const Length l = length_of<E>(ss, lift, n, piece, lane);
+    if (dst)
+        for (int j = lane; j < n; j += 32) reinterpret_cast<uint4*>(dst)[j] = kept_piece<E>(n <= 32 ? last : piece(j), l);
     return l;
 }
 
@@ -194,7 +217,7 @@ __global__ void __launch_bounds__(kThreads) prepare_kernel(const __grid_constant
                     r[i] = lane < a.D / 8 ? __ldg(reinterpret_cast<const uint4*>(static_cast<const E*>(a.w) + (v + i * step) * a.w_stride) + lane) : make_uint4(0, 0, 0, 0);
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    const Length l = length_of(squares<E>(r[i], 0.f), 0);
+                    const Length l = length_of<E>(squares<E>(r[i], 0.f), 0, a.D / 8, [&](int) { return r[i]; }, lane);
                     if (lane == 0) a.iw[v + i * step] = l.inverse;
                 }
             }
@@ -203,7 +226,7 @@ __global__ void __launch_bounds__(kThreads) prepare_kernel(const __grid_constant
             const Length l = copy_row<E>(a.w_out ? static_cast<E*>(a.w_out) + (size_t)v * a.Dp : nullptr, a.w, a.w_type, v * a.w_stride, a.D, a.Dp, a.w_wide, a.norm, a.lift, lane);
             if (a.norm && lane == 0) {
                 a.iw[v] = a.w_up ? l.kept : l.inverse;
-                if (a.w_up) a.w_up[v] = power_of_two(l.up);
+                if (a.w_up) a.w_up[v] = ldexpf(1.f, l.up);
             }
         }
         return;
@@ -254,7 +277,7 @@ __global__ void __launch_bounds__(kThreads) prepare_kernel(const __grid_constant
                 const Length l = copy_row<E>(out + (size_t)p * a.Dp, a.x, a.x_type, (c0 + j) * a.x_stride, a.D, a.Dp, a.wide, a.norm, a.lift, lane);
                 if (a.norm && lane == 0) {
                     a.ix[p] = l.kept;
-                    a.x_up[p] = power_of_two(l.up);
+                    a.x_up[p] = ldexpf(1.f, l.up);
                 }
                 if (a.top && !a.t.flags) teacher_row(a.t, c0 + j, classes_s + warp * a.t.k, lane);
             } else {
@@ -492,7 +515,7 @@ __device__ __forceinline__ void finish_row(void* out, int type, long long at, co
 #pragma unroll
             for (int e = 0; e < 8; ++e) along = fmaf(x[e], 8 * j + e < D ? s[e] : 0.f, along);
         }
-        along = warp_sum(along) * inverse * inverse;
+        along = warp_sum(along) * inverse;   // (a length of 1e-20 has no square in fp32)
     }
     const bool wide = D % 8 == 0 && type != NA1D_FP32;
     for (int j = lane; j < Dp / 8; j += 32) {
@@ -507,7 +530,7 @@ __device__ __forceinline__ void finish_row(void* out, int type, long long at, co
             float x[8];
             unpack_row(own, j, x);
 #pragma unroll
-            for (int e = 0; e < 8; ++e) s[e] = fmaf(-along, x[e], s[e]);
+            for (int e = 0; e < 8; ++e) s[e] = fmaf(-along, x[e] * inverse, s[e]);
         }
 #pragma unroll
         for (int e = 0; e < 8; ++e) s[e] = s[e] * f * back;

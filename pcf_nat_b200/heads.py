@@ -202,8 +202,9 @@ def linear_cross_entropy(x, weight, labels, *, scale=1.0, ignore_index=-100, red
 
 def angular_cross_entropy(x, weight, labels, *, margin=0.2, scale=30.0, ignore_index=-100, reduction="mean"):
     """AAM-softmax: cross entropy of ``scale`` times the cosines of rows and classes, the label's angle widened by ``margin`` radians
-    (``model.AAMSoftmax``; cos(a + m) as cos a cos m - sin a sin m, the squared sine at least 2e-7). A row or class of zeros has cosine 0 with
-    all others and no gradient. Otherwise as ``linear_cross_entropy``."""
+    (``model.AAMSoftmax``; cos(a + m) as cos a cos m - sin a sin m, the squared sine at least 2e-7). A row or class of zeros (or shorter than
+    2^-126) has cosine 0 with all others and no gradient; one with an infinity is NaN. Where the weight is read in its place (16-bit, dense), a probability
+    over its class's length below 2^-126 reaches the gradients with fewer digits. Otherwise as ``linear_cross_entropy``."""
     _numbers(margin=margin, scale=scale, ignore_index=ignore_index)
     loss = None
     if _tensors(x, weight, labels):

@@ -115,3 +115,59 @@ def test_powers_of_two_of_single_rows_change_no_bits(op, copy, dtype):
         near = [bool(((s - r).abs() <= o).all()) for s, r, o in zip(got[0][1:], got[1][1:], off)]
         same[1:] = [s or n for s, n in zip(same[1:], near)]
     assert same == [True] * 3
+
+
+@pytest.mark.parametrize("copy", [False, True])
+@pytest.mark.parametrize("D", [64, 57, 320])
+@pytest.mark.parametrize("op", ["angular", "distill"])
+def test_lengths_whose_squares_leave_fp32(op, D, copy):
+    """bfloat16 rows and classes of 1e-27 to 1e27: as above, no bit changes but the powers of two and what falls into subnormals, which have a step of 2^-133 in bfloat16
+    and 2^-149 in fp32. A gradient there is off by half a step, times the power that is taken out of it here. With the weight in its place a gradient of a logit is
+    divided by the class's own length: half a step of 2^-133 of each, 30 times as large in the result, reaches dx times the class's elements (up to 2) and dw times the
+    N kept rows' (up to 2). The projection at most adds sqrt(D) times that, and results that differ at all may be rounded apart, half a step each."""
+    N, V = 60, 500
+    x, w, y, t, i = _cosine_problem(op, N, D, V, 3)
+    a, b = torch.ones(N, 1, device=DEV), torch.ones(V, 1, device=DEV)
+    a[5], a[6], a[7], a[8] = 2.0 ** -90, 2.0 ** 90, 2.0 ** -64, 2.0 ** 66
+    b[9], b[V - 2], b[11], b[V - 4] = 2.0 ** -90, 2.0 ** 90, 2.0 ** 70, 2.0 ** -62
+    b[y[20]], b[y[21]] = 2.0 ** -90, 2.0 ** 88
+    got = []
+    for p, q in ((torch.ones_like(a), torch.ones_like(b)), (a, b)):
+        u, v = (x * p).bfloat16().requires_grad_(), (w * q).to(torch.float32 if copy else torch.bfloat16).requires_grad_()
+        loss = _cosine_loss(op, u, v, y, t, i, "none")
+        gu, gv = torch.autograd.grad(loss.sum(), (u, v))
+        got.append((loss.detach(), gu.float() * p, gv.float() * q))
+    ops.device_status()
+    assert torch.equal(got[0][0], got[1][0])
+    for s, r, power, out, products in ((got[0][1], got[1][1], a, u.dtype, 2 * b[b > 1].sum()), (got[0][2], got[1][2], b, v.dtype, 2 * N * b * (b > 1))):
+        f, power, products = torch.finfo(out), power.double(), products.double()
+        off = f.tiny * f.eps / 2 * power + 2.0 ** -150 * power
+        if not copy:
+            moved = 30 * 2.0 ** -134 * products * (1 + D ** 0.5)
+            off = off + moved + torch.where(moved > 0, f.eps * (s.abs() + moved), 0.0)
+        assert bool(torch.isfinite(r).all()) and bool(((s - r).abs() <= off).all())
+
+
+@pytest.mark.parametrize("copy", [False, True])
+@pytest.mark.parametrize("op", ["angular", "distill"])
+def test_rows_without_a_length(op, copy):
+    """Shorter than 2^-126: as rows of zeros. An infinity: NaN, in the row's loss and gradient alone, or (in a class) in all."""
+    N, D, V = 60, 64, 500
+    x, w, y, t, i = _cosine_problem(op, N, D, V, 4)
+    wt = torch.float32 if copy else torch.bfloat16
+
+    def run(x, w):
+        u, v = x.bfloat16().requires_grad_(), w.to(wt, copy=True).requires_grad_()
+        loss = _cosine_loss(op, u, v, y, t, i, "none")
+        return (loss.detach(),) + torch.autograd.grad(loss.sum(), (u, v))
+    tiny, zero = [x.clone(), w.clone()], [x.clone(), w.clone()]
+    for s, n in ((0, 5), (1, 9), (1, int(y[20]))):
+        tiny[s][n] = 2.0 ** -133 * torch.randint(-1, 2, (D,), device=DEV)
+        zero[s][n] = 0
+    assert bool(tiny[0].bfloat16()[5].any()) and all(torch.equal(p, q) for p, q in zip(run(*tiny), run(*zero)))
+    x[7, 3] = float("inf")
+    loss, dx, dw = run(x, w)
+    rows = torch.arange(N, device=DEV) == 7
+    assert torch.equal(loss.isnan(), rows) and torch.equal(dx.isnan().all(1), rows) and torch.equal(dx.isnan().any(1), rows) and bool(dw.isnan().all())
+    x[7, 3], w[400, 2] = 1.0, -float("inf")
+    assert all(bool(g.isnan().all()) for g in run(x, w)[:2])
