@@ -60,9 +60,9 @@ Saved saved_at(const na1d_head& h, const Shape& s, void* base) {
     return v;
 }
 
-// A piece of the classes has gradients of at most kPieceBytes, and at least four tiles. Smaller pieces would stay in L2, but cost more than that saves; larger
-// ones gain little for their memory. 32, 64, 128, 256, 512 MB in an earlier build: 2344, 2251, 1992, 2005, 1980 us a pass at
-// 8192 x 1024 x 50000; 381, 336, 323, 269, 306 at 4099 x 192 x 17982; 837, 729, 700, 650, 619 at 1024 x 256 x 200003.
+// A piece of the classes has gradients of at most kPieceBytes, or four tiles where those are more. Smaller pieces would stay in L2, but cost more than that
+// saves; larger ones gain little for their memory. 64, 128, 256, 512 MB: 3152, 3182, 3012, 3157 us a pass at 8192 x 1024 x 50000 (all rows counted);
+// 261, 203, 205, 204 at 4099 x 192 x 17982; 650, 639, 613, 592 at 1024 x 256 x 200003; 3458, 3028, 2870, 2767 at 6400 x 192 x 200000.
 constexpr int64_t kPieceBytes = 256ll << 20;
 // when the last pair is through with its items, in steps (as the products' kernel shares them out)
 static int64_t last_end(int64_t items_x, int64_t item_x, int64_t items_w, int64_t item_w, int64_t pairs) {
@@ -84,7 +84,8 @@ Pieces pieces_of(const Shape& s, bool want_x, bool want_w) {
     p.count = (p.tiles + most - 1) / most;
     p.piece_tiles = (p.tiles + p.count - 1) / p.count;
     p.count = (p.tiles + p.piece_tiles - 1) / p.piece_tiles;
-    if (p.piece_tiles > pairs && p.count > 1) {   // whole rounds of the pairs
+    // Whole rounds of the pairs, where the limit allows (6400 x 192 x 200000: 2870 us in pieces of 79 tiles, 2804 in ones of 148, which are 462 MB, 2915 in ones of 74).
+    if (p.piece_tiles > pairs && p.count > 1 && round_up(p.piece_tiles, pairs) <= most) {
         p.piece_tiles = round_up(p.piece_tiles, pairs);
         p.count = (p.tiles + p.piece_tiles - 1) / p.piece_tiles;
     }

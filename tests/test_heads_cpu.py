@@ -156,3 +156,12 @@ def test_where_the_weight_is_read(more, in_place):
     if in_place >= 0:
         dense = _head(**{**more, "weight": P, "weight_stride": 16, "weight_type": more.get("dtype", 0), "dim": 16, "dtype": 0, "x_type": 0, "weight_type": 0})
         assert (L.na1d_head_saved_bytes(ctypes.byref(h)) > L.na1d_head_saved_bytes(ctypes.byref(dense))) == (in_place == 0)
+
+
+@pytest.mark.parametrize("rows,classes", [(6400, 200000), (6912, 57500), (7000, 57344), (1024, 200003), (3500, 38000), (256, 1 << 20), (1 << 20, 6000), (3, 1 << 24)])
+def test_a_piece_stays_within_its_limit(rows, classes):
+    """8 channels, so that nothing else counts: 33 and 17 partial sums of them a row and a class of the piece."""
+    h = ctypes.byref(_head(rows=rows, dim=8, classes=classes, x_stride=8, weight_stride=8))
+    padded = (rows + 255) // 256 * 256
+    piece = max(256 << 20, padded * 1024 * 2)
+    assert L.na1d_head_backward_scratch(h, 1, 1) <= piece + 33 * 4 * 8 * padded + 17 * 4 * 8 * (piece // (2 * padded) + 256) + 4096
