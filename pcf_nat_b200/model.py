@@ -102,6 +102,8 @@ class AAMSoftmax(nn.Module):
     ``fused``: ``heads.angular_cross_entropy`` -- the same loss of 16-bit embeddings and weights (fp32 ones are rounded, to autocast's type or
     bfloat16) without the (rows, classes) cosines, for many rows or classes. The default computes in fp32 as before."""
 
+    fused = False      # (objects pickled whole before there was a choice have none of their own)
+
     def __init__(self, dim, classes, margin=0.2, scale=30.0, fused=False):
         super().__init__()
         self.weight = nn.Parameter(torch.randn(classes, dim) * 0.01)

@@ -32,3 +32,14 @@ def test_extractor_wiring_with_oracle_operator(monkeypatch):
     # every attention layer's bias received a gradient through the operator
     assert all(float(b.attn.relative_position_bias.grad.abs().sum()) > 0 for st in m.stages for b in st)
     assert model_flops_per_utterance() > 3e10
+
+
+def test_loss_modules_that_were_pickled_whole_before_they_had_a_fused_form():
+    """Such an object has no `fused` of its own: it computes as it did."""
+    from pcf_nat_b200.model import AAMSoftmax
+    torch.manual_seed(0)
+    m = AAMSoftmax(16, 30)
+    emb, y = torch.randn(5, 16), torch.randint(0, 30, (5,))
+    want = m(emb, y)
+    del m.__dict__["fused"]
+    assert torch.equal(m(emb, y), want)
