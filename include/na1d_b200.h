@@ -44,7 +44,7 @@ extern "C" {
 #define NA1D_ERR_BAD_DROPOUT (-12)   /* dropout probability outside [0,1) */
 #define NA1D_ERR_BAD_STRIDE (-11)    /* a stride is not a positive multiple of 8 elements, or the token stride is below C */
 
-#define NA1D_ERR_BAD_SCALE (-13)     /* a scale or temperature is not positive and finite, or a margin where there is none */
+#define NA1D_ERR_BAD_SCALE (-13)     /* a scale or temperature (or what comes of both) is not positive and finite, or a margin where there is none */
 
 #define NA1D_MAX_WINDOW 128 /* the reference asserts win <= 80, models/PCF_NATransformer.py:53 */
 

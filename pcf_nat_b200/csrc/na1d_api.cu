@@ -232,7 +232,7 @@ const char* na1d_status_string(int status) {
         case NA1D_ERR_UNSUPPORTED: return "the requested kernel family or tiling does not support this shape";
         case NA1D_ERR_BAD_DROPOUT: return "bad dropout probability: need 0 <= p < 1";
         case NA1D_ERR_BAD_STRIDE: return "bad stride: element strides must be positive multiples of 8, the token stride >= C";
-        case NA1D_ERR_BAD_SCALE: return "bad scale: scale and temperature have to be positive and finite, a margin needs normalised rows and labels";
+        case NA1D_ERR_BAD_SCALE: return "bad scale: scale, temperature, their ratio and product have to be positive and finite (2^-118 to 2^118), a margin needs normalised rows and labels";
         default: return "unknown status";
     }
 }

@@ -127,7 +127,14 @@ int check(const na1d_head* h) {
     if (h->x_stride < 0 || h->weight_stride < 0) return NA1D_ERR_BAD_STRIDE;
     if (h->reduction != NA1D_HEAD_MEAN && h->reduction != NA1D_HEAD_SUM && h->reduction != NA1D_HEAD_NONE) return NA1D_ERR_BAD_SHAPE;
     if (!(h->scale > 0.f) || !std::isfinite(h->scale) || !std::isfinite(h->margin)) return NA1D_ERR_BAD_SCALE;
-    if (h->top > 0 && (!(h->temperature > 0.f) || !std::isfinite(h->temperature))) return NA1D_ERR_BAD_SCALE;
+    if (!(h->scale < 0x1p118f)) return NA1D_ERR_BAD_SCALE;
+    if (h->top > 0) {
+        if (!(h->temperature > 0.f) || !std::isfinite(h->temperature)) return NA1D_ERR_BAD_SCALE;
+        // the factors of logits, gradients and losses are held in fp32
+        const double tau = h->temperature, factors[3] = {h->scale / tau, h->scale * tau, tau * tau};
+        for (double f : factors)
+            if (!(f > 0x1p-118 && f < 0x1p118)) return NA1D_ERR_BAD_SCALE;
+    }
     if ((h->top > 0 || !h->normalize) && h->margin != 0.f) return NA1D_ERR_BAD_SCALE;
     if (!h->x || !h->weight || (h->top ? !h->teacher_logits || !h->teacher_index : !h->labels)) return NA1D_ERR_NULL_POINTER;
     if (bad_align(h->x, h->x_type == NA1D_FP32 ? 4 : 2) || bad_align(h->weight, h->weight_type == NA1D_FP32 ? 4 : 2) || bad_align(h->labels, 8) ||

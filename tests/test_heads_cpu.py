@@ -165,3 +165,16 @@ def test_a_piece_stays_within_its_limit(rows, classes):
     padded = (rows + 255) // 256 * 256
     piece = max(256 << 20, padded * 1024 * 2)
     assert L.na1d_head_backward_scratch(h, 1, 1) <= piece + 33 * 4 * 8 * padded + 17 * 4 * 8 * (piece // (2 * padded) + 256) + 4096
+
+
+@pytest.mark.parametrize("more", [
+    dict(scale=1e-42), dict(scale=3e38), dict(scale=1e-20, temperature=1e18), dict(scale=1e20, temperature=1e-18), dict(temperature=1e19), dict(temperature=1e-19), dict(scale=1e25, temperature=1e15),
+])
+def test_scales_that_leave_fp32_together(more):
+    """Each is positive and finite; the factor of a logit, the gradient's or the squared temperature is not, or nearly."""
+    top = dict(top=3, teacher_logits=P, teacher_index=P)
+    assert L.na1d_head_saved_bytes(ctypes.byref(_head(**top, **more))) == -13
+    assert L.na1d_head_saved_bytes(ctypes.byref(_head(**top, scale=1e-10, temperature=1e10))) > 0
+    if "temperature" not in more:
+        assert (L.na1d_head_saved_bytes(ctypes.byref(_head(**more))) == -13) == (more["scale"] > 1)
+    assert L.na1d_head_saved_bytes(ctypes.byref(_head(temperature=math.nan))) > 0       # (labels have none)
