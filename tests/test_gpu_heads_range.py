@@ -171,3 +171,25 @@ def test_rows_without_a_length(op, copy):
     assert torch.equal(loss.isnan(), rows) and torch.equal(dx.isnan().all(1), rows) and torch.equal(dx.isnan().any(1), rows) and bool(dw.isnan().all())
     x[7, 3], w[400, 2] = 1.0, -float("inf")
     assert all(bool(g.isnan().all()) for g in run(x, w)[:2])
+
+
+@pytest.mark.parametrize("op", ["ce", "angular"])
+def test_tiny_factors_of_rows_in_fp16(op):
+    """Factors of 2^-130 give 2^-130 times the gradients of factors of 1, to the fp32 weight: half a step of 2^-149 off, and for its two roundings the same again."""
+    g = torch.Generator(device=DEV).manual_seed(6)
+    x, w = torch.randn(50, 64, device=DEV, generator=g).half(), torch.randn(300, 64, device=DEV, generator=g).half().float().requires_grad_()
+    y = torch.randint(0, 300, (50,), device=DEV, generator=g)
+    f = b200.linear_cross_entropy if op == "ce" else b200.angular_cross_entropy
+    (one,), (tiny,) = (torch.autograd.grad(f(x, w, y, reduction="none"), w, torch.full((50,), d, device=DEV)) for d in (1.0, 2.0 ** -130))
+    # Gradients of logits are relative to 2^-120 then, ten bits fewer: half a subnormal step is 2^-25 / 2^(14 - 10), or 2^-25 / 2^(5 - 10) of cosines. Those above
+    # are rounded in both, half a step of 2^-11 each. The projection at most doubles what lies along a class and adds it elsewhere: its length.
+    z, _, ix, iw, slope = orc.logits(x, w.detach(), 1.0 if op == "ce" else 30.0, op != "ce", y, 0.0 if op == "ce" else 0.2)
+    h = torch.softmax(z, 1)
+    h.scatter_(1, y[:, None], (h.gather(1, y[:, None]) - 1) * slope[:, None])
+    each = 2.0 ** -10 * h.abs() + (2.0 ** -29 if op == "ce" else 2.0 ** -20)
+    if op == "ce":
+        size = each.t() @ x.double().abs()
+    else:
+        size = 30 * iw[:, None] * (each.t() @ (x.double().abs() * ix[:, None]))
+        size = size + size.norm(dim=1, keepdim=True)
+    assert bool(torch.isfinite(tiny).all()) and bool(((tiny.double() * 2.0 ** 130 - one.double()).abs() <= size + 2.0 ** -149 * 2.0 ** 130).all())
