@@ -461,7 +461,7 @@ __global__ void __launch_bounds__(kThreads) combine_kernel(const __grid_constant
 }
 
 // ---------------------------------------------------------------- backward
-// factors of single rows' losses, side by side as the rows; fp16: relative to the largest (of 2^-120 at least: its inverse is a number), which follows
+// factors of single rows' losses, side by side as the rows; fp16: relative to the largest finite one (of 2^-120 at least: its inverse is a number), which follows
 // them. A probability times its row's factor keeps all digits down to 2^-28 of the largest factor (cosines: 2^-19 at a margin of 0.2).
 __global__ void __launch_bounds__(1024) coefficients_kernel(const float* __restrict__ d_loss, const Words* __restrict__ words, const int* __restrict__ row, long long Np,
                                                             bool relative, float* __restrict__ coef) {
@@ -470,13 +470,16 @@ __global__ void __launch_bounds__(1024) coefficients_kernel(const float* __restr
     const int counted = words->counted;
     float most = 0.f;
     if (relative) {
-        for (int c = threadIdx.x; c < counted; c += 1024) most = fmaxf(most, fabsf(d_loss[row[c]]));
+        for (int c = threadIdx.x; c < counted; c += 1024) {
+            const float f = fabsf(d_loss[row[c]]);
+            if (f < INFINITY) most = fmaxf(most, f);
+        }
         most = warp_max(most);
         if ((threadIdx.x & 31) == 0) most_s[threadIdx.x >> 5] = most;
         __syncthreads();
         most = warp_max(most_s[threadIdx.x & 31]);
     }
-    most = most > 0.f && most < INFINITY ? fmaxf(most, 0x1p-120f) : 1.f;
+    most = most > 0.f ? fmaxf(most, 0x1p-120f) : 1.f;
     const float r = 1.f / most;
     for (int c = threadIdx.x; c < counted; c += 1024) coef[c] = relative ? d_loss[row[c]] * r : d_loss[row[c]];
     if (threadIdx.x == 0) coef[Np] = most;

@@ -193,3 +193,22 @@ def test_tiny_factors_of_rows_in_fp16(op):
         size = 30 * iw[:, None] * (each.t() @ (x.double().abs() * ix[:, None]))
         size = size + size.norm(dim=1, keepdim=True)
     assert bool(torch.isfinite(tiny).all()) and bool(((tiny.double() * 2.0 ** 130 - one.double()).abs() <= size + 2.0 ** -149 * 2.0 ** 130).all())
+
+
+@pytest.mark.parametrize("op", ["ce", "angular"])
+@pytest.mark.parametrize("dtype", TYPES)
+def test_an_infinite_factor_is_its_row_s_alone(op, dtype):
+    """The other rows' gradients are those beside a factor of 0 there."""
+    g = torch.Generator(device=DEV).manual_seed(7)
+    x, w = torch.randn(50, 64, device=DEV, generator=g).requires_grad_(), torch.randn(300, 64, device=DEV, generator=g).to(dtype)
+    y = torch.randint(0, 300, (50,), device=DEV, generator=g)
+    f = b200.linear_cross_entropy if op == "ce" else b200.angular_cross_entropy
+    d = 65536.0 * torch.rand(50, device=DEV, generator=g)
+    got = []
+    for v in (0.0, float("inf")):
+        d[4] = v
+        with torch.autocast("cuda", dtype=dtype):
+            loss = f(x, w, y, reduction="none")
+        got.append(torch.autograd.grad(loss, x, d)[0])
+    rest = torch.arange(50, device=DEV) != 4
+    assert bool(torch.isfinite(got[0][rest]).all()) and torch.equal(got[0][rest], got[1][rest]) and not bool(torch.isfinite(got[1][4]).any())
