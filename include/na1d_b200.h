@@ -314,8 +314,8 @@ int na1d_stats_pool_backward(void* d_logits, void* dx, const float* d_out, const
  * of zeros (or shorter than 2^-126) has no direction: its cosines are 0 and its gradient is. One with an infinity is NaN. The mean is over rows that count, and 0 where none does.
  *
  * Products are of 16-bit values (dtype) with sums in fp32; fp32 rows or weights are rounded to dtype first, and their gradients are fp32. The
- * gradient of the logits is rounded to dtype once, before its products with weight and rows; everything else is held in fp32. No atomics
- * on results: the same bits from run to run. Nothing of a row that does not count is read by a product.
+ * gradient of the logits is rounded to dtype once, before its products with weight and rows; everything else is held in fp32. Sums have
+ * one order (an atomic addition comes once to a place in a launch): the same bits from run to run. Nothing of a row that does not count is read by a product.
  * ---------------------------------------------------------------------------------------- */
 #define NA1D_HEAD_MEAN 0
 #define NA1D_HEAD_SUM 1

@@ -52,6 +52,12 @@ __device__ __forceinline__ void wait_for_predecessor() {
     ptx::grid_launch_dependents();
 }
 
+__device__ __forceinline__ float exp2_fast(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
 constexpr int kTile = 256;            // rows and classes of a product tile (a pair of CTAs)
 constexpr int kPart = 64;             // classes that one partial maximum and sum stand for
 constexpr float kSineFloor = 2e-7f;   // of the squared sine in the margin's formula

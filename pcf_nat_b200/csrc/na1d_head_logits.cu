@@ -56,11 +56,6 @@ struct Args {
     float cs, up;
 };
 
-__device__ __forceinline__ float exp2_fast(float x) {
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
-}
 __device__ __forceinline__ float log2_fast(float x) {   // (2^-22 of the logarithm: less than 16 bits of a gradient show)
     float y;
     asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));

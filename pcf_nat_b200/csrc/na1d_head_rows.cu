@@ -19,11 +19,6 @@ __device__ __forceinline__ float warp_max(float v) {
     for (int o = 16; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
     return v;
 }
-__device__ __forceinline__ float exp2_fast(float x) {
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
-}
 
 __device__ __forceinline__ float power_of_two(int e) { return __int_as_float((127 + e) << 23); }   // -126 <= e <= 127
 template <typename E> __device__ __forceinline__ float squares(const uint4& v, float ss) {

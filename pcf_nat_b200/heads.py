@@ -2,16 +2,16 @@
 
 ``model.AAMSoftmax`` computes the extractor's loss as PyTorch does: fp32 cosines of every row and class, their softmax, both kept for the
 backward pass. With many rows (a label for every frame), many classes, or a vocabulary, these tensors are the largest of the
-whole step. Here the products run tile by tile on the tensor cores and leave only a maximum and a sum per row; the backward pass forms
-them again, a piece of the classes at a time, as 16-bit gradients that the products with weight and rows read next.
+whole step. Here the products run tile by tile on the tensor cores and leave a maximum and a sum per row and 64 classes (rows x classes / 8 bytes
+of workspace); the backward pass forms them again, a piece of the classes at a time, as 16-bit gradients that the products with weight and rows read next.
 
 * ``linear_cross_entropy``   softmax cross entropy of ``scale * x @ weight.T``
 * ``angular_cross_entropy``  of scaled cosines with an additive angular margin (AAM-softmax)
 * ``linear_distillation``    Kullback-Leibler divergence from a teacher's top logits
 
 ``x`` is bfloat16 or float16 (or, under autocast, float32, rounded to autocast's type), ``weight`` of the same type or float32 (then
-rounded to that type, as autocast does with a projection's; its gradient is float32). Rows may have any stride and number, ``dim`` and
-classes any size. Losses are float32.
+rounded to that type, as autocast does with a projection's; its gradient is float32). Rows may have any stride; there may be up to
+2^22 of them, of up to 2^14 channels, and 2^24 classes. Losses are float32.
 """
 import ctypes
 
@@ -192,7 +192,8 @@ def linear_cross_entropy(x, weight, labels, *, scale=1.0, ignore_index=-100, red
     ``x`` (..., dim), ``weight`` (classes, dim), ``labels`` (...) int64 or int32. Rows labelled ``ignore_index`` do not count: nothing in
     them reaches the loss or a gradient, and no time goes into them; where no row counts the mean is 0. A label outside the classes makes
     its row's loss, and the gradients that depend on it, NaN (there is no synchronisation to raise an error from). ``reduction``: "mean" over
-    the rows that count, "sum", or "none" (0 for the others). Differentiable once in ``x`` and ``weight``; same bits from run to run."""
+    the rows that count, "sum", or "none" (0 for the others; a float16 gradient of a logit is held relative to the largest factor of any row, and keeps all its digits
+    down to 2^-28 of it, of cosines 2^-19). Differentiable once in ``x`` and ``weight``; same bits from run to run."""
     _numbers(scale=scale, ignore_index=ignore_index)
     loss = None
     if _tensors(x, weight, labels):

@@ -462,3 +462,115 @@ def test_transforms_are_refused(op, python, monkeypatch):
         torch.func.vmap(lambda a: f(a, w, t))(torch.stack([x, x]))
     with pytest.raises(RuntimeError):
         torch.func.grad(lambda a: f(a, w, t))(x)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("reduction", ["mean", "none"])
+@pytest.mark.parametrize("scale", [33.2, 33.4, 64.0, 200.0])
+@pytest.mark.parametrize("op", ["angular", "distill"])
+def test_cosines_at_scales_with_a_running_maximum(op, scale, reduction, dtype):
+    """Scales up to 33.27 (2^48) stand for the maximum themselves, larger ones take it from the products; with and without a teacher."""
+    N, D, V, k = 150, 72, 700, 6
+    x, w, y, t, i = make(N, D, V, dtype, cosine=True, k=k)
+    w[11], x[9] = 0, 0                         # (a class and a row without a direction)
+    d = torch.linspace(0.25, 4, N, device=DEV) if reduction == "none" else 1.0
+    if op == "angular":
+        f = lambda x, w, y, reduction: b200.angular_cross_entropy(x, w, y, margin=0.2, scale=scale, reduction=reduction)  # noqa: E731
+        compare(f, x, w, (y,), dict(labels=y, scale=scale, margin=0.2, normalize=True), reduction, d)
+    else:
+        f = lambda x, w, t, i, reduction: b200.linear_distillation(x, w, t, i, scale=scale, normalize=True, reduction=reduction)  # noqa: E731
+        compare(f, x, w, (t, i), dict(teacher_logits=t, teacher_index=i, scale=scale, normalize=True), reduction, d)
+
+
+@pytest.mark.parametrize("cosine", [False, True])
+@pytest.mark.parametrize("N,k,V", [(40, 1024, 1500), (40, 1024, 1024), (300, 777, 2000), (9, 1000, 100)])
+def test_many_entries_of_a_teacher(N, k, V, cosine):
+    """As many as there may be; more than there are classes, so that each comes ten times."""
+    x, w, _, t, i = make(N, 64, V, torch.bfloat16, cosine=cosine, k=k)
+    i[::3, k // 2:] = -1
+    scale = 20.0 if cosine else 1.0
+    f = lambda x, w, t, i, reduction: b200.linear_distillation(x, w, t, i, temperature=2.0, scale=scale, normalize=cosine, reduction=reduction)  # noqa: E731
+    compare(f, x, w, (t, i), dict(teacher_logits=t, teacher_index=i, temperature=2.0, scale=scale, normalize=cosine))
+
+
+@pytest.mark.parametrize("op", ["ce", "angular", "distill"])
+@pytest.mark.parametrize("dtype", TYPES)
+def test_fp32_rows_and_weight_under_autocast(op, dtype):
+    """What the extractor passes: gradients in fp32, whose only 16-bit rounding is that of the logits' gradients. (The oracle rounds a result; here it is not.)"""
+    N, D, V = 200, 192, 900
+    x, w, y, t, i = make(N, D, V, dtype, cosine=op != "ce", k=8)
+    x1, w1 = x.float().requires_grad_(), w.float().requires_grad_()
+    with torch.autocast("cuda", dtype=dtype):
+        if op == "ce":
+            loss, o = b200.linear_cross_entropy(x1, w1, y), dict(labels=y)
+        elif op == "angular":
+            loss, o = b200.angular_cross_entropy(x1, w1, y), dict(labels=y, scale=30.0, margin=0.2, normalize=True)
+        else:
+            loss, o = b200.linear_distillation(x1, w1, t, i, scale=30.0, normalize=True), dict(teacher_logits=t, teacher_index=i, scale=30.0, normalize=True)
+    loss.backward()
+    r = orc.evaluate(x, w, **o)
+    near(loss.detach(), r["loss"], r["loss_off"] + 2 ** -22 * r["loss"].abs(), "loss")
+    near(x1.grad, r["dx"], orc.rounded(r["dx"], r["dx_off"], torch.float32), "dx")
+    near(w1.grad, r["dw"], orc.rounded(r["dw"], r["dw_off"], torch.float32), "dw")
+
+
+def test_offsets_beyond_32_bits():
+    """A weight of 2.2e9 elements, labels at both ends: the sums of all classes in pieces and in 64 bits; dx, and dw of the first and last classes. Bounds as the oracle's:
+    half a step of 2^-8 for each gradient of a logit and for the result, (D + 8) 2^-23 of a logit's terms, V / 64 2^-24 for the sum."""
+    N, D, V = 6, 192, 11_500_000
+    g = torch.Generator(device=DEV).manual_seed(0)
+    w = torch.empty(V, D, device=DEV, dtype=torch.bfloat16).normal_(generator=g).mul_(0.125).requires_grad_()
+    x = torch.randn(N, D, device=DEV, generator=g).bfloat16().requires_grad_()
+    y = torch.tensor([0, 1, V // 2, V - 3, V - 2, V - 1], device=DEV)
+    loss = b200.linear_cross_entropy(x, w, y, reduction="none")
+    dx, dw = torch.autograd.grad(loss.sum(), (x, w))
+    ops.device_status()
+    xd, parts, sums, sizes = x.detach().double(), [], torch.zeros(N, D, dtype=torch.float64, device=DEV), torch.zeros(N, D, dtype=torch.float64, device=DEV)
+    size = 0.0
+    for v in range(0, V, 500_000):
+        wd = w.detach()[v:v + 500_000].double()
+        z = xd @ wd.t()
+        size = max(size, float((xd.abs() @ wd.abs().t()).max()))
+        parts.append(torch.logsumexp(z, 1))
+        sums += torch.exp(z) @ wd             # (logits of some units: nothing overflows)
+        sizes += torch.exp(z) @ wd.abs()
+    lse = torch.logsumexp(torch.stack(parts), 0)
+    own = w.detach()[y].double()
+    off = 2 * ((D + 8) * 2.0 ** -23 * size + V / 64 * 2.0 ** -24)
+    assert bool(((loss.detach().double() - (lse - (xd * own).sum(1))).abs() <= off + 2.0 ** -22 * lse).all())
+    p = torch.exp(-lse)[:, None]
+    near(dx, sums * p - own, (2.0 ** -8 + off) * (sizes * p) + (off + 2.0 ** -20) * own.abs() + 2.0 ** -8 * (sums * p - own).abs(), "dx")
+    for v in (slice(0, 600), slice(V // 2 - 300, V // 2 + 300), slice(V - 600, V)):
+        G = torch.exp(xd @ w.detach()[v].double().t() - lse[:, None])
+        G = G - (torch.arange(V, device=DEV)[v] == y[:, None]).double()
+        ref = G.t() @ xd
+        near(dw[v], ref, (2.0 ** -8 + off) * (G.abs().t() @ xd.abs()) + 2.0 ** -8 * ref.abs(), "dw")
+
+
+@pytest.mark.parametrize("op", ["ce", "angular", "distill"])
+def test_calls_at_once(op):
+    """From several threads, each on a stream of its own: what one call gives."""
+    import threading
+    x, w, y, t, i = make(300, 96, 3000, torch.float16, cosine=op == "angular", k=5)
+    f = {"ce": lambda x, w: b200.linear_cross_entropy(x, w, y), "angular": lambda x, w: b200.angular_cross_entropy(x, w, y),
+         "distill": lambda x, w: b200.linear_distillation(x, w, t, i)}[op]
+
+    def step():
+        x1, w1 = x.detach().requires_grad_(), w.detach().requires_grad_()
+        loss = f(x1, w1)
+        return (loss.detach(),) + torch.autograd.grad(loss, (x1, w1))
+    want, got = step(), [None] * 4
+    torch.cuda.synchronize()
+
+    def work(n):
+        s = torch.cuda.Stream()
+        with torch.cuda.stream(s):
+            for _ in range(20):
+                got[n] = step()
+        s.synchronize()
+    threads = [threading.Thread(target=work, args=(n,)) for n in range(4)]
+    for th in threads:
+        th.start()
+    for th in threads:
+        th.join()
+    assert all(torch.equal(a, b) for g in got for a, b in zip(g, want))
