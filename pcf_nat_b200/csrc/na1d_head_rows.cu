@@ -28,44 +28,47 @@ template <typename E> __device__ __forceinline__ float squares(const uint4& v, f
     for (int k = 0; k < 8; ++k) ss = fmaf(f[k], f[k], ss);
     return ss;
 }
-// Inverse length of a row whose squares the lanes have. `up`: 2^up times the row has a length of 2^lift to twice that, and `kept` is 1 / its length then
+// Inverse length of a row. `up`: 2^up times the row has a length of 2^lift to twice that, and `kept` is 1 / its length then
 struct Length {
     float inverse, kept;
     int up;
 };
-// Squares outside fp32's range, or nearly: taken again of the row (`n` pieces) against its largest element. Rows of zeros, and ones shorter than 2^-126: all 0;
-// a row with an infinity or NaN has no length: NaN.
-template <typename E, typename Piece>
-__device__ __forceinline__ Length length_of(float ss, int lift, int n, Piece piece, int lane) {
-    ss = warp_sum(ss);
-    float inverse;
-    int less = 0;   // `inverse` is of the row times 2^-less
-    if (ss >= 0x1p-100f && ss <= 0x1p100f) {
-        inverse = rsqrtf(ss);
-    } else {
-        float f[8], most = 0.f, again = 0.f;
-        for (int j = lane; j < n; j += 32) {
-            Cvt<E>::unpack(piece(j), f);
-#pragma unroll
-            for (int k = 0; k < 8; ++k) most = fmaxf(most, fabsf(f[k]));
-        }
-        most = warp_max(most);
-        if (ss != ss || most == INFINITY) return Length{NAN, NAN, 0};
-        if (most == 0.f) return Length{0.f, 0.f, 0};
-        frexpf(most, &less);
-        for (int j = lane; j < n; j += 32) {
-            Cvt<E>::unpack(piece(j), f);
-#pragma unroll
-            for (int k = 0; k < 8; ++k) {
-                const float g = ldexpf(f[k], -less);
-                again = fmaf(g, g, again);
-            }
-        }
-        inverse = rsqrtf(warp_sum(again));
-    }
+// from an inverse length of the row times 2^-less
+__device__ __forceinline__ Length length_from(float inverse, int less, int lift) {
     const int e = ((__float_as_int(inverse) >> 23) & 255) - 126;   // inverse = m 2^e, m from 1/2 to 1: the length is 2^-e to twice that
-    if (e - less > 126) return Length{0.f, 0.f, 0};
-    return Length{less ? ldexpf(inverse, -less) : inverse, inverse * power_of_two(-e - lift), e - less + lift};
+    return Length{inverse, inverse * power_of_two(-e - lift), e - less + lift};
+}
+// Squares outside fp32's range, or nearly: taken again of the row against its largest element. Rows of zeros, and ones shorter than 2^-126: all 0; a row with an
+// infinity or NaN has no length: NaN. (A call of its own: inlined, it took 12 registers from the rows of ordinary length: 31.9 us instead of 26.1 at 1024 x 256 x 200003.)
+template <typename E>
+__device__ __noinline__ Length far_length(const void* src, int type, long long at, int D, int lift, int lane) {
+    float most = 0.f, ss = 0.f;
+    bool number = true;
+    auto element = [&](int j) { return (float)E(load_any(src, type, at + j)); };   // (fp32 rows are rounded first)
+    for (int j = lane; j < D; j += 32) {
+        const float f = fabsf(element(j));
+        number &= f < INFINITY;
+        most = fmaxf(most, f);
+    }
+    most = warp_max(most);
+    if (!__all_sync(0xffffffffu, number)) return Length{NAN, NAN, 0};
+    if (most == 0.f) return Length{0.f, 0.f, 0};
+    int less;
+    frexpf(most, &less);
+    for (int j = lane; j < D; j += 32) {
+        const float f = ldexpf(element(j), -less);
+        ss = fmaf(f, f, ss);
+    }
+    Length l = length_from(rsqrtf(warp_sum(ss)), less, lift);
+    if (l.up - lift > 126) return Length{0.f, 0.f, 0};
+    l.inverse = ldexpf(l.inverse, -less);
+    return l;
+}
+__device__ __forceinline__ bool has_squares(float ss) { return ss >= 0x1p-100f && ss <= 0x1p100f; }
+// of a row of D elements whose sum of squares is `ss`
+template <typename E>
+__device__ __forceinline__ Length length_of(float ss, const void* src, int type, long long at, int D, int lift, int lane) {
+    return has_squares(ss) ? length_from(rsqrtf(ss), 0, lift) : far_length<E>(src, type, at, D, lift, lane);
 }
 // eight elements times 2^l.up (in two steps: it may be beyond fp32); zeros, or NaN, where the row has no direction
 template <typename E> __device__ __forceinline__ uint4 kept_piece(const uint4& v, const Length& l) {
@@ -105,7 +108,7 @@ __device__ __forceinline__ Length copy_row(E* dst, const void* src, int type, lo
         last = piece(j);
         ss = squares<E>(last, ss);
     }
-    const Length l = length_of<E>(ss, lift, n, piece, lane);
+    const Length l = length_of<E>(warp_sum(ss), src, type, at, D, lift, lane);
     if (dst)
         for (int j = lane; j < n; j += 32) reinterpret_cast<uint4*>(dst)[j] = kept_piece<E>(n <= 32 ? last : piece(j), l);
     return l;
@@ -210,11 +213,17 @@ __global__ void __launch_bounds__(kThreads) prepare_kernel(const __grid_constant
 #pragma unroll
                 for (int i = 0; i < 4; ++i)
                     r[i] = lane < a.D / 8 ? __ldg(reinterpret_cast<const uint4*>(static_cast<const E*>(a.w) + (v + i * step) * a.w_stride) + lane) : make_uint4(0, 0, 0, 0);
+                float ss[4];
+                bool near = true;
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    const Length l = length_of<E>(squares<E>(r[i], 0.f), 0, a.D / 8, [&](int) { return r[i]; }, lane);
-                    if (lane == 0) a.iw[v + i * step] = l.inverse;
+                    ss[i] = warp_sum(squares<E>(r[i], 0.f));
+                    near &= has_squares(ss[i]);
                 }
+                if (!near) break;   // (one by one from here on)
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    if (lane == 0) a.iw[v + i * step] = rsqrtf(ss[i]);
             }
         }
         for (; v < a.V; v += step) {
