@@ -5,9 +5,9 @@
 // first product and across them for the second; w and x contract across their rows in both. The rows' results leave as
 // fp32 partial sums, one for each split of the contraction: the pieces' shares of dx are added up there in the order of the pieces. The weight's are
 // complete in a tile (unless there are too few tiles for the SMs) and leave as they are wanted.
-// Bound: at 1024 channels the tensor pipe, active 75 % of the cycles (8192 x 1024 x 50000, 6144 rows counted: 1007 us in four pieces, 1.25 PFLOP/s).
-// At 192 and 256 channels mostly memory, since both products read G: 4.4 and 5.2 TB/s from and to HBM, pipe active 45 % (4099 x 192 x 17982: 72 us;
-// 1024 x 256 x 200003: 237 us). One kernel for the gradient of the logits and the weight's, with G as an operand from tensor memory, gained nothing: it and the
+// Bound: at 1024 channels the tensor pipe, active 75 % of the cycles (8192 x 1024 x 50000, 6144 rows counted: 1007 to 1020 us in four pieces, 1.25 PFLOP/s).
+// At 192 and 256 channels mostly memory, since both products read G: 4.4 and 5.2 TB/s from and to HBM, pipe active 45 % (4099 x 192 x 17982: 72 to 74 us;
+// 1024 x 256 x 200003: 238 us). One kernel for the gradient of the logits and the weight's, with G as an operand from tensor memory, gained nothing: it and the
 // rows' products took 119 us where the two kernels take 126, and 390 where they take 375.
 #include "na1d_head.cuh"
 #include "na1d_mlp.cuh"

@@ -5,9 +5,9 @@
 // issues the products, and sixteen warps of each CTA read the accumulators back, a row per lane and a quarter of the columns, while the next tile's
 // products fill the other half of tensor memory.
 // The softmax's maximum and sum stay in 32 bits; the gradient is rounded to 16 bits once, as an operand of the products that follow.
-// Bound, forward: at 1024 channels the tensor pipe (8192 x 1024 x 50000, 6144 rows counted: 372 to 386 us, 1.6 to 1.7 PFLOP/s, pipe active 97 % of the
+// Bound, forward: at 1024 channels the tensor pipe (8192 x 1024 x 50000, 6144 rows counted: 372 to 391 us, 1.6 to 1.7 PFLOP/s, pipe active 97 % of the
 // cycles at 1.53 GHz). At 192 and 256 channels a 256 x 256 tile takes 4400 and 4000 SM cycles where its products take 1536 and 2048 and its exponentials
-// 2048 (4099 x 192 x 17982: 40 us; 1024 x 256 x 200003: 98 us). In an earlier build the tile lost a tenth without exponentials, and a quarter without the epilogue.
+// 2048 (4099 x 192 x 17982: 41 us; 1024 x 256 x 200003: 98 to 103 us). In an earlier build the tile lost a tenth without exponentials, and a quarter without the epilogue.
 // Bound, gradient: the epilogue, 5700 to 5800 cycles a tile there (54 us; 137 us in two pieces), of which that build lost half without it and 2 % without
 // exponentials; at 1024 channels the pipe is active 75 % of the cycles (458 us in four pieces).
 #include "na1d_head.cuh"

@@ -1,6 +1,6 @@
 // The passes around the products of a head's losses: each reads its inputs once, a warp to a row or a class. prepare, combine and finish are 4 % of the kernels' time
-// at 8192 x 1024 x 50000 (13, 17 and 46 us) and a sixth at 4099 x 192 x 17982 (7, 9 and 17 us); at 1024 x 256 x 200003 the weight's lengths take prepare 24 us
-// where its 102 MB need 16.
+// at 8192 x 1024 x 50000 (12, 16 and 43 us) and a sixth at 4099 x 192 x 17982 (9, 9 and 15 us); at 1024 x 256 x 200003 the weight's lengths take prepare 25 us
+// where its 102 MB need 16, and in fp16, with the copy that its powers of two need, a pass takes 621 us instead of 585.
 #include "na1d_head.cuh"
 
 namespace na1d {
